@@ -8,6 +8,7 @@
 #include <string>
 
 #include "../../include/spnc_hip.h"
+#include "guard.h"
 #include "kernel.h"
 
 #include "interp_kernel.h"
@@ -19,22 +20,10 @@ struct spnc_hip_kernel {
 
 namespace {
 thread_local std::string g_lastError;
-
-template <typename Fn>
-int guarded(Fn&& fn) {
-  try {
-    g_lastError.clear();
-    fn();
-    return 0;
-  } catch (const std::exception& e) {
-    g_lastError = e.what();
-    return 1;
-  } catch (...) {
-    g_lastError = "unknown error";
-    return 1;
-  }
 }
-}  // namespace
+
+std::string& spnc_hip::lastError() { return g_lastError; }
+using spnc_hip::guarded;
 
 extern "C" {
 

@@ -1,0 +1,932 @@
+// Operators on device-resident rows around compiled kernels (include/spnc_hip_rows.h): gate, routing, combination,
+// dropout. Device code, launch shapes and the extern "C" entry points.
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+#include <stdexcept>
+#include <string>
+#include <type_traits>
+
+#include "../../include/spnc_hip_rows.h"
+#include "guard.h"
+#include "philox.h"
+
+namespace spnc_hip {
+namespace {
+
+constexpr unsigned WAVE = 64;
+constexpr unsigned BLOCK = 256;
+constexpr unsigned XCDS = 8;             // blocks go to the chip's dies in turn
+constexpr size_t MAX_GRID = 1u << 22;    // a launch must stay below 2^32 threads
+
+template <typename T> struct Wide { using type = float; };
+template <> struct Wide<double> { using type = double; };
+template <typename T> using wide_t = typename Wide<T>::type;
+
+template <typename T, int N>
+struct alignas(sizeof(T) * N) Pack {
+  T v[N];
+};
+
+// Neighbouring tiles of rows go to one die: rows that are neighbours in the sorted buffer come from neighbouring rows,
+// and a cache line of narrow rows is then filled or read within one L2.
+template <typename Body>
+__device__ inline void forTiles(size_t tiles, Body&& body) {
+  const size_t perDie = (tiles + XCDS - 1) / XCDS, first = size_t(blockIdx.x % XCDS) * perDie;
+  for (size_t t = blockIdx.x / XCDS; t < perDie; t += gridDim.x / XCDS)
+    if (first + t < tiles) body(first + t);
+}
+
+unsigned tileGrid(size_t tiles) {
+  const size_t g = (tiles + XCDS - 1) / XCDS * XCDS;
+  return unsigned(g < MAX_GRID ? g : MAX_GRID);
+}
+
+// ---- gate -----------------------------------------------------------------------------------------------------------
+
+// Unsigned keys in the order of the values: NaN above everything, both zeros the same, 0 for "no value".
+template <typename R> struct Order;
+template <> struct Order<float> {
+  using key = uint32_t;
+  __device__ static key of(float x) {
+    const uint32_t u = __float_as_uint(x + 0.0f);
+    return x != x ? 0xFFFFFFFFu : (u & 0x80000000u) ? ~u : u | 0x80000000u;
+  }
+  __device__ static float value(key k) {
+    return k == 0xFFFFFFFFu ? __uint_as_float(0x7FC00000u) : __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
+  }
+  static constexpr key closed = 0x007FFFFFu;  // of minus infinity
+};
+template <> struct Order<double> {
+  using key = uint64_t;
+  __device__ static key of(double x) {
+    const uint64_t u = uint64_t(__double_as_longlong(x + 0.0));
+    return x != x ? ~0ull : (u >> 63) ? ~u : u | (1ull << 63);
+  }
+  __device__ static double value(key k) {
+    if (k == ~0ull) return __longlong_as_double(0x7FF8000000000000ll);
+    return __longlong_as_double((long long)((k >> 63) ? k ^ (1ull << 63) : ~k));
+  }
+  static constexpr key closed = 0x000FFFFFFFFFFFFFull;
+};
+
+template <int G, typename R>
+__device__ inline R groupSum(R x) {
+#pragma unroll
+  for (int d = 1; d < G; d *= 2) x += __shfl_xor(x, d);
+  return x;
+}
+
+template <int G, typename R>
+__device__ inline R groupMax(R x) {
+#pragma unroll
+  for (int d = 1; d < G; d *= 2) {
+    const R y = __shfl_xor(x, d);
+    x = y > x ? y : x;
+  }
+  return x;
+}
+
+// G lanes hold a row, V logits each; k rounds of a maximum over the group, lane j keeps the choice of round j.
+template <typename T, int G, int V>
+__global__ __launch_bounds__(BLOCK) void gateKernel(const T* __restrict__ logits, size_t n, unsigned experts, size_t stride, unsigned k,
+                                                    unsigned flags, int32_t* __restrict__ index, wide_t<T>* __restrict__ weight) {
+  using R = wide_t<T>;
+  using O = Order<R>;
+  using K = typename O::key;
+  const unsigned lane = threadIdx.x % G;
+  forTiles((n + BLOCK / G - 1) / (BLOCK / G), [&](size_t tile) {
+    const size_t row = tile * (BLOCK / G) + threadIdx.x / G;
+    if (row >= n) return;  // whole groups leave; shuffles stay inside a group
+    K key[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const unsigned e = i * G + lane;
+      key[i] = e < experts ? O::of(R(logits[row * stride + e])) : K(0);
+    }
+    K myKey = 0, topKey = 0;
+    unsigned myIndex = 0;
+    R total = 0;
+    for (unsigned j = 0; j < k; ++j) {
+      K best = 0;
+      unsigned at = 0;
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (key[i] > best) best = key[i], at = i * G + lane;
+#pragma unroll
+      for (int d = 1; d < G; d *= 2) {
+        const K otherKey = __shfl_xor(best, d);
+        const unsigned otherAt = __shfl_xor(at, d);
+        if (otherKey > best || (otherKey == best && otherAt < at)) best = otherKey, at = otherAt;
+      }
+      if (j == 0) {
+        topKey = best;
+        if ((flags & SPNC_HIP_GATE_ALL) && best > O::closed) {
+          const R top = O::value(best);
+#pragma unroll
+          for (int i = 0; i < V; ++i)
+            if (key[i] > O::closed) total += std::is_same<R, double>::value ? R(exp(double(O::value(key[i]) - top))) : R(expf(float(O::value(key[i]) - top)));
+          total = groupSum<G>(total);
+        }
+      }
+      if (lane == j) myKey = best, myIndex = at;
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (unsigned(i * G) + lane == at) key[i] = 0;
+    }
+    const bool open = lane < k && myKey > O::closed;
+    const R top = O::value(topKey), mine = O::value(myKey);
+    const R shifted = open ? mine - top : R(0);
+    const R e = open ? (std::is_same<R, double>::value ? R(exp(double(shifted))) : R(expf(float(shifted)))) : R(0);
+    if (!(flags & SPNC_HIP_GATE_ALL)) total = groupSum<G>(e);
+    if (lane < k) {
+      index[row * k + lane] = open ? int32_t(myIndex) : -1;
+      R w;
+      if (flags & SPNC_HIP_GATE_LOG) {
+        const R l = std::is_same<R, double>::value ? R(log(double(total))) : R(logf(float(total)));
+        w = open ? shifted - l : -INFINITY;
+      } else {
+        w = open ? e / total : R(0);
+      }
+      weight[row * k + lane] = w;
+    }
+  });
+}
+
+template <typename T, int G, int V>
+__global__ __launch_bounds__(BLOCK) void gateBackwardKernel(const T* __restrict__ logits, size_t n, unsigned experts, size_t stride, unsigned k,
+                                                            unsigned flags, const int32_t* __restrict__ index, const wide_t<T>* __restrict__ weight,
+                                                            const wide_t<T>* __restrict__ gradWeight, T* __restrict__ gradLogits) {
+  using R = wide_t<T>;
+  const unsigned lane = threadIdx.x % G;
+  const bool all = flags & SPNC_HIP_GATE_ALL, logs = flags & SPNC_HIP_GATE_LOG;
+  forTiles((n + BLOCK / G - 1) / (BLOCK / G), [&](size_t tile) {
+    const size_t row = tile * (BLOCK / G) + threadIdx.x / G;
+    if (row >= n) return;
+    R share[V];  // of the experts, under "all"
+    R total = 0;
+    if (all) {
+      R z[V], top = -INFINITY;
+      bool bad = false;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        const unsigned e = i * G + lane;
+        z[i] = e < experts ? R(logits[row * stride + e]) : R(-INFINITY);
+        bad |= z[i] != z[i];
+        top = z[i] > top ? z[i] : top;
+      }
+      top = groupMax<G>(top);
+      if (groupMax<G>(int(bad))) top = NAN;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        share[i] = z[i] == -INFINITY ? R(0) : std::is_same<R, double>::value ? R(exp(double(z[i] - top))) : R(expf(float(z[i] - top)));
+        total += share[i];
+      }
+      total = groupSum<G>(total);
+    }
+    int32_t at = -1;
+    R d = 0, w = 0;
+    if (lane < k) {
+      at = index[row * k + lane];
+      if (at >= 0) {
+        d = gradWeight[row * k + lane];
+        w = weight[row * k + lane];
+        if (logs) w = std::is_same<R, double>::value ? R(exp(double(w))) : R(expf(float(w)));
+        else d *= w;
+      }
+    }
+    const R common = groupSum<G>(d);
+    if (!all && at >= 0) d -= w * common;
+    R dz[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) dz[i] = all && total > 0 ? -(share[i] / total) * common : all && total != total ? total : R(0);
+    for (unsigned j = 0; j < k; ++j) {
+      const int32_t target = __shfl(at, int(j), G);
+      const R value = __shfl(d, int(j), G);
+#pragma unroll
+      for (int i = 0; i < V; ++i)
+        if (target == int32_t(i * G + lane)) dz[i] += value;
+    }
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      const unsigned e = i * G + lane;
+      if (e < experts) gradLogits[row * experts + e] = T(dz[i]);
+    }
+  });
+}
+
+// ---- routing --------------------------------------------------------------------------------------------------------
+
+constexpr unsigned ROUTE_BLOCK = 1024, ROUTE_WAVES = ROUTE_BLOCK / WAVE, ROUTE_MAX_BLOCKS = 256;
+constexpr size_t ROUTE_SINGLE = 8192;  // slots one block sorts by itself
+
+struct RouteShape {
+  size_t chunk;     // slots a block sorts, a multiple of ROUTE_BLOCK
+  unsigned blocks;
+};
+
+RouteShape routeShape(size_t slots) {
+  if (slots <= ROUTE_SINGLE) return {(slots + ROUTE_BLOCK - 1) / ROUTE_BLOCK * ROUTE_BLOCK, 1};
+  size_t blocks = (slots + 4 * ROUTE_BLOCK - 1) / (4 * ROUTE_BLOCK);
+  if (blocks > ROUTE_MAX_BLOCKS) blocks = ROUTE_MAX_BLOCKS;
+  const size_t chunk = ((slots + blocks - 1) / blocks + ROUTE_BLOCK - 1) / ROUTE_BLOCK * ROUTE_BLOCK;
+  return {chunk, unsigned((slots + chunk - 1) / chunk)};
+}
+
+// Lanes of the wave that hold the same expert, found by one vote per bit of the expert number.
+__device__ inline uint64_t sameExpert(bool routed, uint32_t expert, unsigned bits) {
+  uint64_t same = __ballot(routed);
+  for (unsigned b = 0; b < bits; ++b) {
+    const bool one = (expert >> b) & 1;
+    const uint64_t votes = __ballot(one);
+    same &= one ? votes : ~votes;
+  }
+  return same;
+}
+
+// counter[wave][expert] of this block's slots; every wave sorts a contiguous part of the chunk.
+__device__ inline void countSlots(const int32_t* index, size_t begin, size_t end, unsigned experts, unsigned bits, uint32_t* counter) {
+  const unsigned lane = threadIdx.x % WAVE;
+  for (size_t s = begin; s < end; s += WAVE) {
+    const size_t slot = s + lane;
+    const uint32_t e = slot < end ? uint32_t(index[slot]) : ~0u;
+    const bool routed = e < experts;
+    const uint64_t same = sameExpert(routed, e, bits);
+    if (routed && __ffsll((unsigned long long)same) - 1 == int(lane)) atomicAdd(&counter[e], uint32_t(__popcll(same)));
+  }
+}
+
+__global__ __launch_bounds__(ROUTE_BLOCK) void routeCountKernel(const int32_t* __restrict__ index, size_t slots, unsigned experts, unsigned bits,
+                                                                size_t chunk, uint32_t* __restrict__ counts) {
+  extern __shared__ uint32_t routeLds[];  // [experts]
+  for (unsigned e = threadIdx.x; e < experts; e += ROUTE_BLOCK) routeLds[e] = 0;
+  __syncthreads();
+  const size_t begin = blockIdx.x * chunk + threadIdx.x / WAVE * (chunk / ROUTE_WAVES);
+  size_t end = begin + chunk / ROUTE_WAVES;
+  if (end > slots) end = slots;
+  countSlots(index, begin, end, experts, bits, routeLds);
+  __syncthreads();
+  for (unsigned e = threadIdx.x; e < experts; e += ROUTE_BLOCK) counts[size_t(blockIdx.x) * experts + e] = routeLds[e];
+}
+
+// blockCounts [gridDim.x][experts] of routeCountKernel; unused by a single block.
+__global__ __launch_bounds__(ROUTE_BLOCK) void routeKernel(const int32_t* __restrict__ index, size_t slots, unsigned experts, unsigned bits,
+                                                           unsigned align, size_t chunk, const uint32_t* __restrict__ blockCounts,
+                                                           int32_t* __restrict__ position, int32_t* __restrict__ starts, int32_t* __restrict__ counts) {
+  extern __shared__ uint32_t routeLds[];  // counter[ROUTE_WAVES][experts]
+  __shared__ uint32_t waveSum[ROUTE_WAVES];
+  const unsigned t = threadIdx.x, lane = t % WAVE, wave = t / WAVE;
+  for (unsigned i = t; i < ROUTE_WAVES * experts; i += ROUTE_BLOCK) routeLds[i] = 0;
+  __syncthreads();
+  const size_t begin = blockIdx.x * chunk + wave * (chunk / ROUTE_WAVES);
+  size_t end = begin + chunk / ROUTE_WAVES;
+  if (end > slots) end = slots;
+  countSlots(index, begin, end, experts, bits, routeLds + wave * experts);
+  __syncthreads();
+  // thread e: this block's total of expert e, what earlier blocks hold of it, and the total of all blocks
+  uint32_t before = 0, all = 0;
+  if (t < experts) {
+    if (gridDim.x == 1) {
+      for (unsigned w = 0; w < ROUTE_WAVES; ++w) all += routeLds[w * experts + t];
+    } else {
+      for (unsigned b = 0; b < gridDim.x; ++b) {
+        const uint32_t c = blockCounts[size_t(b) * experts + t];
+        all += c;
+        if (b < blockIdx.x) before += c;
+      }
+    }
+  }
+  // where each segment starts: an exclusive scan of the totals, rounded up
+  const uint32_t rounded = (all + (align - 1)) / align * align;
+  uint32_t scan = rounded;
+  for (unsigned d = 1; d < WAVE; d *= 2) {
+    const uint32_t below = __shfl_up(scan, d);
+    if (lane >= d) scan += below;
+  }
+  if (lane == WAVE - 1) waveSum[wave] = scan;
+  __syncthreads();
+  uint32_t start = scan - rounded;
+  for (unsigned w = 0; w < wave; ++w) start += waveSum[w];
+  if (t < experts) {
+    if (blockIdx.x == 0) {
+      starts[t] = int32_t(start);
+      counts[t] = int32_t(all);
+      if (t == experts - 1) starts[experts] = int32_t(start + rounded);
+    }
+    uint32_t next = start + before;
+    for (unsigned w = 0; w < ROUTE_WAVES; ++w) {
+      const uint32_t c = routeLds[w * experts + t];
+      routeLds[w * experts + t] = next;
+      next += c;
+    }
+  }
+  __syncthreads();
+  uint32_t* counter = routeLds + wave * experts;
+  for (size_t s = begin; s < end; s += WAVE) {
+    const size_t slot = s + lane;
+    const uint32_t e = slot < end ? uint32_t(index[slot]) : ~0u;
+    const bool routed = e < experts;
+    const uint64_t same = sameExpert(routed, e, bits);
+    const int leader = __ffsll((unsigned long long)same) - 1;
+    uint32_t base = 0;
+    if (routed && leader == int(lane)) base = atomicAdd(&counter[e], uint32_t(__popcll(same)));
+    base = __shfl(base, routed ? leader : int(lane));
+    if (slot < end) position[slot] = routed ? int32_t(base + __popcll(same & ((1ull << lane) - 1))) : -1;
+  }
+}
+
+// ---- rows there and back --------------------------------------------------------------------------------------------
+
+// A group of 2^shift lanes handles a row, a piece of up to 16 bytes a lane at a time.
+struct RowShape {
+  unsigned pieces;  // of a row
+  unsigned shift;
+  size_t tiles;
+};
+
+RowShape rowShape(size_t n, size_t rowBytes, unsigned pieceBytes) {
+  RowShape s;
+  s.pieces = unsigned(rowBytes / pieceBytes);
+  s.shift = 0;
+  while (s.shift < 6 && (1u << s.shift) < s.pieces) ++s.shift;
+  const size_t rows = BLOCK >> s.shift;
+  s.tiles = (n + rows - 1) / rows;
+  return s;
+}
+
+// Rows of the sorted buffer that belong to no segment, cleared by the blocks behind the first `rowBlocks`: a wave for
+// every segment's end, and all of them for what follows the last one.
+__device__ inline void clearUnused(unsigned block, unsigned blocks, const int32_t* starts, const int32_t* counts, unsigned experts,
+                                   size_t capacity, size_t rowBytes, unsigned char* out) {
+  const unsigned lane = threadIdx.x % WAVE;
+  const size_t wave = size_t(block) * (BLOCK / WAVE) + threadIdx.x / WAVE, waves = size_t(blocks) * (BLOCK / WAVE);
+  auto clear = [&](size_t from, size_t to, size_t first, size_t step) {  // bytes; pointers may have any alignment
+    if (((reinterpret_cast<uintptr_t>(out) | from | to) & 3) == 0) {
+      uint32_t* words = reinterpret_cast<uint32_t*>(out);
+      for (size_t i = from / 4 + first; i < to / 4; i += step) words[i] = 0;
+    } else {
+      for (size_t i = from + first; i < to; i += step) out[i] = 0;
+    }
+  };
+  for (size_t e = wave; e < experts; e += waves) {
+    size_t from = size_t(starts[e]) + size_t(counts[e]), to = size_t(starts[e + 1]);
+    if (to > capacity) to = capacity;
+    if (from < to) clear(from * rowBytes, to * rowBytes, lane, WAVE);
+  }
+  const size_t end = size_t(starts[experts]);
+  if (end < capacity) clear(end * rowBytes, capacity * rowBytes, wave * WAVE + lane, waves * WAVE);
+}
+
+unsigned clearBlocks(size_t capacity, size_t rowBytes) {
+  const size_t b = capacity * rowBytes / 65536 + 1;
+  return unsigned(b < 256 ? b : 256);
+}
+
+template <typename P>
+__global__ __launch_bounds__(BLOCK) void dispatchKernel(const unsigned char* __restrict__ rows, size_t n, size_t strideBytes, RowShape shape,
+                                                        const int32_t* __restrict__ position, unsigned k, size_t capacity, P* __restrict__ out) {
+  const unsigned lane = threadIdx.x & ((1u << shape.shift) - 1);
+  forTiles(shape.tiles, [&](size_t tile) {
+    const size_t row = tile * (BLOCK >> shape.shift) + (threadIdx.x >> shape.shift);
+    if (row >= n) return;
+    const P* source = reinterpret_cast<const P*>(rows + row * strideBytes);
+    for (unsigned c = lane; c < shape.pieces; c += 1u << shape.shift) {
+      const P piece = source[c];
+      for (unsigned j = 0; j < k; ++j) {
+        const int32_t to = position[row * k + j];
+        if (to >= 0 && size_t(to) < capacity) out[size_t(to) * shape.pieces + c] = piece;
+      }
+    }
+  });
+}
+
+__global__ __launch_bounds__(BLOCK) void clearKernel(const int32_t* __restrict__ starts, const int32_t* __restrict__ counts, unsigned experts,
+                                                     size_t capacity, size_t rowBytes, unsigned char* __restrict__ out) {
+  clearUnused(blockIdx.x, gridDim.x, starts, counts, experts, capacity, rowBytes, out);
+}
+
+template <typename T, int N, typename W>
+__global__ __launch_bounds__(BLOCK) void combineKernel(const T* __restrict__ values, size_t capacity, size_t stride, RowShape shape,
+                                                       const int32_t* __restrict__ position, size_t n, unsigned k, const W* __restrict__ weight,
+                                                       Pack<T, N>* __restrict__ out) {
+  using R = wide_t<T>;
+  const unsigned lane = threadIdx.x & ((1u << shape.shift) - 1);
+  forTiles(shape.tiles, [&](size_t tile) {
+    const size_t row = tile * (BLOCK >> shape.shift) + (threadIdx.x >> shape.shift);
+    if (row >= n) return;
+    for (unsigned c = lane; c < shape.pieces; c += 1u << shape.shift) {
+      R sum[N] = {};
+      for (unsigned j = 0; j < k; ++j) {
+        const int32_t at = position[row * k + j];
+        if (at < 0 || size_t(at) >= capacity) continue;
+        const R w = weight ? R(weight[row * k + j]) : R(1);
+        const Pack<T, N> v = *reinterpret_cast<const Pack<T, N>*>(values + size_t(at) * stride + size_t(c) * N);
+#pragma unroll
+        for (int i = 0; i < N; ++i) sum[i] += w * R(v.v[i]);
+      }
+      Pack<T, N> o;
+#pragma unroll
+      for (int i = 0; i < N; ++i) o.v[i] = T(sum[i]);
+      out[row * shape.pieces + c] = o;
+    }
+  });
+}
+
+template <typename T, int N, typename W>
+__global__ __launch_bounds__(BLOCK) void combineBackwardKernel(const T* __restrict__ values, size_t capacity, size_t stride, RowShape shape,
+                                                               const int32_t* __restrict__ position, size_t n, unsigned k,
+                                                               const W* __restrict__ weight, const T* __restrict__ gradOut, size_t gradStride,
+                                                               Pack<T, N>* __restrict__ gradValues, W* __restrict__ gradWeight) {
+  using R = wide_t<T>;
+  const unsigned group = 1u << shape.shift, lane = threadIdx.x & (group - 1);
+  forTiles(shape.tiles, [&](size_t tile) {
+    const size_t row = tile * (BLOCK >> shape.shift) + (threadIdx.x >> shape.shift);
+    if (row >= n) return;
+    for (unsigned j = 0; j < k; ++j) {
+      const int32_t at = position[row * k + j];
+      const bool routed = at >= 0 && size_t(at) < capacity;
+      R dot = 0;
+      if (routed) {
+        const R w = weight ? R(weight[row * k + j]) : R(1);
+        for (unsigned c = lane; c < shape.pieces; c += group) {
+          const Pack<T, N> g = *reinterpret_cast<const Pack<T, N>*>(gradOut + row * gradStride + size_t(c) * N);
+          if (gradWeight) {
+            const Pack<T, N> v = *reinterpret_cast<const Pack<T, N>*>(values + size_t(at) * stride + size_t(c) * N);
+#pragma unroll
+            for (int i = 0; i < N; ++i) dot += R(g.v[i]) * R(v.v[i]);
+          }
+          if (gradValues) {
+            Pack<T, N> o;
+#pragma unroll
+            for (int i = 0; i < N; ++i) o.v[i] = T(w * R(g.v[i]));
+            gradValues[size_t(at) * shape.pieces + c] = o;
+          }
+        }
+      }
+      if (gradWeight) {
+        for (unsigned d = 1; d < group; d *= 2) dot += __shfl_xor(dot, int(d));
+        if (lane == 0) gradWeight[row * k + j] = W(dot);
+      }
+    }
+  });
+}
+
+// The largest value of the row's slots is taken out before its log weight is added: values of some thousands differ by
+// little, and the difference is exact where the sum would be rounded. Shares are computed from the same terms, not from the
+// rounded result.
+template <typename R, typename W>
+struct LogTerms {
+  const R* values;
+  size_t capacity;
+  const int32_t* position;
+  const W* logWeight;
+  // false: the slot is left out
+  __device__ bool slot(size_t s, R& value, R& lw) const {
+    const int32_t at = position[s];
+    if (at < 0 || size_t(at) >= capacity) return false;
+    lw = R(logWeight[s]);
+    if (lw == -INFINITY) return false;
+    value = values[at];
+    return true;
+  }
+};
+
+template <typename R> __device__ inline R expOf(R x) { return std::is_same<R, double>::value ? R(exp(double(x))) : R(expf(float(x))); }
+template <typename R> __device__ inline R logOf(R x) { return std::is_same<R, double>::value ? R(log(double(x))) : R(logf(float(x))); }
+
+// peak: the largest value; shift: the largest log weight + (value - peak); total: sum of exp(that - shift)
+template <typename R, typename W>
+__device__ inline void logSum(const LogTerms<R, W>& terms, size_t row, unsigned k, R& peak, R& shift, R& total) {
+  peak = -INFINITY;
+  R v, lw;
+  for (unsigned j = 0; j < k; ++j)
+    if (terms.slot(row * k + j, v, lw)) peak = v > peak || v != v ? v : peak;
+  shift = -INFINITY;
+  total = 0;
+  if (!(peak > -INFINITY) && peak == peak) return;  // nothing possible
+  for (unsigned j = 0; j < k; ++j)
+    if (terms.slot(row * k + j, v, lw)) {
+      const R t = lw + (v - peak);
+      shift = t > shift || t != t ? t : shift;
+    }
+  for (unsigned j = 0; j < k; ++j)
+    if (terms.slot(row * k + j, v, lw)) total += expOf<R>(lw + (v - peak) - shift);
+}
+
+template <typename R, typename W>
+__global__ __launch_bounds__(BLOCK) void combineLogKernel(LogTerms<R, W> terms, size_t n, unsigned k, R* __restrict__ out) {
+  forTiles((n + BLOCK - 1) / BLOCK, [&](size_t tile) {
+    const size_t row = tile * BLOCK + threadIdx.x;
+    if (row >= n) return;
+    R peak, shift, total;
+    logSum(terms, row, k, peak, shift, total);
+    out[row] = peak == -INFINITY || peak == INFINITY ? peak : peak + (shift + logOf<R>(total));
+  });
+}
+
+template <typename R, typename W>
+__global__ __launch_bounds__(BLOCK) void combineLogBackwardKernel(LogTerms<R, W> terms, size_t n, unsigned k, const R* __restrict__ gradOut,
+                                                                  R* __restrict__ gradValues, W* __restrict__ gradLogWeight) {
+  forTiles((n + BLOCK - 1) / BLOCK, [&](size_t tile) {
+    const size_t row = tile * BLOCK + threadIdx.x;
+    if (row >= n) return;
+    R peak, shift, total;
+    logSum(terms, row, k, peak, shift, total);
+    const R g = gradOut[row];
+    for (unsigned j = 0; j < k; ++j) {
+      const size_t s = row * k + j;
+      R v, lw, share = 0;
+      if (peak != -INFINITY && terms.slot(s, v, lw)) share = g * (expOf<R>(lw + (v - peak) - shift) / total);
+      const int32_t at = terms.position[s];
+      if (gradValues && at >= 0 && size_t(at) < terms.capacity) gradValues[at] = share;
+      if (gradLogWeight) gradLogWeight[s] = W(share);
+    }
+  });
+}
+
+// ---- dropout --------------------------------------------------------------------------------------------------------
+
+template <typename T>
+__global__ __launch_bounds__(BLOCK) void dropoutKernel(const T* x, size_t n, size_t width, size_t stride, T* out, size_t outStride,
+                                                       uint64_t threshold, wide_t<T> scale, wide_t<T> fill, uint64_t seed, uint64_t offset,
+                                                       const uint64_t* __restrict__ offsetDevice) {
+  using R = wide_t<T>;
+  if (offsetDevice) offset = *offsetDevice;
+  const size_t elements = n * width, blocks = (elements + 3) / 4;
+  for (size_t b = size_t(blockIdx.x) * BLOCK + threadIdx.x; b < blocks; b += size_t(gridDim.x) * BLOCK) {
+    const Philox4 r = philox4x32(uint32_t(b), uint32_t(b >> 32), uint32_t(offset), uint32_t(offset >> 32), uint32_t(seed), uint32_t(seed >> 32));
+    size_t row = 4 * b / width, column = 4 * b - row * width;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (4 * b + i < elements) out[row * outStride + column] = T(r.w[i] >= threshold ? R(x[row * stride + column]) * scale : fill);
+      if (++column == width) column = 0, ++row;
+    }
+  }
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------
+
+[[noreturn]] void refuse(const std::string& what) { throw std::runtime_error(what); }
+
+void launched(const char* what) {
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) refuse(std::string(what) + " launch: " + hipGetErrorString(e));
+}
+
+size_t elementBytes(int dtype) {
+  switch (dtype) {
+    case SPNC_HIP_FLOAT32: return 4;
+    case SPNC_HIP_FLOAT64: return 8;
+    case SPNC_HIP_FLOAT16:
+    case SPNC_HIP_BFLOAT16: return 2;
+  }
+  refuse("unknown element type " + std::to_string(dtype));
+}
+
+// calls fn(T()) for the element type
+template <typename Fn>
+void withType(int dtype, Fn&& fn) {
+  switch (dtype) {
+    case SPNC_HIP_FLOAT32: return fn(float());
+    case SPNC_HIP_FLOAT64: return fn(double());
+    case SPNC_HIP_FLOAT16: return fn(_Float16());
+    case SPNC_HIP_BFLOAT16: return fn(__bf16());
+  }
+  refuse("unknown element type " + std::to_string(dtype));
+}
+
+// the widest piece, in bytes, that a row of rowBytes at these addresses and strides consists of; `least` at the least
+unsigned pieceBytes(unsigned least, std::initializer_list<uintptr_t> addresses) {
+  uintptr_t bits = 16;
+  for (uintptr_t a : addresses) bits |= a;
+  const unsigned widest = unsigned(bits & (~bits + 1));
+  return widest < least ? 0 : widest;
+}
+
+uintptr_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+
+void checkAligned(unsigned piece, const char* what) {
+  if (piece == 0) refuse(std::string(what) + ": pointers are not aligned to the element type");
+}
+
+void checkSlots(size_t n, unsigned k, size_t capacity) {
+  if (k == 0) refuse("k must be at least 1");
+  if (n > (size_t(1) << 31) / k) refuse("too many slots: n * k must be below 2^31");
+  if (capacity >= (size_t(1) << 31)) refuse("too many rows: the capacity must be below 2^31");
+}
+
+void checkExperts(unsigned experts) {
+  if (experts == 0 || experts > SPNC_HIP_MAX_EXPERTS) refuse("experts must be between 1 and " + std::to_string(SPNC_HIP_MAX_EXPERTS));
+}
+
+void checkWeightType(int dtype, int weightDtype) {
+  if (weightDtype != SPNC_HIP_FLOAT32 && !(weightDtype == SPNC_HIP_FLOAT64 && dtype == SPNC_HIP_FLOAT64))
+    refuse("weights must be float32, or float64 with float64 values");
+}
+
+template <typename Fn>
+void withGateShape(unsigned experts, unsigned k, Fn&& fn) {
+  unsigned group = 1;
+  while (group < WAVE && (4 * group < experts || group < k)) group *= 2;
+#define SPN_GATE_SHAPE(G, V) return fn(std::integral_constant<int, G>(), std::integral_constant<int, V>())
+  switch (group) {
+    case 1: SPN_GATE_SHAPE(1, 4);
+    case 2: SPN_GATE_SHAPE(2, 4);
+    case 4: SPN_GATE_SHAPE(4, 4);
+    case 8: SPN_GATE_SHAPE(8, 4);
+    case 16: SPN_GATE_SHAPE(16, 4);
+    case 32: SPN_GATE_SHAPE(32, 4);
+  }
+  if (experts <= 256) SPN_GATE_SHAPE(64, 4);
+  if (experts <= 512) SPN_GATE_SHAPE(64, 8);
+  SPN_GATE_SHAPE(64, 16);
+#undef SPN_GATE_SHAPE
+}
+
+void checkGate(int dtype, size_t n, unsigned experts, size_t stride, unsigned k, unsigned flags) {
+  elementBytes(dtype);
+  checkExperts(experts);
+  if (k == 0 || k > experts || k > SPNC_HIP_MAX_CHOICES)
+    refuse("k must be between 1 and the number of experts, at most " + std::to_string(SPNC_HIP_MAX_CHOICES));
+  if (n > 1 && stride < experts) refuse("rows of logits overlap");
+  if (flags & ~unsigned(SPNC_HIP_GATE_ALL | SPNC_HIP_GATE_LOG)) refuse("unknown gate flags");
+}
+
+template <typename Fn>
+void withPieces(unsigned piece, Fn&& fn) {
+  switch (piece) {
+    case 16: return fn(Pack<uint32_t, 4>());
+    case 8: return fn(Pack<uint32_t, 2>());
+    case 4: return fn(uint32_t());
+    case 2: return fn(uint16_t());
+    default: return fn(uint8_t());
+  }
+}
+
+// calls fn(N) with N elements of T to a piece
+template <typename T, typename Fn>
+void withPack(unsigned piece, Fn&& fn) {
+  if (piece == 16) return fn(std::integral_constant<int, 16 / sizeof(T)>());
+  if constexpr (sizeof(T) <= 8)
+    if (piece == 8) return fn(std::integral_constant<int, 8 / sizeof(T)>());
+  if constexpr (sizeof(T) <= 4)
+    if (piece == 4) return fn(std::integral_constant<int, 4 / sizeof(T)>());
+  if constexpr (sizeof(T) <= 2)
+    if (piece == 2) return fn(std::integral_constant<int, 1>());
+}
+
+template <typename T, typename Fn>
+void withWeight(int weightDtype, Fn&& fn) {
+  if constexpr (std::is_same<T, double>::value)
+    if (weightDtype == SPNC_HIP_FLOAT64) return fn(double());
+  fn(float());
+}
+
+void clearRows(const int32_t* starts, const int32_t* counts, unsigned experts, size_t capacity, size_t rowBytes, void* out, hipStream_t stream) {
+  if (capacity == 0 || rowBytes == 0) return;
+  clearKernel<<<clearBlocks(capacity, rowBytes), BLOCK, 0, stream>>>(starts, counts, experts, capacity, rowBytes, static_cast<unsigned char*>(out));
+  launched("clearing unused rows");
+}
+
+void checkSegments(const int32_t* starts, const int32_t* counts, unsigned experts) {
+  checkExperts(experts);
+  if (!starts || !counts) refuse("null argument");
+}
+
+void checkLogTypes(int dtype, int weightDtype) {
+  if (dtype != SPNC_HIP_FLOAT32 && dtype != SPNC_HIP_FLOAT64) refuse("log-likelihoods must be float32 or float64");
+  if (weightDtype != SPNC_HIP_FLOAT32 && weightDtype != SPNC_HIP_FLOAT64) refuse("log weights must be float32 or float64");
+}
+
+template <typename Fn>
+void withLogTypes(int dtype, int weightDtype, Fn&& fn) {
+  if (dtype == SPNC_HIP_FLOAT32) return weightDtype == SPNC_HIP_FLOAT32 ? fn(float(), float()) : fn(float(), double());
+  return weightDtype == SPNC_HIP_FLOAT32 ? fn(double(), float()) : fn(double(), double());
+}
+
+}  // namespace
+}  // namespace spnc_hip
+
+using namespace spnc_hip;
+
+extern "C" {
+
+int spnc_hip_gate(const void* logits, int dtype, size_t n, unsigned experts, size_t stride, unsigned k, unsigned flags, int32_t* index,
+                  void* weight, void* stream) {
+  return guarded([&] {
+    checkGate(dtype, n, experts, stride, k, flags);
+    if (n == 0) return;
+    if (!logits || !index || !weight) refuse("null argument");
+    withType(dtype, [&](auto t) {
+      using T = decltype(t);
+      withGateShape(experts, k, [&](auto g, auto v) {
+        constexpr int G = decltype(g)::value, V = decltype(v)::value;
+        gateKernel<T, G, V><<<tileGrid((n + BLOCK / G - 1) / (BLOCK / G)), BLOCK, 0, static_cast<hipStream_t>(stream)>>>(
+            static_cast<const T*>(logits), n, experts, stride, k, flags, index, static_cast<wide_t<T>*>(weight));
+      });
+    });
+    launched("gate");
+  });
+}
+
+int spnc_hip_gate_backward(const void* logits, int dtype, size_t n, unsigned experts, size_t stride, unsigned k, unsigned flags,
+                           const int32_t* index, const void* weight, const void* grad_weight, void* grad_logits, void* stream) {
+  return guarded([&] {
+    checkGate(dtype, n, experts, stride, k, flags);
+    if (n == 0) return;
+    if ((!logits && (flags & SPNC_HIP_GATE_ALL)) || !index || !weight || !grad_weight || !grad_logits) refuse("null argument");
+    withType(dtype, [&](auto t) {
+      using T = decltype(t);
+      using R = wide_t<T>;
+      withGateShape(experts, k, [&](auto g, auto v) {
+        constexpr int G = decltype(g)::value, V = decltype(v)::value;
+        gateBackwardKernel<T, G, V><<<tileGrid((n + BLOCK / G - 1) / (BLOCK / G)), BLOCK, 0, static_cast<hipStream_t>(stream)>>>(
+            static_cast<const T*>(logits), n, experts, stride, k, flags, index, static_cast<const R*>(weight), static_cast<const R*>(grad_weight),
+            static_cast<T*>(grad_logits));
+      });
+    });
+    launched("gate gradient");
+  });
+}
+
+size_t spnc_hip_route_workspace(size_t slots, unsigned experts) {
+  const RouteShape shape = routeShape(slots);
+  return shape.blocks <= 1 ? 0 : size_t(shape.blocks) * experts * sizeof(uint32_t);
+}
+
+int spnc_hip_route(const int32_t* index, size_t slots, unsigned experts, unsigned align, int32_t* position, int32_t* starts, int32_t* counts,
+                   void* workspace, size_t workspace_bytes, void* stream) {
+  return guarded([&] {
+    checkExperts(experts);
+    if (align == 0) refuse("align must be at least 1");
+    if (slots >= (size_t(1) << 31) || slots + size_t(experts) * (align - 1) >= (size_t(1) << 31))
+      refuse("too many slots: slots + experts * (align - 1) must be below 2^31");
+    if ((slots && (!index || !position)) || !starts || !counts) refuse("null argument");
+    const RouteShape shape = routeShape(slots);
+    const size_t need = spnc_hip_route_workspace(slots, experts);
+    if (workspace_bytes < need || (need && !workspace)) refuse("the workspace must hold " + std::to_string(need) + " bytes");
+    unsigned bits = 0;
+    while ((1u << bits) < experts) ++bits;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (shape.blocks > 1) {
+      routeCountKernel<<<shape.blocks, ROUTE_BLOCK, experts * sizeof(uint32_t), s>>>(index, slots, experts, bits, shape.chunk,
+                                                                                     static_cast<uint32_t*>(workspace));
+      launched("route");
+    }
+    const size_t lds = ROUTE_WAVES * experts * sizeof(uint32_t);
+    if (lds > 48 * 1024) {
+      const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(routeKernel), hipFuncAttributeMaxDynamicSharedMemorySize, int(lds));
+      if (e != hipSuccess) refuse(std::string("route: ") + hipGetErrorString(e));
+    }
+    routeKernel<<<shape.blocks, ROUTE_BLOCK, lds, s>>>(
+        index, slots, experts, bits, align, shape.chunk, static_cast<const uint32_t*>(workspace), position, starts, counts);
+    launched("route");
+  });
+}
+
+int spnc_hip_dispatch(const void* rows, size_t n, size_t row_bytes, size_t stride_bytes, const int32_t* position, unsigned k, size_t capacity,
+                      const int32_t* starts, const int32_t* counts, unsigned experts, int zero_unused, void* out, void* stream) {
+  return guarded([&] {
+    checkSlots(n, k, capacity);
+    if (row_bytes >> 32) refuse("a row must be shorter than 4 GiB");
+    if (zero_unused) checkSegments(starts, counts, experts);
+    if (capacity == 0 || row_bytes == 0) return;
+    if (!out || (n && (!rows || !position))) refuse("null argument");
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (zero_unused) clearRows(starts, counts, experts, capacity, row_bytes, out, s);
+    if (n == 0) return;
+    const unsigned piece = pieceBytes(1, {address(rows), address(out), row_bytes, stride_bytes});
+    const RowShape shape = rowShape(n, row_bytes, piece);
+    withPieces(piece, [&](auto p) {
+      using P = decltype(p);
+      dispatchKernel<P><<<tileGrid(shape.tiles), BLOCK, 0, s>>>(static_cast<const unsigned char*>(rows), n, stride_bytes, shape, position, k, capacity,
+                                                               static_cast<P*>(out));
+    });
+    launched("dispatch");
+  });
+}
+
+int spnc_hip_combine(const void* values, int dtype, size_t capacity, size_t width, size_t stride, const int32_t* position, size_t n, unsigned k,
+                     const void* weight, int weight_dtype, void* out, void* stream) {
+  return guarded([&] {
+    const size_t bytes = elementBytes(dtype);
+    checkSlots(n, k, capacity);
+    if (weight) checkWeightType(dtype, weight_dtype);
+    if (width * bytes >> 32) refuse("a row must be shorter than 4 GiB");
+    if (n == 0 || width == 0) return;
+    if ((capacity && !values) || !position || !out) refuse("null argument");
+    const unsigned piece = pieceBytes(unsigned(bytes), {address(values), address(out), width * bytes, stride * bytes});
+    checkAligned(piece, "combine");
+    const RowShape shape = rowShape(n, width * bytes, piece);
+    withType(dtype, [&](auto t) {
+      using T = decltype(t);
+      withPack<T>(piece, [&](auto count) {
+        constexpr int N = decltype(count)::value;
+        withWeight<T>(weight_dtype, [&](auto w) {
+          using W = decltype(w);
+          combineKernel<T, N, W><<<tileGrid(shape.tiles), BLOCK, 0, static_cast<hipStream_t>(stream)>>>(
+              static_cast<const T*>(values), capacity, stride, shape, position, n, k, static_cast<const W*>(weight), static_cast<Pack<T, N>*>(out));
+        });
+      });
+    });
+    launched("combine");
+  });
+}
+
+int spnc_hip_combine_backward(const void* values, int dtype, size_t capacity, size_t width, size_t stride, const int32_t* position, size_t n,
+                              unsigned k, const void* weight, int weight_dtype, const void* grad_out, size_t grad_stride, const int32_t* starts,
+                              const int32_t* counts, unsigned experts, void* grad_values, void* grad_weight, void* stream) {
+  return guarded([&] {
+    const size_t bytes = elementBytes(dtype);
+    checkSlots(n, k, capacity);
+    checkWeightType(dtype, weight_dtype);
+    if (width * bytes >> 32) refuse("a row must be shorter than 4 GiB");
+    if (grad_values) checkSegments(starts, counts, experts);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (grad_values) clearRows(starts, counts, experts, capacity, width * bytes, grad_values, s);
+    if (n == 0 || (!grad_values && !grad_weight)) return;
+    if ((capacity && width && !values) || !position || !weight || (width && !grad_out)) refuse("null argument");
+    const unsigned piece = pieceBytes(unsigned(bytes), {address(values), address(grad_out), address(grad_values), width * bytes, stride * bytes,
+                                                        grad_stride * bytes});
+    checkAligned(piece, "combine gradient");
+    const RowShape shape = rowShape(n, width * bytes, piece);
+    withType(dtype, [&](auto t) {
+      using T = decltype(t);
+      withPack<T>(piece, [&](auto count) {
+        constexpr int N = decltype(count)::value;
+        withWeight<T>(weight_dtype, [&](auto w) {
+          using W = decltype(w);
+          combineBackwardKernel<T, N, W><<<tileGrid(shape.tiles), BLOCK, 0, s>>>(
+              static_cast<const T*>(values), capacity, stride, shape, position, n, k, static_cast<const W*>(weight), static_cast<const T*>(grad_out),
+              grad_stride, static_cast<Pack<T, N>*>(grad_values), static_cast<W*>(grad_weight));
+        });
+      });
+    });
+    launched("combine gradient");
+  });
+}
+
+int spnc_hip_combine_log(const void* values, int dtype, size_t capacity, const int32_t* position, size_t n, unsigned k, const void* log_weight,
+                         int weight_dtype, void* out, void* stream) {
+  return guarded([&] {
+    checkLogTypes(dtype, weight_dtype);
+    checkSlots(n, k, capacity);
+    if (n == 0) return;
+    if ((capacity && !values) || !position || !log_weight || !out) refuse("null argument");
+    withLogTypes(dtype, weight_dtype, [&](auto r, auto w) {
+      using R = decltype(r);
+      using W = decltype(w);
+      const LogTerms<R, W> terms{static_cast<const R*>(values), capacity, position, static_cast<const W*>(log_weight)};
+      combineLogKernel<R, W><<<tileGrid((n + BLOCK - 1) / BLOCK), BLOCK, 0, static_cast<hipStream_t>(stream)>>>(terms, n, k, static_cast<R*>(out));
+    });
+    launched("combine_log");
+  });
+}
+
+int spnc_hip_combine_log_backward(const void* values, int dtype, size_t capacity, const int32_t* position, size_t n, unsigned k,
+                                  const void* log_weight, int weight_dtype, const void* grad_out, const int32_t* starts, const int32_t* counts,
+                                  unsigned experts, void* grad_values, void* grad_log_weight, void* stream) {
+  return guarded([&] {
+    checkLogTypes(dtype, weight_dtype);
+    checkSlots(n, k, capacity);
+    if (grad_values) checkSegments(starts, counts, experts);
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    if (grad_values) clearRows(starts, counts, experts, capacity, elementBytes(dtype), grad_values, s);
+    if (n == 0 || (!grad_values && !grad_log_weight)) return;
+    if ((capacity && !values) || !position || !log_weight || !grad_out) refuse("null argument");
+    withLogTypes(dtype, weight_dtype, [&](auto r, auto w) {
+      using R = decltype(r);
+      using W = decltype(w);
+      const LogTerms<R, W> terms{static_cast<const R*>(values), capacity, position, static_cast<const W*>(log_weight)};
+      combineLogBackwardKernel<R, W><<<tileGrid((n + BLOCK - 1) / BLOCK), BLOCK, 0, s>>>(terms, n, k, static_cast<const R*>(grad_out),
+                                                                                       static_cast<R*>(grad_values), static_cast<W*>(grad_log_weight));
+    });
+    launched("combine_log gradient");
+  });
+}
+
+int spnc_hip_dropout(const void* x, int dtype, size_t n, size_t width, size_t stride, void* out, size_t out_stride, double p, int mode,
+                     uint64_t seed, uint64_t offset, const uint64_t* offset_device, void* stream) {
+  return guarded([&] {
+    elementBytes(dtype);
+    if (!(p >= 0.0 && p <= 1.0)) refuse("the probability of dropping an element must be between 0 and 1");
+    if (mode < SPNC_HIP_DROPOUT_ZERO || mode > SPNC_HIP_DROPOUT_MASK) refuse("unknown dropout mode " + std::to_string(mode));
+    if (n > 1 && (stride < width || out_stride < width)) refuse("rows overlap");
+    if (n == 0 || width == 0) return;
+    if (!x || !out) refuse("null argument");
+    const uint64_t threshold = uint64_t(std::llrint(p * 4294967296.0));
+    const double scale = mode != SPNC_HIP_DROPOUT_ZERO ? 1.0 : threshold >> 32 ? 0.0 : 1.0 / (1.0 - p);
+    const double fill = mode == SPNC_HIP_DROPOUT_MARGINAL ? NAN : 0.0;
+    const size_t blocks = ((n * width + 3) / 4 + BLOCK - 1) / BLOCK;
+    withType(dtype, [&](auto t) {
+      using T = decltype(t);
+      using R = wide_t<T>;
+      dropoutKernel<T><<<unsigned(blocks < MAX_GRID ? blocks : MAX_GRID), BLOCK, 0, static_cast<hipStream_t>(stream)>>>(
+          static_cast<const T*>(x), n, width, stride, static_cast<T*>(out), out_stride, threshold, R(scale), R(fill), seed, offset, offset_device);
+    });
+    launched("dropout");
+  });
+}
+
+}  // extern "C"

@@ -71,6 +71,12 @@ class HIPCompiler:
             raise RuntimeError("Compilation failed, not Kernel produced")
         return kernel
 
+    def compile_mixture(self, spns, inputDataType="float64", errorModel=ErrorModel(), batchSize=64, supportMarginal=True, name="spn_hip"):
+        """Compile SPNs over the same features into the experts of a gated mixture (``spnc.mixture.Mixture``)."""
+        from .mixture import Mixture
+        return Mixture([self.compile_ll(spn, inputDataType, errorModel=errorModel, batchSize=batchSize, supportMarginal=supportMarginal,
+                                        name=f"{name}_{i}") for i, spn in enumerate(spns)])
+
     def execute(self, kernel, inputs):
         """Execute a compiled kernel on the given inputs."""
         if type(inputs) is not np.ndarray:

@@ -98,6 +98,19 @@ def _load():
     lib.spnc_hip_destroy.argtypes = [vp]
     lib.spnc_hip_destroy.restype = None
     lib.spnc_hip_last_error.restype = cp
+    # include/spnc_hip_rows.h
+    i, u, d, u64 = ctypes.c_int, ctypes.c_uint, ctypes.c_double, ctypes.c_uint64
+    lib.spnc_hip_gate.argtypes = [vp, i, sz, u, sz, u, u, vp, vp, vp]
+    lib.spnc_hip_gate_backward.argtypes = [vp, i, sz, u, sz, u, u, vp, vp, vp, vp, vp]
+    lib.spnc_hip_route_workspace.argtypes = [sz, u]
+    lib.spnc_hip_route_workspace.restype = sz
+    lib.spnc_hip_route.argtypes = [vp, sz, u, u, vp, vp, vp, vp, sz, vp]
+    lib.spnc_hip_dispatch.argtypes = [vp, sz, sz, sz, vp, u, sz, vp, vp, u, i, vp, vp]
+    lib.spnc_hip_combine.argtypes = [vp, i, sz, sz, sz, vp, sz, u, vp, i, vp, vp]
+    lib.spnc_hip_combine_backward.argtypes = [vp, i, sz, sz, sz, vp, sz, u, vp, i, vp, sz, vp, vp, u, vp, vp, vp]
+    lib.spnc_hip_combine_log.argtypes = [vp, i, sz, vp, sz, u, vp, i, vp, vp]
+    lib.spnc_hip_combine_log_backward.argtypes = [vp, i, sz, vp, sz, u, vp, i, vp, vp, vp, u, vp, vp, vp]
+    lib.spnc_hip_dropout.argtypes = [vp, i, sz, sz, sz, vp, sz, d, i, u64, u64, vp, vp]
     _lib = lib
     return lib
 
