@@ -25,16 +25,16 @@ template <> struct Wide<double> { using type = double; };
 template <typename T> using wide_t = typename Wide<T>::type;
 
 template <typename T, int N>
-struct alignas(sizeof(T) * N) Pack {
+struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack {
   T v[N];
 };
 
 // Neighbouring tiles of rows go to one die: rows that are neighbours in the sorted buffer come from neighbouring rows,
 // and a cache line of narrow rows is then filled or read within one L2.
 template <typename Body>
-__device__ inline void forTiles(size_t tiles, Body&& body) {
+__device__ inline void forTiles(size_t tiles, unsigned grid, Body&& body) {
   const size_t perDie = (tiles + XCDS - 1) / XCDS, first = size_t(blockIdx.x % XCDS) * perDie;
-  for (size_t t = blockIdx.x / XCDS; t < perDie; t += gridDim.x / XCDS)
+  for (size_t t = blockIdx.x / XCDS; t < perDie; t += grid / XCDS)
     if (first + t < tiles) body(first + t);
 }
 
@@ -96,7 +96,7 @@ __global__ __launch_bounds__(BLOCK) void gateKernel(const T* __restrict__ logits
   using O = Order<R>;
   using K = typename O::key;
   const unsigned lane = threadIdx.x % G;
-  forTiles((n + BLOCK / G - 1) / (BLOCK / G), [&](size_t tile) {
+  forTiles((n + BLOCK / G - 1) / (BLOCK / G), gridDim.x, [&](size_t tile) {
     const size_t row = tile * (BLOCK / G) + threadIdx.x / G;
     if (row >= n) return;  // whole groups leave; shuffles stay inside a group
     K key[V];
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(BLOCK) void gateBackwardKernel(const T* __restrict_
   using R = wide_t<T>;
   const unsigned lane = threadIdx.x % G;
   const bool all = flags & SPNC_HIP_GATE_ALL, logs = flags & SPNC_HIP_GATE_LOG;
-  forTiles((n + BLOCK / G - 1) / (BLOCK / G), [&](size_t tile) {
+  forTiles((n + BLOCK / G - 1) / (BLOCK / G), gridDim.x, [&](size_t tile) {
     const size_t row = tile * (BLOCK / G) + threadIdx.x / G;
     if (row >= n) return;
     R share[V];  // of the experts, under "all"
@@ -219,17 +219,19 @@ __global__ __launch_bounds__(BLOCK) void gateBackwardKernel(const T* __restrict_
 // ---- routing --------------------------------------------------------------------------------------------------------
 
 constexpr unsigned ROUTE_BLOCK = 1024, ROUTE_WAVES = ROUTE_BLOCK / WAVE, ROUTE_MAX_BLOCKS = 256;
-constexpr size_t ROUTE_SINGLE = 8192;  // slots one block sorts by itself
+constexpr size_t ROUTE_SINGLE = 8192;      // slots one block sorts by itself
+constexpr unsigned ROUTE_MAX_COUNTS = 65536;  // counters (blocks * experts) that every block adds up
 
 struct RouteShape {
   size_t chunk;     // slots a block sorts, a multiple of ROUTE_BLOCK
   unsigned blocks;
 };
 
-RouteShape routeShape(size_t slots) {
+RouteShape routeShape(size_t slots, unsigned experts) {
   if (slots <= ROUTE_SINGLE) return {(slots + ROUTE_BLOCK - 1) / ROUTE_BLOCK * ROUTE_BLOCK, 1};
   size_t blocks = (slots + 4 * ROUTE_BLOCK - 1) / (4 * ROUTE_BLOCK);
-  if (blocks > ROUTE_MAX_BLOCKS) blocks = ROUTE_MAX_BLOCKS;
+  const size_t most = ROUTE_MAX_COUNTS / experts < ROUTE_MAX_BLOCKS ? ROUTE_MAX_COUNTS / experts : ROUTE_MAX_BLOCKS;
+  if (blocks > most) blocks = most;
   const size_t chunk = ((slots + blocks - 1) / blocks + ROUTE_BLOCK - 1) / ROUTE_BLOCK * ROUTE_BLOCK;
   return {chunk, unsigned((slots + chunk - 1) / chunk)};
 }
@@ -275,28 +277,32 @@ __global__ __launch_bounds__(ROUTE_BLOCK) void routeKernel(const int32_t* __rest
                                                            unsigned align, size_t chunk, const uint32_t* __restrict__ blockCounts,
                                                            int32_t* __restrict__ position, int32_t* __restrict__ starts, int32_t* __restrict__ counts) {
   extern __shared__ uint32_t routeLds[];  // counter[ROUTE_WAVES][experts]
-  __shared__ uint32_t waveSum[ROUTE_WAVES];
+  __shared__ uint32_t waveSum[ROUTE_WAVES], total[ROUTE_BLOCK], earlier[ROUTE_BLOCK];
   const unsigned t = threadIdx.x, lane = t % WAVE, wave = t / WAVE;
   for (unsigned i = t; i < ROUTE_WAVES * experts; i += ROUTE_BLOCK) routeLds[i] = 0;
+  total[t] = earlier[t] = 0;
   __syncthreads();
+  // what all blocks, and the blocks before this one, hold of every expert: integer sums, the same in any order
+  if (gridDim.x > 1) {
+    const unsigned slices = ROUTE_BLOCK / experts, slice = t / experts, e = t % experts;
+    uint32_t all = 0, before = 0;
+    if (slice < slices)
+      for (unsigned b = slice; b < gridDim.x; b += slices) {
+        const uint32_t c = blockCounts[size_t(b) * experts + e];
+        all += c;
+        before += b < blockIdx.x ? c : 0;
+      }
+    if (all) atomicAdd(&total[e], all);
+    if (before) atomicAdd(&earlier[e], before);
+  }
   const size_t begin = blockIdx.x * chunk + wave * (chunk / ROUTE_WAVES);
   size_t end = begin + chunk / ROUTE_WAVES;
   if (end > slots) end = slots;
   countSlots(index, begin, end, experts, bits, routeLds + wave * experts);
   __syncthreads();
-  // thread e: this block's total of expert e, what earlier blocks hold of it, and the total of all blocks
-  uint32_t before = 0, all = 0;
-  if (t < experts) {
-    if (gridDim.x == 1) {
-      for (unsigned w = 0; w < ROUTE_WAVES; ++w) all += routeLds[w * experts + t];
-    } else {
-      for (unsigned b = 0; b < gridDim.x; ++b) {
-        const uint32_t c = blockCounts[size_t(b) * experts + t];
-        all += c;
-        if (b < blockIdx.x) before += c;
-      }
-    }
-  }
+  uint32_t all = total[t];
+  if (gridDim.x == 1 && t < experts)
+    for (unsigned w = 0; w < ROUTE_WAVES; ++w) all += routeLds[w * experts + t];
   // where each segment starts: an exclusive scan of the totals, rounded up
   const uint32_t rounded = (all + (align - 1)) / align * align;
   uint32_t scan = rounded;
@@ -314,7 +320,7 @@ __global__ __launch_bounds__(ROUTE_BLOCK) void routeKernel(const int32_t* __rest
       counts[t] = int32_t(all);
       if (t == experts - 1) starts[experts] = int32_t(start + rounded);
     }
-    uint32_t next = start + before;
+    uint32_t next = start + earlier[t];
     for (unsigned w = 0; w < ROUTE_WAVES; ++w) {
       const uint32_t c = routeLds[w * experts + t];
       routeLds[w * experts + t] = next;
@@ -355,27 +361,37 @@ RowShape rowShape(size_t n, size_t rowBytes, unsigned pieceBytes) {
   return s;
 }
 
-// Rows of the sorted buffer that belong to no segment, cleared by the blocks behind the first `rowBlocks`: a wave for
-// every segment's end, and all of them for what follows the last one.
-__device__ inline void clearUnused(unsigned block, unsigned blocks, const int32_t* starts, const int32_t* counts, unsigned experts,
-                                   size_t capacity, size_t rowBytes, unsigned char* out) {
+// Rows of the sorted buffer that belong to no segment, cleared by blocks of their own behind the rowBlocks that write the
+// others: a wave for what follows each segment, all of them for what follows the last one.
+struct Unused {
+  unsigned rowBlocks, blocks;
+  const int32_t *starts, *counts;
+  unsigned experts;
+  size_t capacity, rowBytes;
+  unsigned char* out;
+};
+
+__device__ inline void clearUnused(const Unused& u) {
   const unsigned lane = threadIdx.x % WAVE;
-  const size_t wave = size_t(block) * (BLOCK / WAVE) + threadIdx.x / WAVE, waves = size_t(blocks) * (BLOCK / WAVE);
+  const size_t wave = size_t(blockIdx.x - u.rowBlocks) * (BLOCK / WAVE) + threadIdx.x / WAVE, waves = size_t(u.blocks) * (BLOCK / WAVE);
   auto clear = [&](size_t from, size_t to, size_t first, size_t step) {  // bytes; pointers may have any alignment
-    if (((reinterpret_cast<uintptr_t>(out) | from | to) & 3) == 0) {
-      uint32_t* words = reinterpret_cast<uint32_t*>(out);
+    if (((reinterpret_cast<uintptr_t>(u.out) | from | to) & 15) == 0) {
+      Pack<uint32_t, 4>* words = reinterpret_cast<Pack<uint32_t, 4>*>(u.out);
+      for (size_t i = from / 16 + first; i < to / 16; i += step) words[i] = Pack<uint32_t, 4>{};
+    } else if (((reinterpret_cast<uintptr_t>(u.out) | from | to) & 3) == 0) {
+      uint32_t* words = reinterpret_cast<uint32_t*>(u.out);
       for (size_t i = from / 4 + first; i < to / 4; i += step) words[i] = 0;
     } else {
-      for (size_t i = from + first; i < to; i += step) out[i] = 0;
+      for (size_t i = from + first; i < to; i += step) u.out[i] = 0;
     }
   };
-  for (size_t e = wave; e < experts; e += waves) {
-    size_t from = size_t(starts[e]) + size_t(counts[e]), to = size_t(starts[e + 1]);
-    if (to > capacity) to = capacity;
-    if (from < to) clear(from * rowBytes, to * rowBytes, lane, WAVE);
+  for (size_t e = wave; e < u.experts; e += waves) {
+    size_t from = size_t(u.starts[e]) + size_t(u.counts[e]), to = size_t(u.starts[e + 1]);
+    if (to > u.capacity) to = u.capacity;
+    if (from < to) clear(from * u.rowBytes, to * u.rowBytes, lane, WAVE);
   }
-  const size_t end = size_t(starts[experts]);
-  if (end < capacity) clear(end * rowBytes, capacity * rowBytes, wave * WAVE + lane, waves * WAVE);
+  const size_t end = size_t(u.starts[u.experts]);
+  if (end < u.capacity) clear(end * u.rowBytes, u.capacity * u.rowBytes, wave * WAVE + lane, waves * WAVE);
 }
 
 unsigned clearBlocks(size_t capacity, size_t rowBytes) {
@@ -383,47 +399,76 @@ unsigned clearBlocks(size_t capacity, size_t rowBytes) {
   return unsigned(b < 256 ? b : 256);
 }
 
-template <typename P>
+// Positions of KB slots from `first` on, -1 where there is no slot or it is not routed.
+template <int KB>
+__device__ inline void loadPositions(const int32_t* position, size_t row, unsigned k, unsigned first, size_t capacity, int32_t (&at)[KB]) {
+#pragma unroll
+  for (int j = 0; j < KB; ++j) {
+    at[j] = first + j < k ? position[row * k + first + j] : -1;
+    if (at[j] >= 0 && size_t(at[j]) >= capacity) at[j] = -1;
+  }
+}
+
+template <int KB, typename W, typename R>
+__device__ inline void loadWeights(const W* weight, size_t row, unsigned k, unsigned first, R (&w)[KB]) {
+#pragma unroll
+  for (int j = 0; j < KB; ++j) w[j] = !weight ? R(1) : first + j < k ? R(weight[row * k + first + j]) : R(0);
+}
+
+template <typename P, int KB>
 __global__ __launch_bounds__(BLOCK) void dispatchKernel(const unsigned char* __restrict__ rows, size_t n, size_t strideBytes, RowShape shape,
-                                                        const int32_t* __restrict__ position, unsigned k, size_t capacity, P* __restrict__ out) {
+                                                        const int32_t* __restrict__ position, unsigned k, size_t capacity, P* __restrict__ out,
+                                                        Unused unused) {
+  if (blockIdx.x >= unused.rowBlocks) return clearUnused(unused);
   const unsigned lane = threadIdx.x & ((1u << shape.shift) - 1);
-  forTiles(shape.tiles, [&](size_t tile) {
+  forTiles(shape.tiles, unused.rowBlocks, [&](size_t tile) {
     const size_t row = tile * (BLOCK >> shape.shift) + (threadIdx.x >> shape.shift);
     if (row >= n) return;
     const P* source = reinterpret_cast<const P*>(rows + row * strideBytes);
-    for (unsigned c = lane; c < shape.pieces; c += 1u << shape.shift) {
-      const P piece = source[c];
-      for (unsigned j = 0; j < k; ++j) {
-        const int32_t to = position[row * k + j];
-        if (to >= 0 && size_t(to) < capacity) out[size_t(to) * shape.pieces + c] = piece;
+    for (unsigned first = 0; first < k; first += KB) {
+      int32_t at[KB];
+      loadPositions<KB>(position, row, k, first, capacity, at);
+      for (unsigned c = lane; c < shape.pieces; c += 1u << shape.shift) {
+        const P piece = source[c];
+#pragma unroll
+        for (int j = 0; j < KB; ++j)
+          if (at[j] >= 0) out[size_t(at[j]) * shape.pieces + c] = piece;
       }
     }
   });
 }
 
-__global__ __launch_bounds__(BLOCK) void clearKernel(const int32_t* __restrict__ starts, const int32_t* __restrict__ counts, unsigned experts,
-                                                     size_t capacity, size_t rowBytes, unsigned char* __restrict__ out) {
-  clearUnused(blockIdx.x, gridDim.x, starts, counts, experts, capacity, rowBytes, out);
-}
-
-template <typename T, int N, typename W>
+// Slots are read KB at a time, all loads before the first product; a slot that is not routed reads row 0 and drops it.
+template <typename T, int N, typename W, int KB, bool ONE>
 __global__ __launch_bounds__(BLOCK) void combineKernel(const T* __restrict__ values, size_t capacity, size_t stride, RowShape shape,
                                                        const int32_t* __restrict__ position, size_t n, unsigned k, const W* __restrict__ weight,
                                                        Pack<T, N>* __restrict__ out) {
   using R = wide_t<T>;
   const unsigned lane = threadIdx.x & ((1u << shape.shift) - 1);
-  forTiles(shape.tiles, [&](size_t tile) {
+  forTiles(shape.tiles, gridDim.x, [&](size_t tile) {
     const size_t row = tile * (BLOCK >> shape.shift) + (threadIdx.x >> shape.shift);
     if (row >= n) return;
+    int32_t at[KB];
+    R w[KB];
+    if (ONE) {
+      loadPositions<KB>(position, row, k, 0, capacity, at);
+      loadWeights<KB>(weight, row, k, 0, w);
+    }
     for (unsigned c = lane; c < shape.pieces; c += 1u << shape.shift) {
       R sum[N] = {};
-      for (unsigned j = 0; j < k; ++j) {
-        const int32_t at = position[row * k + j];
-        if (at < 0 || size_t(at) >= capacity) continue;
-        const R w = weight ? R(weight[row * k + j]) : R(1);
-        const Pack<T, N> v = *reinterpret_cast<const Pack<T, N>*>(values + size_t(at) * stride + size_t(c) * N);
+      for (unsigned first = 0; first < (ONE ? 1 : k); first += KB) {
+        if (!ONE) {
+          loadPositions<KB>(position, row, k, first, capacity, at);
+          loadWeights<KB>(weight, row, k, first, w);
+        }
+        Pack<T, N> v[KB];
 #pragma unroll
-        for (int i = 0; i < N; ++i) sum[i] += w * R(v.v[i]);
+        for (int j = 0; j < KB; ++j)
+          if (capacity) v[j] = *reinterpret_cast<const Pack<T, N>*>(values + size_t(at[j] >= 0 ? at[j] : 0) * stride + size_t(c) * N);
+#pragma unroll
+        for (int j = 0; j < KB; ++j)
+#pragma unroll
+          for (int i = 0; i < N; ++i) sum[i] += at[j] >= 0 ? w[j] * R(v[j].v[i]) : R(0);
       }
       Pack<T, N> o;
 #pragma unroll
@@ -433,40 +478,50 @@ __global__ __launch_bounds__(BLOCK) void combineKernel(const T* __restrict__ val
   });
 }
 
-template <typename T, int N, typename W>
+template <typename T, int N, typename W, int KB>
 __global__ __launch_bounds__(BLOCK) void combineBackwardKernel(const T* __restrict__ values, size_t capacity, size_t stride, RowShape shape,
                                                                const int32_t* __restrict__ position, size_t n, unsigned k,
                                                                const W* __restrict__ weight, const T* __restrict__ gradOut, size_t gradStride,
-                                                               Pack<T, N>* __restrict__ gradValues, W* __restrict__ gradWeight) {
+                                                               Pack<T, N>* __restrict__ gradValues, W* __restrict__ gradWeight, Unused unused) {
   using R = wide_t<T>;
+  if (blockIdx.x >= unused.rowBlocks) return clearUnused(unused);
   const unsigned group = 1u << shape.shift, lane = threadIdx.x & (group - 1);
-  forTiles(shape.tiles, [&](size_t tile) {
+  forTiles(shape.tiles, unused.rowBlocks, [&](size_t tile) {
     const size_t row = tile * (BLOCK >> shape.shift) + (threadIdx.x >> shape.shift);
     if (row >= n) return;
-    for (unsigned j = 0; j < k; ++j) {
-      const int32_t at = position[row * k + j];
-      const bool routed = at >= 0 && size_t(at) < capacity;
-      R dot = 0;
-      if (routed) {
-        const R w = weight ? R(weight[row * k + j]) : R(1);
-        for (unsigned c = lane; c < shape.pieces; c += group) {
-          const Pack<T, N> g = *reinterpret_cast<const Pack<T, N>*>(gradOut + row * gradStride + size_t(c) * N);
-          if (gradWeight) {
-            const Pack<T, N> v = *reinterpret_cast<const Pack<T, N>*>(values + size_t(at) * stride + size_t(c) * N);
+    for (unsigned first = 0; first < k; first += KB) {
+      int32_t at[KB];
+      R w[KB], dot[KB] = {};
+      loadPositions<KB>(position, row, k, first, capacity, at);
+      loadWeights<KB>(weight, row, k, first, w);
+      for (unsigned c = lane; c < shape.pieces; c += group) {
+        const Pack<T, N> g = *reinterpret_cast<const Pack<T, N>*>(gradOut + row * gradStride + size_t(c) * N);
+        if (gradWeight && capacity) {
+          Pack<T, N> v[KB];
 #pragma unroll
-            for (int i = 0; i < N; ++i) dot += R(g.v[i]) * R(v.v[i]);
-          }
-          if (gradValues) {
-            Pack<T, N> o;
+          for (int j = 0; j < KB; ++j) v[j] = *reinterpret_cast<const Pack<T, N>*>(values + size_t(at[j] >= 0 ? at[j] : 0) * stride + size_t(c) * N);
 #pragma unroll
-            for (int i = 0; i < N; ++i) o.v[i] = T(w * R(g.v[i]));
-            gradValues[size_t(at) * shape.pieces + c] = o;
-          }
+          for (int j = 0; j < KB; ++j)
+#pragma unroll
+            for (int i = 0; i < N; ++i) dot[j] += at[j] >= 0 ? R(g.v[i]) * R(v[j].v[i]) : R(0);
+        }
+        if (gradValues) {
+#pragma unroll
+          for (int j = 0; j < KB; ++j)
+            if (at[j] >= 0) {
+              Pack<T, N> o;
+#pragma unroll
+              for (int i = 0; i < N; ++i) o.v[i] = T(w[j] * R(g.v[i]));
+              gradValues[size_t(at[j]) * shape.pieces + c] = o;
+            }
         }
       }
       if (gradWeight) {
-        for (unsigned d = 1; d < group; d *= 2) dot += __shfl_xor(dot, int(d));
-        if (lane == 0) gradWeight[row * k + j] = W(dot);
+#pragma unroll
+        for (int j = 0; j < KB; ++j) {
+          for (unsigned d = 1; d < group; d *= 2) dot[j] += __shfl_xor(dot[j], int(d));
+          if (lane == 0 && first + j < k) gradWeight[row * k + first + j] = W(dot[j]);
+        }
       }
     }
   });
@@ -475,94 +530,214 @@ __global__ __launch_bounds__(BLOCK) void combineBackwardKernel(const T* __restri
 // The largest value of the row's slots is taken out before its log weight is added: values of some thousands differ by
 // little, and the difference is exact where the sum would be rounded. Shares are computed from the same terms, not from the
 // rounded result.
-template <typename R, typename W>
+template <typename R> __device__ inline R expOf(R x) { return std::is_same<R, double>::value ? R(exp(double(x))) : R(expf(float(x))); }
+template <typename R> __device__ inline R logOf(R x) { return std::is_same<R, double>::value ? R(log(double(x))) : R(logf(float(x))); }
+
+// A row's slots. K > 0: held in registers, read as one piece each of positions and weights; K = 0: read again for every use.
+template <typename R, typename W, int K>
 struct LogTerms {
   const R* values;
   size_t capacity;
   const int32_t* position;
   const W* logWeight;
+  unsigned k;
+  int32_t at[K > 0 ? K : 1];
+  R value[K > 0 ? K : 1], weight[K > 0 ? K : 1];
+
+  __device__ unsigned count() const { return K > 0 ? K : k; }
   // false: the slot is left out
-  __device__ bool slot(size_t s, R& value, R& lw) const {
-    const int32_t at = position[s];
-    if (at < 0 || size_t(at) >= capacity) return false;
-    lw = R(logWeight[s]);
+  __device__ bool read(size_t s, R& v, R& lw, int32_t& p) const {
+    p = position[s];
+    if (p >= 0 && size_t(p) >= capacity) p = -1;
+    lw = p >= 0 ? R(logWeight[s]) : R(-INFINITY);
     if (lw == -INFINITY) return false;
-    value = values[at];
+    v = values[p];
     return true;
+  }
+  __device__ void load(size_t row) {
+    if constexpr (K > 0) {
+      const Pack<int32_t, K> p = *reinterpret_cast<const Pack<int32_t, K>*>(position + row * K);
+      const Pack<W, K> w = *reinterpret_cast<const Pack<W, K>*>(logWeight + row * K);
+#pragma unroll
+      for (int j = 0; j < K; ++j) {
+        at[j] = p.v[j] >= 0 && size_t(p.v[j]) < capacity ? p.v[j] : -1;
+        weight[j] = at[j] >= 0 ? R(w.v[j]) : R(-INFINITY);
+        value[j] = capacity ? values[at[j] >= 0 ? at[j] : 0] : R(0);
+      }
+    }
+  }
+  __device__ bool slot(size_t row, unsigned j, R& v, R& lw) const {
+    if constexpr (K > 0) {
+      v = value[j];
+      lw = weight[j];
+      return lw != -INFINITY;
+    } else {
+      int32_t p;
+      return read(row * k + j, v, lw, p);
+    }
   }
 };
 
-template <typename R> __device__ inline R expOf(R x) { return std::is_same<R, double>::value ? R(exp(double(x))) : R(expf(float(x))); }
-template <typename R> __device__ inline R logOf(R x) { return std::is_same<R, double>::value ? R(log(double(x))) : R(logf(float(x))); }
-
 // peak: the largest value; shift: the largest log weight + (value - peak); total: sum of exp(that - shift)
-template <typename R, typename W>
-__device__ inline void logSum(const LogTerms<R, W>& terms, size_t row, unsigned k, R& peak, R& shift, R& total) {
+template <typename R, typename W, int K>
+__device__ inline void logSum(const LogTerms<R, W, K>& terms, size_t row, R& peak, R& shift, R& total) {
   peak = -INFINITY;
   R v, lw;
-  for (unsigned j = 0; j < k; ++j)
-    if (terms.slot(row * k + j, v, lw)) peak = v > peak || v != v ? v : peak;
+#pragma unroll
+  for (unsigned j = 0; j < terms.count(); ++j)
+    if (terms.slot(row, j, v, lw)) peak = v > peak || v != v ? v : peak;
   shift = -INFINITY;
   total = 0;
-  if (!(peak > -INFINITY) && peak == peak) return;  // nothing possible
-  for (unsigned j = 0; j < k; ++j)
-    if (terms.slot(row * k + j, v, lw)) {
+  if (peak == -INFINITY) return;  // nothing possible
+#pragma unroll
+  for (unsigned j = 0; j < terms.count(); ++j)
+    if (terms.slot(row, j, v, lw)) {
       const R t = lw + (v - peak);
       shift = t > shift || t != t ? t : shift;
     }
-  for (unsigned j = 0; j < k; ++j)
-    if (terms.slot(row * k + j, v, lw)) total += expOf<R>(lw + (v - peak) - shift);
+#pragma unroll
+  for (unsigned j = 0; j < terms.count(); ++j)
+    if (terms.slot(row, j, v, lw)) total += expOf<R>(lw + (v - peak) - shift);
 }
 
-template <typename R, typename W>
-__global__ __launch_bounds__(BLOCK) void combineLogKernel(LogTerms<R, W> terms, size_t n, unsigned k, R* __restrict__ out) {
-  forTiles((n + BLOCK - 1) / BLOCK, [&](size_t tile) {
+template <typename R, typename W, int K>
+__global__ __launch_bounds__(BLOCK) void combineLogKernel(const R* __restrict__ values, size_t capacity, const int32_t* __restrict__ position,
+                                                          const W* __restrict__ logWeight, size_t n, unsigned k, R* __restrict__ out) {
+  forTiles((n + BLOCK - 1) / BLOCK, gridDim.x, [&](size_t tile) {
     const size_t row = tile * BLOCK + threadIdx.x;
     if (row >= n) return;
+    LogTerms<R, W, K> terms{values, capacity, position, logWeight, k};
+    terms.load(row);
     R peak, shift, total;
-    logSum(terms, row, k, peak, shift, total);
+    logSum(terms, row, peak, shift, total);
     out[row] = peak == -INFINITY || peak == INFINITY ? peak : peak + (shift + logOf<R>(total));
   });
 }
 
-template <typename R, typename W>
-__global__ __launch_bounds__(BLOCK) void combineLogBackwardKernel(LogTerms<R, W> terms, size_t n, unsigned k, const R* __restrict__ gradOut,
-                                                                  R* __restrict__ gradValues, W* __restrict__ gradLogWeight) {
-  forTiles((n + BLOCK - 1) / BLOCK, [&](size_t tile) {
+template <typename R, typename W, int K>
+__global__ __launch_bounds__(BLOCK) void combineLogBackwardKernel(const R* __restrict__ values, size_t capacity, const int32_t* __restrict__ position,
+                                                                  const W* __restrict__ logWeight, size_t n, unsigned k, const R* __restrict__ gradOut,
+                                                                  R* __restrict__ gradValues, W* __restrict__ gradLogWeight, Unused unused) {
+  if (blockIdx.x >= unused.rowBlocks) return clearUnused(unused);
+  forTiles((n + BLOCK - 1) / BLOCK, unused.rowBlocks, [&](size_t tile) {
     const size_t row = tile * BLOCK + threadIdx.x;
     if (row >= n) return;
+    LogTerms<R, W, K> terms{values, capacity, position, logWeight, k};
+    terms.load(row);
     R peak, shift, total;
-    logSum(terms, row, k, peak, shift, total);
+    logSum(terms, row, peak, shift, total);
     const R g = gradOut[row];
-    for (unsigned j = 0; j < k; ++j) {
-      const size_t s = row * k + j;
-      R v, lw, share = 0;
-      if (peak != -INFINITY && terms.slot(s, v, lw)) share = g * (expOf<R>(lw + (v - peak) - shift) / total);
-      const int32_t at = terms.position[s];
-      if (gradValues && at >= 0 && size_t(at) < terms.capacity) gradValues[at] = share;
-      if (gradLogWeight) gradLogWeight[s] = W(share);
+    if constexpr (K > 0) {
+      Pack<W, K> o;
+#pragma unroll
+      for (int j = 0; j < K; ++j) {
+        R v, lw, share = 0;
+        if (peak != -INFINITY && terms.slot(row, j, v, lw)) share = g * (expOf<R>(lw + (v - peak) - shift) / total);
+        if (gradValues && terms.at[j] >= 0) gradValues[terms.at[j]] = share;
+        o.v[j] = W(share);
+      }
+      if (gradLogWeight) *reinterpret_cast<Pack<W, K>*>(gradLogWeight + row * K) = o;
+    } else {
+      for (unsigned j = 0; j < k; ++j) {
+        const size_t s = row * k + j;
+        R v, lw, share = 0;
+        int32_t p;
+        if (terms.read(s, v, lw, p) && peak != -INFINITY) share = g * (expOf<R>(lw + (v - peak) - shift) / total);
+        if (gradValues && p >= 0) gradValues[p] = share;
+        if (gradLogWeight) gradLogWeight[s] = W(share);
+      }
     }
   });
 }
 
 // ---- dropout --------------------------------------------------------------------------------------------------------
 
-template <typename T>
-__global__ __launch_bounds__(BLOCK) void dropoutKernel(const T* x, size_t n, size_t width, size_t stride, T* out, size_t outStride,
-                                                       uint64_t threshold, wide_t<T> scale, wide_t<T> fill, uint64_t seed, uint64_t offset,
-                                                       const uint64_t* __restrict__ offsetDevice) {
-  using R = wide_t<T>;
-  if (offsetDevice) offset = *offsetDevice;
-  const size_t elements = n * width, blocks = (elements + 3) / 4;
-  for (size_t b = size_t(blockIdx.x) * BLOCK + threadIdx.x; b < blocks; b += size_t(gridDim.x) * BLOCK) {
-    const Philox4 r = philox4x32(uint32_t(b), uint32_t(b >> 32), uint32_t(offset), uint32_t(offset >> 32), uint32_t(seed), uint32_t(seed >> 32));
-    size_t row = 4 * b / width, column = 4 * b - row * width;
+template <typename R>
+struct Dropout {
+  uint64_t threshold;
+  R scale, fill;
+  uint64_t seed, offset;
+  const uint64_t* offsetDevice;
+
+  __device__ Philox4 words(size_t block, uint64_t at) const {
+    return philox4x32(uint32_t(block), uint32_t(block >> 32), uint32_t(at), uint32_t(at >> 32), uint32_t(seed), uint32_t(seed >> 32));
+  }
+  template <typename T>
+  __device__ T apply(uint32_t word, T x) const {
+    return T(word >= threshold ? R(x) * scale : fill);
+  }
+};
+
+template <typename T> constexpr int DROPOUT_UNIT = sizeof(T) == 2 ? 8 : 4;  // elements of 16 bytes, at least the four of one counter
+constexpr unsigned DROPOUT_UNITS = 2;                                       // of a thread
+
+// Contiguous elements; VEC: read and written 16 bytes at a time.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(BLOCK) void dropoutFlatKernel(const T* x, size_t elements, T* out, Dropout<wide_t<T>> d) {
+  constexpr int E = DROPOUT_UNIT<T>;
+  using P = Pack<T, E>;
+  const uint64_t at = d.offsetDevice ? *d.offsetDevice : d.offset;
+  const size_t units = (elements + E - 1) / E, tiles = (units + DROPOUT_UNITS * BLOCK - 1) / (DROPOUT_UNITS * BLOCK);
+  for (size_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const size_t first = tile * (DROPOUT_UNITS * BLOCK) + threadIdx.x;
+    P v[DROPOUT_UNITS];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      if (4 * b + i < elements) out[row * outStride + column] = T(r.w[i] >= threshold ? R(x[row * stride + column]) * scale : fill);
-      if (++column == width) column = 0, ++row;
+    for (unsigned i = 0; i < DROPOUT_UNITS; ++i) {
+      const size_t e = (first + i * BLOCK) * E;
+      if (VEC && e + E <= elements) v[i] = *reinterpret_cast<const P*>(x + e);
+      else
+#pragma unroll
+        for (int q = 0; q < E; ++q)
+          if (e + q < elements) v[i].v[q] = x[e + q];
+    }
+#pragma unroll
+    for (unsigned i = 0; i < DROPOUT_UNITS; ++i) {
+      const size_t e = (first + i * BLOCK) * E;
+      if (e >= elements) continue;
+#pragma unroll
+      for (int b = 0; b < E / 4; ++b) {
+        const Philox4 r = d.words(e / 4 + b, at);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[i].v[4 * b + q] = d.apply(r.w[q], v[i].v[4 * b + q]);
+      }
+      if (VEC && e + E <= elements) *reinterpret_cast<P*>(out + e) = v[i];
+      else
+#pragma unroll
+        for (int q = 0; q < E; ++q)
+          if (e + q < elements) out[e + q] = v[i].v[q];
     }
   }
+}
+
+// Rows that are not adjacent; VEC: widths, strides and addresses in multiples of four elements, so that a counter's four
+// elements are neighbours. Otherwise a counter whose elements lie in two rows is computed for both.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(BLOCK) void dropoutRowsKernel(const T* x, size_t n, size_t width, size_t stride, T* out, size_t outStride, RowShape shape,
+                                                           Dropout<wide_t<T>> d) {
+  const uint64_t at = d.offsetDevice ? *d.offsetDevice : d.offset;
+  const unsigned lane = threadIdx.x & ((1u << shape.shift) - 1);
+  forTiles(shape.tiles, gridDim.x, [&](size_t tile) {
+    const size_t row = tile * (BLOCK >> shape.shift) + (threadIdx.x >> shape.shift);
+    if (row >= n) return;
+    const size_t begin = row * width, end = begin + width;
+    const T* from = x + row * stride;
+    T* to = out + row * outStride;
+    for (size_t b = begin / 4 + lane; 4 * b < end; b += size_t(1) << shape.shift) {
+      const Philox4 r = d.words(b, at);
+      if constexpr (VEC) {
+        Pack<T, 4> v = *reinterpret_cast<const Pack<T, 4>*>(from + (4 * b - begin));
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v.v[q] = d.apply(r.w[q], v.v[q]);
+        *reinterpret_cast<Pack<T, 4>*>(to + (4 * b - begin)) = v;
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const size_t e = 4 * b + q;
+          if (e >= begin && e < end) to[e - begin] = d.apply(r.w[q], from[e - begin]);
+        }
+      }
+    }
+  });
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------
@@ -683,15 +858,37 @@ void withWeight(int weightDtype, Fn&& fn) {
   fn(float());
 }
 
-void clearRows(const int32_t* starts, const int32_t* counts, unsigned experts, size_t capacity, size_t rowBytes, void* out, hipStream_t stream) {
-  if (capacity == 0 || rowBytes == 0) return;
-  clearKernel<<<clearBlocks(capacity, rowBytes), BLOCK, 0, stream>>>(starts, counts, experts, capacity, rowBytes, static_cast<unsigned char*>(out));
-  launched("clearing unused rows");
+// Clearing rides along with the kernel that writes the used rows: its blocks follow that kernel's.
+Unused unusedRows(unsigned rowBlocks, const int32_t* starts, const int32_t* counts, unsigned experts, size_t capacity, size_t rowBytes, void* out) {
+  Unused u{rowBlocks, 0, starts, counts, experts, capacity, rowBytes, static_cast<unsigned char*>(out)};
+  if (out && capacity && rowBytes) u.blocks = clearBlocks(capacity, rowBytes);
+  return u;
+}
+
+// calls fn(KB, ONE): slots are taken KB at a time; ONE says that this is all of them
+template <typename Fn>
+void withChoices(unsigned k, Fn&& fn) {
+  if (k == 1) return fn(std::integral_constant<int, 1>(), std::true_type());
+  if (k == 2) return fn(std::integral_constant<int, 2>(), std::true_type());
+  if (k <= 4) return fn(std::integral_constant<int, 4>(), std::true_type());
+  if (k <= 8) return fn(std::integral_constant<int, 8>(), std::true_type());
+  fn(std::integral_constant<int, 8>(), std::false_type());
 }
 
 void checkSegments(const int32_t* starts, const int32_t* counts, unsigned experts) {
   checkExperts(experts);
   if (!starts || !counts) refuse("null argument");
+}
+
+// calls fn(K): K slots a row read as one piece each of positions and weights, or 0 for any number and alignment
+template <typename W, typename Fn>
+void withLogChoices(unsigned k, const void* position, const void* weight, const void* gradWeight, Fn&& fn) {
+  const uintptr_t bits = address(position) | address(weight) | address(gradWeight);
+  if (k == 1) return fn(std::integral_constant<int, 1>());
+  if (k == 2 && bits % (2 * sizeof(W)) == 0) return fn(std::integral_constant<int, 2>());
+  if (k == 4 && bits % 16 == 0) return fn(std::integral_constant<int, 4>());
+  if (k == 8 && bits % 16 == 0) return fn(std::integral_constant<int, 8>());
+  fn(std::integral_constant<int, 0>());
 }
 
 void checkLogTypes(int dtype, int weightDtype) {
@@ -751,7 +948,7 @@ int spnc_hip_gate_backward(const void* logits, int dtype, size_t n, unsigned exp
 }
 
 size_t spnc_hip_route_workspace(size_t slots, unsigned experts) {
-  const RouteShape shape = routeShape(slots);
+  const RouteShape shape = routeShape(slots, experts);
   return shape.blocks <= 1 ? 0 : size_t(shape.blocks) * experts * sizeof(uint32_t);
 }
 
@@ -763,7 +960,7 @@ int spnc_hip_route(const int32_t* index, size_t slots, unsigned experts, unsigne
     if (slots >= (size_t(1) << 31) || slots + size_t(experts) * (align - 1) >= (size_t(1) << 31))
       refuse("too many slots: slots + experts * (align - 1) must be below 2^31");
     if ((slots && (!index || !position)) || !starts || !counts) refuse("null argument");
-    const RouteShape shape = routeShape(slots);
+    const RouteShape shape = routeShape(slots, experts);
     const size_t need = spnc_hip_route_workspace(slots, experts);
     if (workspace_bytes < need || (need && !workspace)) refuse("the workspace must hold " + std::to_string(need) + " bytes");
     unsigned bits = 0;
@@ -794,14 +991,17 @@ int spnc_hip_dispatch(const void* rows, size_t n, size_t row_bytes, size_t strid
     if (capacity == 0 || row_bytes == 0) return;
     if (!out || (n && (!rows || !position))) refuse("null argument");
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (zero_unused) clearRows(starts, counts, experts, capacity, row_bytes, out, s);
-    if (n == 0) return;
     const unsigned piece = pieceBytes(1, {address(rows), address(out), row_bytes, stride_bytes});
     const RowShape shape = rowShape(n, row_bytes, piece);
+    const Unused unused = unusedRows(tileGrid(shape.tiles), starts, counts, experts, capacity, row_bytes, zero_unused ? out : nullptr);
+    if (unused.rowBlocks + unused.blocks == 0) return;
     withPieces(piece, [&](auto p) {
       using P = decltype(p);
-      dispatchKernel<P><<<tileGrid(shape.tiles), BLOCK, 0, s>>>(static_cast<const unsigned char*>(rows), n, stride_bytes, shape, position, k, capacity,
-                                                               static_cast<P*>(out));
+      withChoices(k, [&](auto kb, auto) {
+        constexpr int KB = decltype(kb)::value;
+        dispatchKernel<P, KB><<<unused.rowBlocks + unused.blocks, BLOCK, 0, s>>>(static_cast<const unsigned char*>(rows), n, stride_bytes, shape, position,
+                                                                                 k, capacity, static_cast<P*>(out), unused);
+      });
     });
     launched("dispatch");
   });
@@ -825,8 +1025,10 @@ int spnc_hip_combine(const void* values, int dtype, size_t capacity, size_t widt
         constexpr int N = decltype(count)::value;
         withWeight<T>(weight_dtype, [&](auto w) {
           using W = decltype(w);
-          combineKernel<T, N, W><<<tileGrid(shape.tiles), BLOCK, 0, static_cast<hipStream_t>(stream)>>>(
-              static_cast<const T*>(values), capacity, stride, shape, position, n, k, static_cast<const W*>(weight), static_cast<Pack<T, N>*>(out));
+          withChoices(k, [&](auto kb, auto one) {
+            combineKernel<T, N, W, decltype(kb)::value, decltype(one)::value><<<tileGrid(shape.tiles), BLOCK, 0, static_cast<hipStream_t>(stream)>>>(
+                static_cast<const T*>(values), capacity, stride, shape, position, n, k, static_cast<const W*>(weight), static_cast<Pack<T, N>*>(out));
+          });
         });
       });
     });
@@ -844,22 +1046,25 @@ int spnc_hip_combine_backward(const void* values, int dtype, size_t capacity, si
     if (width * bytes >> 32) refuse("a row must be shorter than 4 GiB");
     if (grad_values) checkSegments(starts, counts, experts);
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (grad_values) clearRows(starts, counts, experts, capacity, width * bytes, grad_values, s);
-    if (n == 0 || (!grad_values && !grad_weight)) return;
-    if ((capacity && width && !values) || !position || !weight || (width && !grad_out)) refuse("null argument");
+    if (!grad_values && !grad_weight) return;
+    if (n && ((capacity && width && !values) || !position || !weight || (width && !grad_out))) refuse("null argument");
     const unsigned piece = pieceBytes(unsigned(bytes), {address(values), address(grad_out), address(grad_values), width * bytes, stride * bytes,
                                                         grad_stride * bytes});
     checkAligned(piece, "combine gradient");
     const RowShape shape = rowShape(n, width * bytes, piece);
+    const Unused unused = unusedRows(tileGrid(shape.tiles), starts, counts, experts, capacity, width * bytes, grad_values);
+    if (unused.rowBlocks + unused.blocks == 0) return;
     withType(dtype, [&](auto t) {
       using T = decltype(t);
       withPack<T>(piece, [&](auto count) {
         constexpr int N = decltype(count)::value;
         withWeight<T>(weight_dtype, [&](auto w) {
           using W = decltype(w);
-          combineBackwardKernel<T, N, W><<<tileGrid(shape.tiles), BLOCK, 0, s>>>(
-              static_cast<const T*>(values), capacity, stride, shape, position, n, k, static_cast<const W*>(weight), static_cast<const T*>(grad_out),
-              grad_stride, static_cast<Pack<T, N>*>(grad_values), static_cast<W*>(grad_weight));
+          withChoices(k, [&](auto kb, auto) {
+            combineBackwardKernel<T, N, W, decltype(kb)::value><<<unused.rowBlocks + unused.blocks, BLOCK, 0, s>>>(
+                static_cast<const T*>(values), capacity, stride, shape, position, n, k, static_cast<const W*>(weight), static_cast<const T*>(grad_out),
+                grad_stride, static_cast<Pack<T, N>*>(grad_values), static_cast<W*>(grad_weight), unused);
+          });
         });
       });
     });
@@ -877,8 +1082,10 @@ int spnc_hip_combine_log(const void* values, int dtype, size_t capacity, const i
     withLogTypes(dtype, weight_dtype, [&](auto r, auto w) {
       using R = decltype(r);
       using W = decltype(w);
-      const LogTerms<R, W> terms{static_cast<const R*>(values), capacity, position, static_cast<const W*>(log_weight)};
-      combineLogKernel<R, W><<<tileGrid((n + BLOCK - 1) / BLOCK), BLOCK, 0, static_cast<hipStream_t>(stream)>>>(terms, n, k, static_cast<R*>(out));
+      withLogChoices<W>(k, position, log_weight, nullptr, [&](auto kb) {
+        combineLogKernel<R, W, decltype(kb)::value><<<tileGrid((n + BLOCK - 1) / BLOCK), BLOCK, 0, static_cast<hipStream_t>(stream)>>>(
+            static_cast<const R*>(values), capacity, position, static_cast<const W*>(log_weight), n, k, static_cast<R*>(out));
+      });
     });
     launched("combine_log");
   });
@@ -892,15 +1099,19 @@ int spnc_hip_combine_log_backward(const void* values, int dtype, size_t capacity
     checkSlots(n, k, capacity);
     if (grad_values) checkSegments(starts, counts, experts);
     const hipStream_t s = static_cast<hipStream_t>(stream);
-    if (grad_values) clearRows(starts, counts, experts, capacity, elementBytes(dtype), grad_values, s);
-    if (n == 0 || (!grad_values && !grad_log_weight)) return;
-    if ((capacity && !values) || !position || !log_weight || !grad_out) refuse("null argument");
+    if (!grad_values && !grad_log_weight) return;
+    if (n && ((capacity && !values) || !position || !log_weight || !grad_out)) refuse("null argument");
+    const Unused unused =
+        unusedRows(tileGrid((n + BLOCK - 1) / BLOCK), starts, counts, experts, capacity, elementBytes(dtype), grad_values);
+    if (unused.rowBlocks + unused.blocks == 0) return;
     withLogTypes(dtype, weight_dtype, [&](auto r, auto w) {
       using R = decltype(r);
       using W = decltype(w);
-      const LogTerms<R, W> terms{static_cast<const R*>(values), capacity, position, static_cast<const W*>(log_weight)};
-      combineLogBackwardKernel<R, W><<<tileGrid((n + BLOCK - 1) / BLOCK), BLOCK, 0, s>>>(terms, n, k, static_cast<const R*>(grad_out),
-                                                                                       static_cast<R*>(grad_values), static_cast<W*>(grad_log_weight));
+      withLogChoices<W>(k, position, log_weight, grad_log_weight, [&](auto kb) {
+        combineLogBackwardKernel<R, W, decltype(kb)::value><<<unused.rowBlocks + unused.blocks, BLOCK, 0, s>>>(
+            static_cast<const R*>(values), capacity, position, static_cast<const W*>(log_weight), n, k, static_cast<const R*>(grad_out),
+            static_cast<R*>(grad_values), static_cast<W*>(grad_log_weight), unused);
+      });
     });
     launched("combine_log gradient");
   });
@@ -918,12 +1129,27 @@ int spnc_hip_dropout(const void* x, int dtype, size_t n, size_t width, size_t st
     const uint64_t threshold = uint64_t(std::llrint(p * 4294967296.0));
     const double scale = mode != SPNC_HIP_DROPOUT_ZERO ? 1.0 : threshold >> 32 ? 0.0 : 1.0 / (1.0 - p);
     const double fill = mode == SPNC_HIP_DROPOUT_MARGINAL ? NAN : 0.0;
-    const size_t blocks = ((n * width + 3) / 4 + BLOCK - 1) / BLOCK;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
     withType(dtype, [&](auto t) {
       using T = decltype(t);
       using R = wide_t<T>;
-      dropoutKernel<T><<<unsigned(blocks < MAX_GRID ? blocks : MAX_GRID), BLOCK, 0, static_cast<hipStream_t>(stream)>>>(
-          static_cast<const T*>(x), n, width, stride, static_cast<T*>(out), out_stride, threshold, R(scale), R(fill), seed, offset, offset_device);
+      const Dropout<R> d{threshold, R(scale), R(fill), seed, offset, offset_device};
+      const uintptr_t bits = address(x) | address(out);
+      if (n == 1 || (stride == width && out_stride == width)) {
+        constexpr int E = DROPOUT_UNIT<T>;
+        const size_t elements = n * width, units = (elements + E - 1) / E, blocks = (units + DROPOUT_UNITS * BLOCK - 1) / (DROPOUT_UNITS * BLOCK);
+        const unsigned grid = unsigned(blocks < MAX_GRID ? blocks : MAX_GRID);
+        if (bits % (sizeof(Pack<T, E>) < 16 ? sizeof(Pack<T, E>) : 16) == 0)
+          dropoutFlatKernel<T, true><<<grid, BLOCK, 0, s>>>(static_cast<const T*>(x), elements, static_cast<T*>(out), d);
+        else
+          dropoutFlatKernel<T, false><<<grid, BLOCK, 0, s>>>(static_cast<const T*>(x), elements, static_cast<T*>(out), d);
+      } else {
+        const RowShape shape = rowShape(n, (width + 3) / 4, 1);
+        if (((width | stride | out_stride) % 4 | bits % (4 * sizeof(T) < 16 ? 4 * sizeof(T) : 16)) == 0)
+          dropoutRowsKernel<T, true><<<tileGrid(shape.tiles), BLOCK, 0, s>>>(static_cast<const T*>(x), n, width, stride, static_cast<T*>(out), out_stride, shape, d);
+        else
+          dropoutRowsKernel<T, false><<<tileGrid(shape.tiles), BLOCK, 0, s>>>(static_cast<const T*>(x), n, width, stride, static_cast<T*>(out), out_stride, shape, d);
+      }
     });
     launched("dropout");
   });
