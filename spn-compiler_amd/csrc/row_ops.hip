@@ -43,24 +43,91 @@ unsigned tileGrid(size_t tiles) {
   return unsigned(g < MAX_GRID ? g : MAX_GRID);
 }
 
+// ---- lanes ----------------------------------------------------------------------------------------------------------
+
+// For a lane, its word and that of the lane it is paired with at distance D, in an order that is the same for both lanes or
+// does not matter to a symmetric operation. D = 4 and 8 mirror instead of exchanging: all lanes at smaller distances must hold the
+// same already. Vector instructions throughout (DPP, and row swaps of gfx950 for 16 and 32), no LDS.
+template <int D>
+__device__ inline void lanePair(uint32_t x, uint32_t& a, uint32_t& b) {
+  if constexpr (D <= 8) {
+    constexpr int control = D == 1 ? 0xB1 : D == 2 ? 0x4E : D == 4 ? 0x141 : 0x140;  // quad_perm, half row and row mirror
+    a = x;
+    b = uint32_t(__builtin_amdgcn_update_dpp(0, int(x), control, 0xF, 0xF, true));
+  } else if constexpr (D == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    a = r[0], b = r[1];
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    a = r[0], b = r[1];
+  }
+}
+
+template <int D, int G, typename R, typename Op>
+__device__ inline R groupFrom(R x, Op op) {
+  if constexpr (D >= G) {
+    return x;
+  } else {
+    R a, b;
+    if constexpr (sizeof(R) == 4) {
+      uint32_t wa, wb;
+      lanePair<D>(__builtin_bit_cast(uint32_t, x), wa, wb);
+      a = __builtin_bit_cast(R, wa), b = __builtin_bit_cast(R, wb);
+    } else {
+      const uint64_t w = __builtin_bit_cast(uint64_t, x);
+      uint32_t la, lb, ha, hb;
+      lanePair<D>(uint32_t(w), la, lb);
+      lanePair<D>(uint32_t(w >> 32), ha, hb);
+      a = __builtin_bit_cast(R, uint64_t(ha) << 32 | la), b = __builtin_bit_cast(R, uint64_t(hb) << 32 | lb);
+    }
+    return groupFrom<D * 2, G>(op(a, b), op);
+  }
+}
+
+// The sum, maximum or minimum over a group of G lanes, in all of them.
+template <int G, typename R> __device__ inline R groupSum(R x) {
+  return groupFrom<1, G>(x, [](R a, R b) { return a + b; });
+}
+template <int G, typename R> __device__ inline R groupMax(R x) {
+  return groupFrom<1, G>(x, [](R a, R b) { return a > b ? a : b; });
+}
+template <int G, typename R> __device__ inline R groupMin(R x) {
+  return groupFrom<1, G>(x, [](R a, R b) { return a < b ? a : b; });
+}
+
+// exp(x): x log2(e) in two parts, the hardware's exp2 of the first, the second as a factor 1 + r ln 2. Within two units in the
+// last place; below exp(-87) the result is 0.
+__device__ inline float expOf(float x) {
+  x = x < -200.0f ? -200.0f : x;  // minus infinity has no second part
+  const float t = x * 1.44269502f, r = __builtin_fmaf(x, 1.92596299e-8f, __builtin_fmaf(x, 1.44269502f, -t));
+  const float y = __builtin_amdgcn_exp2f(t);
+  return __builtin_fmaf(y, r * 0.693147182f, y);
+}
+__device__ inline double expOf(double x) { return exp(x); }
+__device__ inline float logOf(float x) { return logf(x); }
+__device__ inline double logOf(double x) { return log(x); }
+
 // ---- gate -----------------------------------------------------------------------------------------------------------
 
-// Unsigned keys in the order of the values: NaN above everything, both zeros the same, 0 for "no value".
-template <typename R> struct Order;
-template <> struct Order<float> {
+// Unsigned keys in the order of the values: NaN above everything, both zeros the same, 0 for "no value". Keys of 16-bit types
+// carry the expert below the value, descending, so that one maximum finds both; 26 bits in all.
+template <typename T> struct GateKey;
+template <> struct GateKey<float> {
   using key = uint32_t;
-  __device__ static key of(float x) {
+  static constexpr bool packed = false;
+  __device__ static key of(float x, unsigned) {
     const uint32_t u = __float_as_uint(x + 0.0f);
     return x != x ? 0xFFFFFFFFu : (u & 0x80000000u) ? ~u : u | 0x80000000u;
   }
   __device__ static float value(key k) {
     return k == 0xFFFFFFFFu ? __uint_as_float(0x7FC00000u) : __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
   }
-  static constexpr key closed = 0x007FFFFFu;  // of minus infinity
+  __device__ static bool open(key k) { return k > 0x007FFFFFu; }  // above minus infinity
 };
-template <> struct Order<double> {
+template <> struct GateKey<double> {
   using key = uint64_t;
-  __device__ static key of(double x) {
+  static constexpr bool packed = false;
+  __device__ static key of(double x, unsigned) {
     const uint64_t u = uint64_t(__double_as_longlong(x + 0.0));
     return x != x ? ~0ull : (u >> 63) ? ~u : u | (1ull << 63);
   }
@@ -68,151 +135,205 @@ template <> struct Order<double> {
     if (k == ~0ull) return __longlong_as_double(0x7FF8000000000000ll);
     return __longlong_as_double((long long)((k >> 63) ? k ^ (1ull << 63) : ~k));
   }
-  static constexpr key closed = 0x000FFFFFFFFFFFFFull;
+  __device__ static bool open(key k) { return k > 0x000FFFFFFFFFFFFFull; }
 };
-
-template <int G, typename R>
-__device__ inline R groupSum(R x) {
-#pragma unroll
-  for (int d = 1; d < G; d *= 2) x += __shfl_xor(x, d);
-  return x;
-}
-
-template <int G, typename R>
-__device__ inline R groupMax(R x) {
-#pragma unroll
-  for (int d = 1; d < G; d *= 2) {
-    const R y = __shfl_xor(x, d);
-    x = y > x ? y : x;
+template <typename T, uint32_t INF> struct GateKey16 {
+  using key = uint32_t;
+  static constexpr bool packed = true;
+  __device__ static key of(T x, unsigned e) {
+    uint32_t u = __builtin_bit_cast(uint16_t, x);
+    const bool nan = (u & 0x7FFFu) > INF;
+    u = u == 0x8000u ? 0u : u;
+    u = nan ? 0xFFFFu : (u & 0x8000u) ? u ^ 0xFFFFu : u | 0x8000u;
+    return u << 10 | (1023u - e);
   }
-  return x;
+  __device__ static float value(key k) {
+    const uint32_t u = k >> 10;
+    const float x = float(__builtin_bit_cast(T, uint16_t((u & 0x8000u) ? u ^ 0x8000u : u ^ 0xFFFFu)));
+    return u == 0xFFFFu ? __uint_as_float(0x7FC00000u) : x;
+  }
+  __device__ static bool open(key k) { return k >> 10 > (INF ^ 0x7FFFu); }
+};
+template <> struct GateKey<__bf16> : GateKey16<__bf16, 0x7F80u> {};
+template <> struct GateKey<_Float16> : GateKey16<_Float16, 0x7C00u> {};
+
+// The expert of a lane's i-th logit. VEC: read four at a time.
+template <int G, bool VEC>
+__device__ inline unsigned gateExpert(int i, unsigned lane) {
+  return VEC ? (i / 4) * (4 * G) + 4 * lane + i % 4 : i * G + lane;
 }
 
-// G lanes hold a row, V logits each; k rounds of a maximum over the group, lane j keeps the choice of round j.
-template <typename T, int G, int V>
+template <typename T, int G, int V, bool VEC>
+__device__ inline void gateLoad(const T* row, unsigned experts, unsigned lane, T (&z)[V]) {
+#pragma unroll
+  for (int i = 0; i < V; i += VEC ? 4 : 1) {
+    const unsigned e = gateExpert<G, VEC>(i, lane);
+    if constexpr (VEC) {
+      if (e < experts) {
+        const Pack<T, 4> p = *reinterpret_cast<const Pack<T, 4>*>(row + e);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) z[i + q] = p.v[q];
+      }
+    } else if (e < experts) {
+      z[i] = row[e];
+    }
+  }
+}
+
+// G lanes hold a row, V logits each. k rounds: the largest key of the group, the lowest expert that has it, and out it goes; lane
+// j keeps the choice of round j. The whole row is in registers, so the logits are read once.
+template <typename T, int G, int V, bool VEC>
 __global__ __launch_bounds__(BLOCK) void gateKernel(const T* __restrict__ logits, size_t n, unsigned experts, size_t stride, unsigned k,
                                                     unsigned flags, int32_t* __restrict__ index, wide_t<T>* __restrict__ weight) {
   using R = wide_t<T>;
-  using O = Order<R>;
+  using O = GateKey<T>;
   using K = typename O::key;
   const unsigned lane = threadIdx.x % G;
   forTiles((n + BLOCK / G - 1) / (BLOCK / G), gridDim.x, [&](size_t tile) {
     const size_t row = tile * (BLOCK / G) + threadIdx.x / G;
-    if (row >= n) return;  // whole groups leave; shuffles stay inside a group
+    if (row >= n) return;  // whole groups leave; lanes are paired inside a group
+    T z[V];
     K key[V];
+    gateLoad<T, G, V, VEC>(logits + row * stride, experts, lane, z);
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-      const unsigned e = i * G + lane;
-      key[i] = e < experts ? O::of(R(logits[row * stride + e])) : K(0);
+      const unsigned e = gateExpert<G, VEC>(i, lane);
+      key[i] = e < experts ? O::of(z[i], e) : K(0);
     }
-    K myKey = 0, topKey = 0;
+    K myKey = 0, topKey = 0, last = 0;
     unsigned myIndex = 0;
     R total = 0;
     for (unsigned j = 0; j < k; ++j) {
       K best = 0;
       unsigned at = 0;
+      if constexpr (O::packed) {
+        // Keys are distinct and have 26 bits: modulo 2^32, key - last is above 2^31 for keys below the last choice and below 2^26
+        // for the others, so its maximum belongs to the largest key below, and nothing has to be taken out.
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (key[i] > best) best = key[i], at = i * G + lane;
+        for (int i = 0; i < V; ++i) {
+          const K below = j == 0 ? key[i] : key[i] - last;
+          best = below > best ? below : best;
+        }
+        best = groupMax<G>(best);
+        best = j == 0 ? best : best >> 31 ? best + last : K(0);
+        last = best ? best : last;
+        at = 1023u - (best & 1023u);
+      } else {
 #pragma unroll
-      for (int d = 1; d < G; d *= 2) {
-        const K otherKey = __shfl_xor(best, d);
-        const unsigned otherAt = __shfl_xor(at, d);
-        if (otherKey > best || (otherKey == best && otherAt < at)) best = otherKey, at = otherAt;
+        for (int i = 0; i < V; ++i) best = key[i] > best ? key[i] : best;
+        best = groupMax<G>(best);
+        at = ~0u;
+#pragma unroll
+        for (int i = V - 1; i >= 0; --i) at = key[i] == best ? gateExpert<G, VEC>(i, lane) : at;
+        at = groupMin<G>(at);
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+          if (gateExpert<G, VEC>(i, lane) == at) key[i] = 0;
       }
       if (j == 0) {
         topKey = best;
-        if ((flags & SPNC_HIP_GATE_ALL) && best > O::closed) {
+        if ((flags & SPNC_HIP_GATE_ALL) && O::open(best)) {
           const R top = O::value(best);
 #pragma unroll
-          for (int i = 0; i < V; ++i)
-            if (key[i] > O::closed) total += std::is_same<R, double>::value ? R(exp(double(O::value(key[i]) - top))) : R(expf(float(O::value(key[i]) - top)));
+          for (int i = 0; i < V; ++i) {
+            const unsigned e = gateExpert<G, VEC>(i, lane);
+            if (e < experts && R(z[i]) != -INFINITY) total += expOf(R(z[i]) - top);
+          }
           total = groupSum<G>(total);
         }
       }
       if (lane == j) myKey = best, myIndex = at;
-#pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (unsigned(i * G) + lane == at) key[i] = 0;
     }
-    const bool open = lane < k && myKey > O::closed;
-    const R top = O::value(topKey), mine = O::value(myKey);
-    const R shifted = open ? mine - top : R(0);
-    const R e = open ? (std::is_same<R, double>::value ? R(exp(double(shifted))) : R(expf(float(shifted)))) : R(0);
+    const bool open = lane < k && O::open(myKey);
+    const R shifted = open ? O::value(myKey) - O::value(topKey) : R(0);
+    const R e = open ? expOf(shifted) : R(0);
     if (!(flags & SPNC_HIP_GATE_ALL)) total = groupSum<G>(e);
     if (lane < k) {
       index[row * k + lane] = open ? int32_t(myIndex) : -1;
-      R w;
-      if (flags & SPNC_HIP_GATE_LOG) {
-        const R l = std::is_same<R, double>::value ? R(log(double(total))) : R(logf(float(total)));
-        w = open ? shifted - l : -INFINITY;
-      } else {
-        w = open ? e / total : R(0);
-      }
-      weight[row * k + lane] = w;
+      weight[row * k + lane] = (flags & SPNC_HIP_GATE_LOG) ? (open ? shifted - logOf(total) : R(-INFINITY)) : open ? e / total : R(0);
     }
   });
 }
 
-template <typename T, int G, int V>
+// dz_e of the experts that were not chosen is 0, or -p_e times the sum over the slots under "all"; the k chosen ones get their
+// slot's term on top, through LDS: every lane has V of the row's entries in registers, and a slot's expert may be any of them.
+template <typename T, int G, int V, bool VEC>
 __global__ __launch_bounds__(BLOCK) void gateBackwardKernel(const T* __restrict__ logits, size_t n, unsigned experts, size_t stride, unsigned k,
                                                             unsigned flags, const int32_t* __restrict__ index, const wide_t<T>* __restrict__ weight,
                                                             const wide_t<T>* __restrict__ gradWeight, T* __restrict__ gradLogits) {
   using R = wide_t<T>;
+  __shared__ R entries[BLOCK / G][V * G];
   const unsigned lane = threadIdx.x % G;
+  R* const mine = entries[threadIdx.x / G];
   const bool all = flags & SPNC_HIP_GATE_ALL, logs = flags & SPNC_HIP_GATE_LOG;
   forTiles((n + BLOCK / G - 1) / (BLOCK / G), gridDim.x, [&](size_t tile) {
     const size_t row = tile * (BLOCK / G) + threadIdx.x / G;
     if (row >= n) return;
-    R share[V];  // of the experts, under "all"
-    R total = 0;
-    if (all) {
-      R z[V], top = -INFINITY;
-      bool bad = false;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        const unsigned e = i * G + lane;
-        z[i] = e < experts ? R(logits[row * stride + e]) : R(-INFINITY);
-        bad |= z[i] != z[i];
-        top = z[i] > top ? z[i] : top;
-      }
-      top = groupMax<G>(top);
-      if (groupMax<G>(int(bad))) top = NAN;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        share[i] = z[i] == -INFINITY ? R(0) : std::is_same<R, double>::value ? R(exp(double(z[i] - top))) : R(expf(float(z[i] - top)));
-        total += share[i];
-      }
-      total = groupSum<G>(total);
-    }
     int32_t at = -1;
     R d = 0, w = 0;
     if (lane < k) {
       at = index[row * k + lane];
+      if (at >= int32_t(experts)) at = -1;
       if (at >= 0) {
         d = gradWeight[row * k + lane];
         w = weight[row * k + lane];
-        if (logs) w = std::is_same<R, double>::value ? R(exp(double(w))) : R(expf(float(w)));
+        if (logs) w = w == -INFINITY ? R(0) : expOf(w);
         else d *= w;
       }
     }
+    R dz[V] = {};
+    R top = -INFINITY, total = 0;
+    if (all) {
+      T z[V];
+      gateLoad<T, G, V, VEC>(logits + row * stride, experts, lane, z);
+      int bad = 0;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        dz[i] = gateExpert<G, VEC>(i, lane) < experts ? R(z[i]) : R(-INFINITY);
+        bad |= dz[i] != dz[i];
+        top = dz[i] > top ? dz[i] : top;
+      }
+      top = groupMax<G>(top);
+      if (groupMax<G>(bad)) top = NAN;
+#pragma unroll
+      for (int i = 0; i < V; ++i) {
+        dz[i] = dz[i] == -INFINITY ? R(0) : expOf(dz[i] - top);
+        total += dz[i];
+      }
+      total = groupSum<G>(total);
+    }
     const R common = groupSum<G>(d);
-    if (!all && at >= 0) d -= w * common;
-    R dz[V];
+    if (!all) d -= w * common;
+    const R factor = total == 0 ? R(0) : -common / total;
 #pragma unroll
-    for (int i = 0; i < V; ++i) dz[i] = all && total > 0 ? -(share[i] / total) * common : all && total != total ? total : R(0);
-    for (unsigned j = 0; j < k; ++j) {
-      const int32_t target = __shfl(at, int(j), G);
-      const R value = __shfl(d, int(j), G);
+    for (int i = 0; i < V; i += VEC ? 4 : 1) {
+      const unsigned e = gateExpert<G, VEC>(i, lane);
+      if constexpr (VEC) {
+        Pack<R, 4> p;
 #pragma unroll
-      for (int i = 0; i < V; ++i)
-        if (target == int32_t(i * G + lane)) dz[i] += value;
+        for (int q = 0; q < 4; ++q) p.v[q] = dz[i + q] * factor;
+        *reinterpret_cast<Pack<R, 4>*>(mine + e) = p;
+      } else {
+        mine[e] = dz[i] * factor;
+      }
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the group is part of one wave, whose LDS accesses stay in order
+    if (at >= 0) mine[at] += d;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const unsigned e = i * G + lane;
-      if (e < experts) gradLogits[row * experts + e] = T(dz[i]);
+    for (int i = 0; i < V; i += VEC ? 4 : 1) {
+      const unsigned e = gateExpert<G, VEC>(i, lane);
+      if constexpr (VEC) {
+        const Pack<R, 4> p = *reinterpret_cast<const Pack<R, 4>*>(mine + e);
+        Pack<T, 4> o;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) o.v[q] = T(p.v[q]);
+        if (e < experts) *reinterpret_cast<Pack<T, 4>*>(gradLogits + row * experts + e) = o;
+      } else if (e < experts) {
+        gradLogits[row * experts + e] = T(mine[e]);
+      }
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   });
 }
 
@@ -530,8 +651,6 @@ __global__ __launch_bounds__(BLOCK) void combineBackwardKernel(const T* __restri
 // The largest value of the row's slots is taken out before its log weight is added: values of some thousands differ by
 // little, and the difference is exact where the sum would be rounded. Shares are computed from the same terms, not from the
 // rounded result.
-template <typename R> __device__ inline R expOf(R x) { return std::is_same<R, double>::value ? R(exp(double(x))) : R(expf(float(x))); }
-template <typename R> __device__ inline R logOf(R x) { return std::is_same<R, double>::value ? R(log(double(x))) : R(logf(float(x))); }
 
 // A row's slots. K > 0: held in registers, read as one piece each of positions and weights; K = 0: read again for every use.
 template <typename R, typename W, int K>
@@ -597,7 +716,7 @@ __device__ inline void logSum(const LogTerms<R, W, K>& terms, size_t row, R& pea
     }
 #pragma unroll
   for (unsigned j = 0; j < terms.count(); ++j)
-    if (terms.slot(row, j, v, lw)) total += expOf<R>(lw + (v - peak) - shift);
+    if (terms.slot(row, j, v, lw)) total += expOf(lw + (v - peak) - shift);
 }
 
 template <typename R, typename W, int K>
@@ -610,7 +729,7 @@ __global__ __launch_bounds__(BLOCK) void combineLogKernel(const R* __restrict__ 
     terms.load(row);
     R peak, shift, total;
     logSum(terms, row, peak, shift, total);
-    out[row] = peak == -INFINITY || peak == INFINITY ? peak : peak + (shift + logOf<R>(total));
+    out[row] = peak == -INFINITY || peak == INFINITY ? peak : peak + (shift + logOf(total));
   });
 }
 
@@ -632,7 +751,7 @@ __global__ __launch_bounds__(BLOCK) void combineLogBackwardKernel(const R* __res
 #pragma unroll
       for (int j = 0; j < K; ++j) {
         R v, lw, share = 0;
-        if (peak != -INFINITY && terms.slot(row, j, v, lw)) share = g * (expOf<R>(lw + (v - peak) - shift) / total);
+        if (peak != -INFINITY && terms.slot(row, j, v, lw)) share = g * (expOf(lw + (v - peak) - shift) / total);
         if (gradValues && terms.at[j] >= 0) gradValues[terms.at[j]] = share;
         o.v[j] = W(share);
       }
@@ -642,7 +761,7 @@ __global__ __launch_bounds__(BLOCK) void combineLogBackwardKernel(const R* __res
         const size_t s = row * k + j;
         R v, lw, share = 0;
         int32_t p;
-        if (terms.read(s, v, lw, p) && peak != -INFINITY) share = g * (expOf<R>(lw + (v - peak) - shift) / total);
+        if (terms.read(s, v, lw, p) && peak != -INFINITY) share = g * (expOf(lw + (v - peak) - shift) / total);
         if (gradValues && p >= 0) gradValues[p] = share;
         if (gradLogWeight) gradLogWeight[s] = W(share);
       }
@@ -800,11 +919,14 @@ void checkWeightType(int dtype, int weightDtype) {
     refuse("weights must be float32, or float64 with float64 values");
 }
 
-template <typename Fn>
-void withGateShape(unsigned experts, unsigned k, Fn&& fn) {
+// calls fn(G, V, VEC): a row's logits in G lanes of V; at least as many lanes as choices, four logits a lane until 64 lanes are used
+template <typename T, typename Fn>
+void withGateShape(unsigned experts, unsigned k, size_t stride, uintptr_t addresses, Fn&& fn) {
   unsigned group = 1;
   while (group < WAVE && (4 * group < experts || group < k)) group *= 2;
-#define SPN_GATE_SHAPE(G, V) return fn(std::integral_constant<int, G>(), std::integral_constant<int, V>())
+  const bool vec = (experts | stride) % 4 == 0 && addresses % alignof(Pack<T, 4>) == 0;
+  auto shape = [&](auto g, auto v) { vec ? fn(g, v, std::true_type()) : fn(g, v, std::false_type()); };
+#define SPN_GATE_SHAPE(G, V) return shape(std::integral_constant<int, G>(), std::integral_constant<int, V>())
   switch (group) {
     case 1: SPN_GATE_SHAPE(1, 4);
     case 2: SPN_GATE_SHAPE(2, 4);
@@ -917,9 +1039,9 @@ int spnc_hip_gate(const void* logits, int dtype, size_t n, unsigned experts, siz
     if (!logits || !index || !weight) refuse("null argument");
     withType(dtype, [&](auto t) {
       using T = decltype(t);
-      withGateShape(experts, k, [&](auto g, auto v) {
+      withGateShape<T>(experts, k, stride, address(logits), [&](auto g, auto v, auto vec) {
         constexpr int G = decltype(g)::value, V = decltype(v)::value;
-        gateKernel<T, G, V><<<tileGrid((n + BLOCK / G - 1) / (BLOCK / G)), BLOCK, 0, static_cast<hipStream_t>(stream)>>>(
+        gateKernel<T, G, V, decltype(vec)::value><<<tileGrid((n + BLOCK / G - 1) / (BLOCK / G)), BLOCK, 0, static_cast<hipStream_t>(stream)>>>(
             static_cast<const T*>(logits), n, experts, stride, k, flags, index, static_cast<wide_t<T>*>(weight));
       });
     });
@@ -936,9 +1058,10 @@ int spnc_hip_gate_backward(const void* logits, int dtype, size_t n, unsigned exp
     withType(dtype, [&](auto t) {
       using T = decltype(t);
       using R = wide_t<T>;
-      withGateShape(experts, k, [&](auto g, auto v) {
+      withGateShape<T>(experts, k, (flags & SPNC_HIP_GATE_ALL) ? stride : experts,
+                       address(grad_logits) | ((flags & SPNC_HIP_GATE_ALL) ? address(logits) : 0), [&](auto g, auto v, auto vec) {
         constexpr int G = decltype(g)::value, V = decltype(v)::value;
-        gateBackwardKernel<T, G, V><<<tileGrid((n + BLOCK / G - 1) / (BLOCK / G)), BLOCK, 0, static_cast<hipStream_t>(stream)>>>(
+        gateBackwardKernel<T, G, V, decltype(vec)::value><<<tileGrid((n + BLOCK / G - 1) / (BLOCK / G)), BLOCK, 0, static_cast<hipStream_t>(stream)>>>(
             static_cast<const T*>(logits), n, experts, stride, k, flags, index, static_cast<const R*>(weight), static_cast<const R*>(grad_weight),
             static_cast<T*>(grad_logits));
       });
