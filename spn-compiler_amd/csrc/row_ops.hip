@@ -29,6 +29,21 @@ struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack {
   T v[N];
 };
 
+// Accesses that are not kept in the caches. A piece of another size than 16 bytes goes the ordinary way.
+typedef uint32_t Words4 __attribute__((ext_vector_type(4)));
+
+template <typename P>
+__device__ inline P streamLoad(const P* p) {
+  if constexpr (sizeof(P) == 16) return __builtin_bit_cast(P, __builtin_nontemporal_load(reinterpret_cast<const Words4*>(p)));
+  else return *p;
+}
+
+template <typename P>
+__device__ inline void streamStore(P* p, const P& v) {
+  if constexpr (sizeof(P) == 16) __builtin_nontemporal_store(__builtin_bit_cast(Words4, v), reinterpret_cast<Words4*>(p));
+  else *p = v;
+}
+
 // Neighbouring tiles of rows go to one die: rows that are neighbours in the sorted buffer come from neighbouring rows,
 // and a cache line of narrow rows is then filled or read within one L2.
 template <typename Body>
@@ -466,19 +481,26 @@ __global__ __launch_bounds__(ROUTE_BLOCK) void routeKernel(const int32_t* __rest
 // ---- rows there and back --------------------------------------------------------------------------------------------
 
 // A group of 2^shift lanes handles a row, a piece of up to 16 bytes a lane at a time.
+//
+// Rows that are written to scattered places bypass the caches where they consist of whole 64-byte halves of cache lines: 1 M rows
+// of 64 bytes to two places each take 36 us instead of 50, of 2 KB to four places 52 instead of 67 (a consumer that reads
+// them next loses up to half of that where they would have fit the last-level cache). Rows that share their halves must not: 48
+// bytes take 87 us instead of 61, since each piece goes to memory by itself.
 struct RowShape {
   unsigned pieces;  // of a row
   unsigned shift;
   size_t tiles;
+  bool stream;      // scattered rows are written past the caches
 };
 
-RowShape rowShape(size_t n, size_t rowBytes, unsigned pieceBytes) {
+RowShape rowShape(size_t n, size_t rowBytes, unsigned pieceBytes, const void* scattered = nullptr) {
   RowShape s;
   s.pieces = unsigned(rowBytes / pieceBytes);
   s.shift = 0;
   while (s.shift < 6 && (1u << s.shift) < s.pieces) ++s.shift;
   const size_t rows = BLOCK >> s.shift;
   s.tiles = (n + rows - 1) / rows;
+  s.stream = pieceBytes == 16 && rowBytes % 64 == 0 && reinterpret_cast<uintptr_t>(scattered) % 64 == 0;
   return s;
 }
 
@@ -536,7 +558,7 @@ __device__ inline void loadWeights(const W* weight, size_t row, unsigned k, unsi
   for (int j = 0; j < KB; ++j) w[j] = !weight ? R(1) : first + j < k ? R(weight[row * k + first + j]) : R(0);
 }
 
-template <typename P, int KB>
+template <typename P, int KB, bool STREAM>
 __global__ __launch_bounds__(BLOCK) void dispatchKernel(const unsigned char* __restrict__ rows, size_t n, size_t strideBytes, RowShape shape,
                                                         const int32_t* __restrict__ position, unsigned k, size_t capacity, P* __restrict__ out,
                                                         Unused unused) {
@@ -553,14 +575,21 @@ __global__ __launch_bounds__(BLOCK) void dispatchKernel(const unsigned char* __r
         const P piece = source[c];
 #pragma unroll
         for (int j = 0; j < KB; ++j)
-          if (at[j] >= 0) out[size_t(at[j]) * shape.pieces + c] = piece;
+          if (at[j] >= 0) {
+            P* const to = &out[size_t(at[j]) * shape.pieces + c];
+            if constexpr (STREAM) streamStore(to, piece);
+            else *to = piece;
+          }
       }
     }
   });
 }
 
-// Slots are read KB at a time, all loads before the first product; a slot that is not routed reads row 0 and drops it.
-template <typename T, int N, typename W, int KB, bool ONE>
+// Slots are read KB at a time, all loads before the first product; a slot that is not routed reads row 0 and drops it. Results
+// bypass the caches, which leaves the values there for the backward pass (32769 x 4 rows of 2 KB, forward and backward: 164 us
+// instead of 191), and so do values without weights: gradients of dispatch, whose last use this is (139 instead of 150 us for the
+// whole of routing, dispatch and its gradient at that size).
+template <typename T, int N, typename W, int KB, bool ONE, bool WEIGHTED>
 __global__ __launch_bounds__(BLOCK) void combineKernel(const T* __restrict__ values, size_t capacity, size_t stride, RowShape shape,
                                                        const int32_t* __restrict__ position, size_t n, unsigned k, const W* __restrict__ weight,
                                                        Pack<T, N>* __restrict__ out) {
@@ -573,19 +602,22 @@ __global__ __launch_bounds__(BLOCK) void combineKernel(const T* __restrict__ val
     R w[KB];
     if (ONE) {
       loadPositions<KB>(position, row, k, 0, capacity, at);
-      loadWeights<KB>(weight, row, k, 0, w);
+      loadWeights<KB>(WEIGHTED ? weight : nullptr, row, k, 0, w);
     }
     for (unsigned c = lane; c < shape.pieces; c += 1u << shape.shift) {
       R sum[N] = {};
       for (unsigned first = 0; first < (ONE ? 1 : k); first += KB) {
         if (!ONE) {
           loadPositions<KB>(position, row, k, first, capacity, at);
-          loadWeights<KB>(weight, row, k, first, w);
+          loadWeights<KB>(WEIGHTED ? weight : nullptr, row, k, first, w);
         }
         Pack<T, N> v[KB];
 #pragma unroll
         for (int j = 0; j < KB; ++j)
-          if (capacity) v[j] = *reinterpret_cast<const Pack<T, N>*>(values + size_t(at[j] >= 0 ? at[j] : 0) * stride + size_t(c) * N);
+          if (capacity) {
+            const Pack<T, N>* from = reinterpret_cast<const Pack<T, N>*>(values + size_t(at[j] >= 0 ? at[j] : 0) * stride + size_t(c) * N);
+            v[j] = WEIGHTED ? *from : streamLoad(from);
+          }
 #pragma unroll
         for (int j = 0; j < KB; ++j)
 #pragma unroll
@@ -594,12 +626,12 @@ __global__ __launch_bounds__(BLOCK) void combineKernel(const T* __restrict__ val
       Pack<T, N> o;
 #pragma unroll
       for (int i = 0; i < N; ++i) o.v[i] = T(sum[i]);
-      out[row * shape.pieces + c] = o;
+      streamStore(&out[row * shape.pieces + c], o);
     }
   });
 }
 
-template <typename T, int N, typename W, int KB>
+template <typename T, int N, typename W, int KB, bool STREAM>
 __global__ __launch_bounds__(BLOCK) void combineBackwardKernel(const T* __restrict__ values, size_t capacity, size_t stride, RowShape shape,
                                                                const int32_t* __restrict__ position, size_t n, unsigned k,
                                                                const W* __restrict__ weight, const T* __restrict__ gradOut, size_t gradStride,
@@ -616,7 +648,7 @@ __global__ __launch_bounds__(BLOCK) void combineBackwardKernel(const T* __restri
       loadPositions<KB>(position, row, k, first, capacity, at);
       loadWeights<KB>(weight, row, k, first, w);
       for (unsigned c = lane; c < shape.pieces; c += group) {
-        const Pack<T, N> g = *reinterpret_cast<const Pack<T, N>*>(gradOut + row * gradStride + size_t(c) * N);
+        const Pack<T, N> g = streamLoad(reinterpret_cast<const Pack<T, N>*>(gradOut + row * gradStride + size_t(c) * N));
         if (gradWeight && capacity) {
           Pack<T, N> v[KB];
 #pragma unroll
@@ -633,7 +665,9 @@ __global__ __launch_bounds__(BLOCK) void combineBackwardKernel(const T* __restri
               Pack<T, N> o;
 #pragma unroll
               for (int i = 0; i < N; ++i) o.v[i] = T(w[j] * R(g.v[i]));
-              gradValues[size_t(at[j]) * shape.pieces + c] = o;
+              Pack<T, N>* const to = &gradValues[size_t(at[j]) * shape.pieces + c];
+              if constexpr (STREAM) streamStore(to, o);
+              else *to = o;
             }
         }
       }
@@ -987,6 +1021,14 @@ Unused unusedRows(unsigned rowBlocks, const int32_t* starts, const int32_t* coun
   return u;
 }
 
+// calls fn(STREAM); only 16-byte pieces are ever written past the caches
+template <size_t PIECE, typename Fn>
+void withStream(const RowShape& shape, Fn&& fn) {
+  if constexpr (PIECE == 16)
+    if (shape.stream) return fn(std::true_type());
+  fn(std::false_type());
+}
+
 // calls fn(KB, ONE): slots are taken KB at a time; ONE says that this is all of them
 template <typename Fn>
 void withChoices(unsigned k, Fn&& fn) {
@@ -1115,15 +1157,17 @@ int spnc_hip_dispatch(const void* rows, size_t n, size_t row_bytes, size_t strid
     if (!out || (n && (!rows || !position))) refuse("null argument");
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const unsigned piece = pieceBytes(1, {address(rows), address(out), row_bytes, stride_bytes});
-    const RowShape shape = rowShape(n, row_bytes, piece);
+    const RowShape shape = rowShape(n, row_bytes, piece, out);
     const Unused unused = unusedRows(tileGrid(shape.tiles), starts, counts, experts, capacity, row_bytes, zero_unused ? out : nullptr);
     if (unused.rowBlocks + unused.blocks == 0) return;
     withPieces(piece, [&](auto p) {
       using P = decltype(p);
       withChoices(k, [&](auto kb, auto) {
         constexpr int KB = decltype(kb)::value;
-        dispatchKernel<P, KB><<<unused.rowBlocks + unused.blocks, BLOCK, 0, s>>>(static_cast<const unsigned char*>(rows), n, stride_bytes, shape, position,
-                                                                                 k, capacity, static_cast<P*>(out), unused);
+        withStream<sizeof(P)>(shape, [&](auto stream) {
+          dispatchKernel<P, KB, decltype(stream)::value><<<unused.rowBlocks + unused.blocks, BLOCK, 0, s>>>(
+              static_cast<const unsigned char*>(rows), n, stride_bytes, shape, position, k, capacity, static_cast<P*>(out), unused);
+        });
       });
     });
     launched("dispatch");
@@ -1149,8 +1193,12 @@ int spnc_hip_combine(const void* values, int dtype, size_t capacity, size_t widt
         withWeight<T>(weight_dtype, [&](auto w) {
           using W = decltype(w);
           withChoices(k, [&](auto kb, auto one) {
-            combineKernel<T, N, W, decltype(kb)::value, decltype(one)::value><<<tileGrid(shape.tiles), BLOCK, 0, static_cast<hipStream_t>(stream)>>>(
-                static_cast<const T*>(values), capacity, stride, shape, position, n, k, static_cast<const W*>(weight), static_cast<Pack<T, N>*>(out));
+            auto launch = [&](auto weighted) {
+              combineKernel<T, N, W, decltype(kb)::value, decltype(one)::value, decltype(weighted)::value>
+                  <<<tileGrid(shape.tiles), BLOCK, 0, static_cast<hipStream_t>(stream)>>>(
+                      static_cast<const T*>(values), capacity, stride, shape, position, n, k, static_cast<const W*>(weight), static_cast<Pack<T, N>*>(out));
+            };
+            weight ? launch(std::true_type()) : launch(std::false_type());
           });
         });
       });
@@ -1174,7 +1222,7 @@ int spnc_hip_combine_backward(const void* values, int dtype, size_t capacity, si
     const unsigned piece = pieceBytes(unsigned(bytes), {address(values), address(grad_out), address(grad_values), width * bytes, stride * bytes,
                                                         grad_stride * bytes});
     checkAligned(piece, "combine gradient");
-    const RowShape shape = rowShape(n, width * bytes, piece);
+    const RowShape shape = rowShape(n, width * bytes, piece, grad_values);
     const Unused unused = unusedRows(tileGrid(shape.tiles), starts, counts, experts, capacity, width * bytes, grad_values);
     if (unused.rowBlocks + unused.blocks == 0) return;
     withType(dtype, [&](auto t) {
@@ -1184,9 +1232,11 @@ int spnc_hip_combine_backward(const void* values, int dtype, size_t capacity, si
         withWeight<T>(weight_dtype, [&](auto w) {
           using W = decltype(w);
           withChoices(k, [&](auto kb, auto) {
-            combineBackwardKernel<T, N, W, decltype(kb)::value><<<unused.rowBlocks + unused.blocks, BLOCK, 0, s>>>(
-                static_cast<const T*>(values), capacity, stride, shape, position, n, k, static_cast<const W*>(weight), static_cast<const T*>(grad_out),
-                grad_stride, static_cast<Pack<T, N>*>(grad_values), static_cast<W*>(grad_weight), unused);
+            withStream<sizeof(T) * N>(shape, [&](auto past) {
+              combineBackwardKernel<T, N, W, decltype(kb)::value, decltype(past)::value><<<unused.rowBlocks + unused.blocks, BLOCK, 0, s>>>(
+                  static_cast<const T*>(values), capacity, stride, shape, position, n, k, static_cast<const W*>(weight),
+                  static_cast<const T*>(grad_out), grad_stride, static_cast<Pack<T, N>*>(grad_values), static_cast<W*>(grad_weight), unused);
+            });
           });
         });
       });
