@@ -14,93 +14,33 @@ arguments raise ``RuntimeError``. There is no CPU path.
 import math
 
 import torch
-from torch.autograd import Function
-from torch.autograd.function import once_differentiable
 
 from . import spncpy
 
 MAX_EXPERTS = 1024
 MAX_CHOICES = 64
 
-_TYPES = {torch.float32: 0, torch.float64: 1, torch.float16: 2, torch.bfloat16: 3}
 _OVER = {"chosen": 0, "all": 1}
 _LOG = 2
-_ZERO, _MARGINAL, _MASK = 0, 1, 2
-_LIMIT = 2 ** 31
+_native = None
+
+
+def _ops():
+    """The native half (csrc/torch_binding.cpp). It finds libspnc_hip.so already loaded, by the way every user of it takes."""
+    global _native
+    if _native is None:
+        spncpy._load()
+        try:
+            from . import _mixture_ops
+        except ImportError as e:
+            raise RuntimeError(f"The native part of spnc.mixture is missing; build it with `make -C spn-compiler_amd/csrc` ({e})") from e
+        _native = _mixture_ops
+    return _native
 
 
 def _refuse(condition, message):
     if condition:
         raise RuntimeError(message)
-
-
-def _on_gpu(*tensors):
-    """All tensors on one GPU; returns it."""
-    device = tensors[0].device
-    for t in tensors:
-        _refuse(t.device.type != "cuda", f"Tensors must be on a GPU, got one on {t.device}")
-        _refuse(t.device != device, f"Tensors must be on one GPU, got {device} and {t.device}")
-    return device
-
-
-def _call(name, device, *arguments):
-    """Calls a function of the C-ABI on the device's current stream."""
-    function = getattr(spncpy._load(), name)
-    if torch.cuda.current_device() != device.index:
-        with torch.cuda.device(device):
-            spncpy._check(function(*arguments, torch.cuda.current_stream(device).cuda_stream))
-    else:
-        spncpy._check(function(*arguments, torch.cuda.current_stream(device).cuda_stream))
-
-
-def _rows(t):
-    """A 2-D tensor whose rows are contiguous and do not overlap; a copy where they are not."""
-    n, width = t.shape
-    if (width <= 1 or t.stride(1) == 1) and (n <= 1 or t.stride(0) >= width):
-        return t
-    return t.contiguous()
-
-
-def _stride(t):
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _wants_grad(*tensors):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
-
-
-# ---- gate -----------------------------------------------------------------------------------------------------------
-
-def _gate_forward(logits, k, flags):
-    logits = _rows(logits)
-    n, experts = logits.shape
-    index = torch.empty((n, k), dtype=torch.int32, device=logits.device)
-    weight = torch.empty((n, k), dtype=torch.float64 if logits.dtype == torch.float64 else torch.float32, device=logits.device)
-    _call("spnc_hip_gate", logits.device, logits.data_ptr(), _TYPES[logits.dtype], n, experts, _stride(logits), k, flags, index.data_ptr(),
-          weight.data_ptr())
-    return index, weight
-
-
-class _Gate(Function):
-    @staticmethod
-    def forward(ctx, logits, k, flags):
-        index, weight = _gate_forward(logits, k, flags)
-        ctx.flags, ctx.shape, ctx.dtype = flags, logits.shape, logits.dtype
-        ctx.save_for_backward(logits if flags & 1 else None, index, weight)
-        ctx.mark_non_differentiable(index)
-        return index, weight
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, _, grad):
-        logits, index, weight = ctx.saved_tensors
-        (n, experts), k = ctx.shape, index.shape[1]
-        logits = None if logits is None else _rows(logits)
-        grad = grad.contiguous()
-        out = torch.empty((n, experts), dtype=ctx.dtype, device=index.device)
-        _call("spnc_hip_gate_backward", index.device, None if logits is None else logits.data_ptr(), _TYPES[ctx.dtype], n, experts,
-              experts if logits is None else _stride(logits), k, ctx.flags, index.data_ptr(), weight.data_ptr(), grad.data_ptr(), out.data_ptr())
-        return out, None, None
 
 
 def gate(logits, k, *, over="chosen", log=False):
@@ -116,20 +56,9 @@ def gate(logits, k, *, over="chosen", log=False):
     slots that are left over hold index -1 and weight 0 (log weight minus infinity). NaN among the logits makes the
     row's weights NaN if it is chosen, or anywhere in the row with "all".
     """
-    _refuse(logits.dim() != 2, f"Logits must have shape [rows, experts], got {tuple(logits.shape)}")
-    _refuse(logits.dtype not in _TYPES, f"Logits must be float32, float64, float16 or bfloat16, got {logits.dtype}")
     _refuse(over not in _OVER, f"over must be 'chosen' or 'all', got {over!r}")
-    experts = logits.shape[1]
-    _refuse(not 1 <= experts <= MAX_EXPERTS, f"The number of experts must be between 1 and {MAX_EXPERTS}, got {experts}")
-    _refuse(not 1 <= k <= min(experts, MAX_CHOICES), f"k must be between 1 and {min(experts, MAX_CHOICES)}, got {k}")
-    _on_gpu(logits)
-    flags = _OVER[over] | (_LOG if log else 0)
-    if _wants_grad(logits):
-        return _Gate.apply(logits, k, flags)
-    return _gate_forward(logits, k, flags)
+    return (_native or _ops()).gate(logits, k, _OVER[over] | (_LOG if log else 0))
 
-
-# ---- routing --------------------------------------------------------------------------------------------------------
 
 class Plan:
     """Where every slot (row i, choice j) stands in the buffer sorted by expert.
@@ -142,12 +71,7 @@ class Plan:
     __slots__ = ("position", "starts", "counts", "capacity")
 
     def __init__(self, position, starts, counts, capacity):
-        for name, t, dim in (("position", position, 2), ("starts", starts, 1), ("counts", counts, 1)):
-            _refuse(t.dtype != torch.int32 or t.dim() != dim or not t.is_contiguous(), f"{name} must be a contiguous int32 tensor of {dim} dimensions")
-        _refuse(position.shape[1] < 1, "A row must have at least one slot")
-        _refuse(starts.shape[0] != counts.shape[0] + 1, "starts must have one entry more than counts")
-        _refuse(not 1 <= counts.shape[0] <= MAX_EXPERTS, f"The number of experts must be between 1 and {MAX_EXPERTS}, got {counts.shape[0]}")
-        _refuse(not 0 <= capacity < _LIMIT, f"The capacity must be below 2^31, got {capacity}")
+        (_native or _ops()).check_plan(position, starts, counts, capacity)
         self.position, self.starts, self.counts, self.capacity = position, starts, counts, capacity
 
     @property
@@ -169,57 +93,9 @@ def route(index, experts, *, align=1):
 
     Returns a ``Plan`` with capacity ``n * k + experts * (align - 1)``.
     """
-    _refuse(index.dim() != 2 or index.dtype != torch.int32 or index.shape[1] < 1, f"The index must be int32 [rows, choices], got {index.dtype} {tuple(index.shape)}")
-    _refuse(not 1 <= experts <= MAX_EXPERTS, f"The number of experts must be between 1 and {MAX_EXPERTS}, got {experts}")
-    _refuse(align < 1, f"align must be at least 1, got {align}")
-    slots = index.numel()
-    capacity = slots + experts * (align - 1)
-    _refuse(capacity >= _LIMIT, f"{slots} slots and {experts} segments aligned to {align} rows exceed 2^31 rows")
-    device = _on_gpu(index)
-    index = index.contiguous()
-    position = torch.empty_like(index)
-    starts = torch.empty(experts + 1, dtype=torch.int32, device=device)
-    counts = torch.empty(experts, dtype=torch.int32, device=device)
-    bytes_ = spncpy._load().spnc_hip_route_workspace(slots, experts)
-    workspace = torch.empty(bytes_, dtype=torch.uint8, device=device) if bytes_ else None
-    _call("spnc_hip_route", device, index.data_ptr(), slots, experts, align, position.data_ptr(), starts.data_ptr(), counts.data_ptr(),
-          workspace.data_ptr() if bytes_ else None, bytes_)
-    return Plan(position, starts, counts, capacity)
-
-
-def _dispatch_forward(rows, plan, out, clear):
-    rows = _rows(rows)
-    n, width = rows.shape
-    size = rows.element_size()
-    if out is None:
-        out = torch.empty((plan.capacity, width), dtype=rows.dtype, device=rows.device)
-    _call("spnc_hip_dispatch", rows.device, rows.data_ptr(), n, width * size, _stride(rows) * size, plan.position.data_ptr(), plan.position.shape[1],
-          plan.capacity, plan.starts.data_ptr(), plan.counts.data_ptr(), plan.experts, int(clear), out.data_ptr())
-    return out
-
-
-def _combine_forward(values, plan, weights):
-    values = _rows(values)
-    width = values.shape[1]
-    out = torch.empty((plan.rows, width), dtype=values.dtype, device=values.device)
-    _call("spnc_hip_combine", values.device, values.data_ptr(), _TYPES[values.dtype], plan.capacity, width, _stride(values), plan.position.data_ptr(),
-          plan.rows, plan.position.shape[1], None if weights is None else weights.data_ptr(), 0 if weights is None else _TYPES[weights.dtype],
-          out.data_ptr())
-    return out
-
-
-class _Dispatch(Function):
-    @staticmethod
-    def forward(ctx, rows, plan):
-        ctx.plan = plan
-        ctx.save_for_backward(plan.position)
-        return _dispatch_forward(rows, plan, None, True)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        ctx.saved_tensors  # raises if the plan was written to in the meantime
-        return _combine_forward(grad, ctx.plan, None), None
+    plan = Plan.__new__(Plan)
+    plan.position, plan.starts, plan.counts, plan.capacity = (_native or _ops()).route(index, experts, align)
+    return plan
 
 
 def dispatch(rows, plan, out=None):
@@ -229,51 +105,7 @@ def dispatch(rows, plan, out=None):
     out  : [capacity, width] to write into; its rows that belong to no segment are left as they were. Without it a new
            tensor is returned in which they are zero.
     """
-    _refuse(rows.dim() != 2, f"Rows must have shape [rows, width], got {tuple(rows.shape)}")
-    _refuse(rows.shape[0] != plan.rows, f"The plan is for {plan.rows} rows, got {rows.shape[0]}")
-    _refuse(rows.element_size() not in (1, 2, 4, 8) or rows.dtype.is_complex, f"Rows of {rows.dtype} are not supported")
-    if out is not None:
-        _refuse(tuple(out.shape) != (plan.capacity, rows.shape[1]) or out.dtype != rows.dtype or not out.is_contiguous(),
-                f"out must be a contiguous {rows.dtype} tensor of shape {(plan.capacity, rows.shape[1])}")
-        _refuse(_wants_grad(rows, out), "dispatch with out= has no gradient; call it without")
-        _on_gpu(rows, plan.position, plan.starts, plan.counts, out)
-        return _dispatch_forward(rows, plan, out, False)
-    _on_gpu(rows, plan.position, plan.starts, plan.counts)
-    if _wants_grad(rows):
-        _refuse(rows.dtype not in _TYPES, f"Rows of {rows.dtype} have no gradient")
-        return _Dispatch.apply(rows, plan)
-    return _dispatch_forward(rows, plan, None, True)
-
-
-# ---- combination ----------------------------------------------------------------------------------------------------
-
-class _Combine(Function):
-    @staticmethod
-    def forward(ctx, values, weights, plan):
-        ctx.plan = plan
-        ctx.save_for_backward(values, weights, plan.position)
-        return _combine_forward(values, plan, weights)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        values, weights, position = ctx.saved_tensors
-        plan, values, grad = ctx.plan, _rows(values), _rows(grad)
-        width = values.shape[1]
-        if weights is None:
-            return _dispatch_forward(grad, plan, None, True), None, None
-        grad_values = torch.empty((plan.capacity, width), dtype=values.dtype, device=values.device) if ctx.needs_input_grad[0] else None
-        grad_weights = torch.empty_like(weights) if ctx.needs_input_grad[1] else None
-        _call("spnc_hip_combine_backward", values.device, values.data_ptr(), _TYPES[values.dtype], plan.capacity, width, _stride(values),
-              position.data_ptr(), plan.rows, position.shape[1], weights.data_ptr(), _TYPES[weights.dtype], grad.data_ptr(), _stride(grad),
-              plan.starts.data_ptr(), plan.counts.data_ptr(), plan.experts, None if grad_values is None else grad_values.data_ptr(),
-              None if grad_weights is None else grad_weights.data_ptr())
-        return grad_values, grad_weights, None
-
-
-def _check_weights(weights, plan, allowed):
-    _refuse(tuple(weights.shape) != tuple(plan.position.shape), f"Weights must have shape {tuple(plan.position.shape)}, got {tuple(weights.shape)}")
-    _refuse(weights.dtype not in allowed, f"Weights must be {' or '.join(str(t) for t in allowed)}, got {weights.dtype}")
+    return (_native or _ops()).dispatch(rows, plan.position, plan.starts, plan.counts, plan.capacity, out)
 
 
 def combine(values, plan, weights=None):
@@ -284,44 +116,7 @@ def combine(values, plan, weights=None):
 
     Slots that are not routed are left out; a row without slots becomes zero.
     """
-    _refuse(values.dim() != 2 or values.shape[0] != plan.capacity, f"Values must have shape [{plan.capacity}, width], got {tuple(values.shape)}")
-    _refuse(values.dtype not in _TYPES, f"Values must be float32, float64, float16 or bfloat16, got {values.dtype}")
-    if weights is None:
-        _on_gpu(values, plan.position, plan.starts, plan.counts)
-    else:
-        _check_weights(weights, plan, (torch.float32, torch.float64) if values.dtype == torch.float64 else (torch.float32,))
-        _on_gpu(values, plan.position, plan.starts, plan.counts, weights)
-        weights = weights.contiguous()
-    if _wants_grad(values, weights):
-        return _Combine.apply(values, weights, plan)
-    return _combine_forward(values, plan, weights)
-
-
-def _combine_log_forward(values, plan, weights):
-    out = torch.empty(plan.rows, dtype=values.dtype, device=values.device)
-    _call("spnc_hip_combine_log", values.device, values.data_ptr(), _TYPES[values.dtype], plan.capacity, plan.position.data_ptr(), plan.rows,
-          plan.position.shape[1], weights.data_ptr(), _TYPES[weights.dtype], out.data_ptr())
-    return out
-
-
-class _CombineLog(Function):
-    @staticmethod
-    def forward(ctx, values, weights, plan):
-        ctx.plan = plan
-        ctx.save_for_backward(values, weights, plan.position)
-        return _combine_log_forward(values, plan, weights)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        values, weights, position = ctx.saved_tensors
-        plan, grad = ctx.plan, grad.contiguous()
-        grad_values = torch.empty_like(values) if ctx.needs_input_grad[0] else None
-        grad_weights = torch.empty_like(weights) if ctx.needs_input_grad[1] else None
-        _call("spnc_hip_combine_log_backward", values.device, values.data_ptr(), _TYPES[values.dtype], plan.capacity, position.data_ptr(), plan.rows,
-              position.shape[1], weights.data_ptr(), _TYPES[weights.dtype], grad.data_ptr(), plan.starts.data_ptr(), plan.counts.data_ptr(),
-              plan.experts, None if grad_values is None else grad_values.data_ptr(), None if grad_weights is None else grad_weights.data_ptr())
-        return grad_values, grad_weights, None
+    return (_native or _ops()).combine(values, plan.position, plan.starts, plan.counts, plan.capacity, weights)
 
 
 def combine_log(values, plan, log_weights):
@@ -334,44 +129,7 @@ def combine_log(values, plan, log_weights):
     A slot that is not routed, or whose log weight is minus infinity, is left out whatever its value is; a row without
     slots, or all of whose values are minus infinity, becomes minus infinity and has no gradient.
     """
-    _refuse(values.dim() != 1 or values.shape[0] != plan.capacity, f"Values must have shape [{plan.capacity}], got {tuple(values.shape)}")
-    _refuse(values.dtype not in (torch.float32, torch.float64), f"Values must be float32 or float64, got {values.dtype}")
-    _check_weights(log_weights, plan, (torch.float32, torch.float64))
-    _on_gpu(values, plan.position, plan.starts, plan.counts, log_weights)
-    values, log_weights = values.contiguous(), log_weights.contiguous()
-    if _wants_grad(values, log_weights):
-        return _CombineLog.apply(values, log_weights, plan)
-    return _combine_log_forward(values, plan, log_weights)
-
-
-# ---- dropout --------------------------------------------------------------------------------------------------------
-
-def _dropout_forward(x, p, mode, seed, offset):
-    shape = x.shape
-    if x.dim() != 2:
-        x = x.reshape(1, -1) if x.dim() < 2 else x.reshape(-1, shape[-1])
-    x = _rows(x)
-    out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    on_device = isinstance(offset, torch.Tensor)
-    _call("spnc_hip_dropout", x.device, x.data_ptr(), _TYPES[x.dtype], x.shape[0], x.shape[1], _stride(x), out.data_ptr(), x.shape[1], p, mode, seed,
-          0 if on_device else offset, offset.data_ptr() if on_device else None)
-    return out.view(shape)
-
-
-class _Dropout(Function):
-    @staticmethod
-    def forward(ctx, x, p, mode, seed, offset):
-        ctx.arguments = p, mode, seed
-        on_device = isinstance(offset, torch.Tensor)
-        ctx.save_for_backward(offset if on_device else None)  # the mask must be the same: a change in between is an error
-        ctx.offset = None if on_device else offset
-        return _dropout_forward(x, p, mode, seed, offset)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, grad):
-        (offset,), (p, mode, seed) = ctx.saved_tensors, ctx.arguments
-        return _dropout_forward(grad, p, _MASK if mode == _MARGINAL else mode, seed, ctx.offset if offset is None else offset), None, None, None, None
+    return (_native or _ops()).combine_log(values, plan.position, plan.starts, plan.counts, plan.capacity, log_weights)
 
 
 def dropout(x, p, seed, *, offset=0, marginal=False):
@@ -387,22 +145,13 @@ def dropout(x, p, seed, *, offset=0, marginal=False):
     Element e of x, counted in its logical order whatever the strides and the type are, is dropped where word e % 4 of
     Philox4x32-10 with the seed as key and (e // 4, offset) as counter is below round(p * 2^32).
     """
-    _refuse(x.dtype not in _TYPES, f"x must be float32, float64, float16 or bfloat16, got {x.dtype}")
     _refuse(not 0.0 <= p <= 1.0, f"p must be between 0 and 1, got {p}")
     _refuse(not 0 <= seed < 2 ** 64, f"The seed must be between 0 and 2^64 - 1, got {seed}")
     if isinstance(offset, torch.Tensor):
-        _refuse(offset.dtype != torch.int64 or offset.numel() != 1, "An offset on the device must be a one-element int64 tensor")
-        _on_gpu(x, offset)
-    else:
-        _refuse(not 0 <= offset < 2 ** 64, f"The offset must be between 0 and 2^64 - 1, got {offset}")
-        _on_gpu(x)
-    mode = _MARGINAL if marginal else _ZERO
-    if _wants_grad(x):
-        return _Dropout.apply(x, p, mode, seed, offset)
-    return _dropout_forward(x, p, mode, seed, offset)
+        return (_native or _ops()).dropout(x, p, seed, 0, offset, marginal)
+    _refuse(not 0 <= offset < 2 ** 64, f"The offset must be between 0 and 2^64 - 1, got {offset}")
+    return (_native or _ops()).dropout(x, p, seed, offset, None, marginal)
 
-
-# ---- mixtures of kernels --------------------------------------------------------------------------------------------
 
 class Mixture:
     """A gated mixture whose experts are compiled kernels (``HIPCompiler.compile_ll``) over the same features."""
@@ -430,7 +179,9 @@ class Mixture:
                 f"Sorted rows must be contiguous with shape {(plan.capacity, self.num_features)}, got {tuple(rows.shape)}")
         _refuse(plan.experts != len(self.kernels), f"The plan is for {plan.experts} experts, the mixture has {len(self.kernels)}")
         self._check_type(rows)
-        device = _on_gpu(rows, plan.position, plan.starts, plan.counts)
+        device = rows.device
+        _refuse(device.type != "cuda" or any(t.device != device for t in (plan.position, plan.starts, plan.counts)),
+                f"Rows and plan must be on one GPU, got {device} and {plan.position.device}")
         _refuse(torch.cuda.is_current_stream_capturing(), "A mixture cannot run under graph capture: the host needs the segments' sizes")
         values = torch.empty(plan.capacity, dtype=self._result, device=device)
         row_bytes, result_bytes = self.num_features * self._feature_bytes, values.element_size()
@@ -460,9 +211,9 @@ class Mixture:
         _refuse(logits.dim() != 2 or tuple(logits.shape) != (rows.shape[0], len(self.kernels)),
                 f"Logits must have shape [{rows.shape[0]}, {len(self.kernels)}], got {tuple(logits.shape)}")
         self._check_type(rows)
-        _refuse(_wants_grad(rows), "Compiled kernels have no gradient with respect to their features")
-        device = _on_gpu(rows, logits)
+        _refuse(torch.is_grad_enabled() and rows.requires_grad, "Compiled kernels have no gradient with respect to their features")
+        _refuse(rows.device.type != "cuda" or logits.device != rows.device, f"Rows and logits must be on one GPU, got {rows.device} and {logits.device}")
         index, log_weights = gate(logits, k, over=over, log=True)
         plan = route(index, len(self.kernels), align=self._align)
-        sorted_rows = torch.empty((plan.capacity, self.num_features), dtype=rows.dtype, device=device)
+        sorted_rows = torch.empty((plan.capacity, self.num_features), dtype=rows.dtype, device=rows.device)
         return combine_log(self.execute(dispatch(rows, plan, out=sorted_rows), plan), plan, log_weights)

@@ -494,6 +494,25 @@ def test_gradients_against_differences(native):
             assert abs(float((up - down) / (2 * h)) - float(grad.flatten()[i])) <= 1e-8
 
 
+@pytest.mark.gpu
+def test_second_gradients_and_changed_plans_are_errors(native):
+    torch = _torch()
+    from spnc import mixture as m
+    plan = m.route(torch.zeros(4, 1, dtype=torch.int32, device="cuda"), 1)
+    x, w, v = torch.randn(4, 3, device="cuda", requires_grad=True), torch.rand(4, 1, device="cuda", requires_grad=True), torch.randn(4, device="cuda", requires_grad=True)
+    for f, leaf in ((lambda: m.gate(x, 2, log=True)[1], x), (lambda: m.gate(x, 2, over="all")[1], x), (lambda: m.dispatch(x, plan), x), (lambda: m.combine(x, plan), x),
+                    (lambda: m.combine(x, plan, w), w), (lambda: m.combine_log(v, plan, w), v), (lambda: m.dropout(x, 0.1, 3), x)):
+        first, = torch.autograd.grad((f() ** 2).sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="cannot be differentiated again"):
+            first.sum().backward()
+    for f in (lambda: m.dispatch(x, plan), lambda: m.combine(x, plan, w), lambda: m.combine_log(v, plan, w)):
+        y = f()
+        plan.position.zero_()
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+        plan = m.route(torch.zeros(4, 1, dtype=torch.int32, device="cuda"), 1)
+
+
 # ---- dropout --------------------------------------------------------------------------------------------------------
 
 @pytest.mark.gpu
