@@ -42,6 +42,24 @@ def gate_gradient(z, index, grad, over="chosen", log=False):
     return dz
 
 
+def gate_many(z, k, over, log, grad):
+    """index, weight and the logits' gradient of many rows without NaN at once."""
+    order = np.argsort(-z, axis=1, kind="stable")[:, :k]
+    chosen = np.take_along_axis(z, order, axis=1)
+    is_open = chosen > -np.inf
+    with np.errstate(all="ignore"):
+        total = np.logaddexp.reduce(chosen if over == "chosen" else z, axis=1, keepdims=True)
+        log_weight = np.where(is_open, chosen - total, -np.inf)
+        p = np.where(z > -np.inf, np.exp(z - total), 0.0)
+    weight = np.exp(log_weight)
+    dlog = np.where(is_open, grad, 0.0) * (1.0 if log else weight)
+    dz = -p * dlog.sum(axis=1, keepdims=True) if over == "all" else np.zeros_like(z)
+    if over == "chosen":
+        dlog = dlog - weight * dlog.sum(axis=1, keepdims=True)
+    np.add.at(dz, (np.arange(z.shape[0])[:, None], order), np.where(is_open, dlog, 0.0))
+    return np.where(is_open, order, -1), log_weight if log else weight, dz
+
+
 def route(index, experts, align=1):
     """position, starts, counts by going through the slots in order."""
     flat = np.asarray(index).reshape(-1)

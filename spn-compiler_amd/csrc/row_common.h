@@ -1,0 +1,218 @@
+// What the kernels on device-resident rows share (row_gate.hip, row_route.hip, row_dropout.hip): launch shapes, packed accesses,
+// operations over groups of lanes, and argument checks of their entry points (include/spnc_hip_rows.h).
+#pragma once
+#include <hip/hip_runtime.h>
+
+#include <cmath>
+#include <cstdint>
+#include <initializer_list>
+#include <stdexcept>
+#include <string>
+#include <type_traits>
+
+#include "../../include/spnc_hip_rows.h"
+#include "guard.h"
+
+namespace spnc_hip {
+namespace {
+
+constexpr unsigned WAVE = 64;
+constexpr unsigned BLOCK = 256;
+constexpr unsigned XCDS = 8;             // blocks go to the chip's dies in turn
+constexpr size_t MAX_GRID = 1u << 22;    // a launch must stay below 2^32 threads
+
+template <typename T> struct Wide { using type = float; };
+template <> struct Wide<double> { using type = double; };
+template <typename T> using wide_t = typename Wide<T>::type;
+
+template <typename T, int N>
+struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack {
+  T v[N];
+};
+
+// Accesses that are not kept in the caches. A piece of another size than 16 bytes goes the ordinary way.
+typedef uint32_t Words4 __attribute__((ext_vector_type(4)));
+
+template <typename P>
+__device__ inline P streamLoad(const P* p) {
+  if constexpr (sizeof(P) == 16) return __builtin_bit_cast(P, __builtin_nontemporal_load(reinterpret_cast<const Words4*>(p)));
+  else return *p;
+}
+
+template <typename P>
+__device__ inline void streamStore(P* p, const P& v) {
+  if constexpr (sizeof(P) == 16) __builtin_nontemporal_store(__builtin_bit_cast(Words4, v), reinterpret_cast<Words4*>(p));
+  else *p = v;
+}
+
+// Neighbouring tiles of rows go to one die: rows that are neighbours in the sorted buffer come from neighbouring rows,
+// and a cache line of narrow rows is then filled or read within one L2.
+template <typename Body>
+__device__ inline void forTiles(size_t tiles, unsigned grid, Body&& body) {
+  const size_t perDie = (tiles + XCDS - 1) / XCDS, first = size_t(blockIdx.x % XCDS) * perDie;
+  for (size_t t = blockIdx.x / XCDS; t < perDie; t += grid / XCDS)
+    if (first + t < tiles) body(first + t);
+}
+
+inline unsigned tileGrid(size_t tiles) {
+  const size_t g = (tiles + XCDS - 1) / XCDS * XCDS;
+  return unsigned(g < MAX_GRID ? g : MAX_GRID);
+}
+
+// A group of 2^shift lanes handles a row, a piece of up to 16 bytes a lane at a time.
+//
+// Rows that are written to scattered places bypass the caches where they consist of whole 64-byte halves of cache lines: 1 M rows
+// of 64 bytes to two places each take 36 us instead of 50, of 2 KB to four places 52 instead of 67 (a consumer that reads
+// them next loses up to half of that where they would have fit the last-level cache). Rows that share their halves must not: 48
+// bytes take 87 us instead of 61, since each piece goes to memory by itself.
+struct RowShape {
+  unsigned pieces;  // of a row
+  unsigned shift;
+  size_t tiles;
+  bool stream;      // scattered rows are written past the caches
+};
+
+inline RowShape rowShape(size_t n, size_t rowBytes, unsigned pieceBytes, const void* scattered = nullptr) {
+  RowShape s;
+  s.pieces = unsigned(rowBytes / pieceBytes);
+  s.shift = 0;
+  while (s.shift < 6 && (1u << s.shift) < s.pieces) ++s.shift;
+  const size_t rows = BLOCK >> s.shift;
+  s.tiles = (n + rows - 1) / rows;
+  s.stream = pieceBytes == 16 && rowBytes % 64 == 0 && reinterpret_cast<uintptr_t>(scattered) % 64 == 0;
+  return s;
+}
+
+// ---- lanes ----------------------------------------------------------------------------------------------------------
+
+// For a lane, its word and that of the lane it is paired with at distance D, in an order that is the same for both lanes or
+// does not matter to a symmetric operation. D = 4 and 8 mirror instead of exchanging: all lanes at smaller distances must hold the
+// same already. Vector instructions throughout (DPP, and row swaps of gfx950 for 16 and 32), no LDS.
+template <int D>
+__device__ inline void lanePair(uint32_t x, uint32_t& a, uint32_t& b) {
+  if constexpr (D <= 8) {
+    constexpr int control = D == 1 ? 0xB1 : D == 2 ? 0x4E : D == 4 ? 0x141 : 0x140;  // quad_perm, half row and row mirror
+    a = x;
+    b = uint32_t(__builtin_amdgcn_update_dpp(0, int(x), control, 0xF, 0xF, true));
+  } else if constexpr (D == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    a = r[0], b = r[1];
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    a = r[0], b = r[1];
+  }
+}
+
+template <int D, int G, typename R, typename Op>
+__device__ inline R groupFrom(R x, Op op) {
+  if constexpr (D >= G) {
+    return x;
+  } else {
+    R a, b;
+    if constexpr (sizeof(R) == 4) {
+      uint32_t wa, wb;
+      lanePair<D>(__builtin_bit_cast(uint32_t, x), wa, wb);
+      a = __builtin_bit_cast(R, wa), b = __builtin_bit_cast(R, wb);
+    } else {
+      const uint64_t w = __builtin_bit_cast(uint64_t, x);
+      uint32_t la, lb, ha, hb;
+      lanePair<D>(uint32_t(w), la, lb);
+      lanePair<D>(uint32_t(w >> 32), ha, hb);
+      a = __builtin_bit_cast(R, uint64_t(ha) << 32 | la), b = __builtin_bit_cast(R, uint64_t(hb) << 32 | lb);
+    }
+    return groupFrom<D * 2, G>(op(a, b), op);
+  }
+}
+
+// The same over a whole wave for operations on words with 0 as neutral element, in fewer instructions: lane 15 of a row to the
+// next row, lane 31 to the upper half, and lane 63, which then has everything, to all lanes as a scalar.
+template <typename R, typename Op>
+__device__ inline R waveFrom(R x, Op op) {
+  x = groupFrom<1, 16>(x, op);
+  x = op(x, __builtin_bit_cast(R, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x142, 0xF, 0xF, true)));  // row_bcast:15
+  x = op(x, __builtin_bit_cast(R, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x143, 0xF, 0xF, true)));  // row_bcast:31
+  return __builtin_bit_cast(R, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), 63));
+}
+
+// The sum, maximum or minimum over a group of G lanes, in all of them.
+template <int G, typename R> __device__ inline R groupSum(R x) {
+  auto op = [](R a, R b) { return a + b; };
+  if constexpr (G == WAVE && sizeof(R) == 4) return waveFrom(x, op);
+  else return groupFrom<1, G>(x, op);
+}
+template <int G, typename R> __device__ inline R groupMax(R x) {
+  auto op = [](R a, R b) { return a > b ? a : b; };
+  if constexpr (G == WAVE && std::is_same<R, uint32_t>::value) return waveFrom(x, op);
+  else return groupFrom<1, G>(x, op);
+}
+template <int G, typename R> __device__ inline R groupMin(R x) {
+  return groupFrom<1, G>(x, [](R a, R b) { return a < b ? a : b; });
+}
+
+// exp(x): x log2(e) in two parts, the hardware's exp2 of the first, the second as a factor 1 + r ln 2. Within two units in the
+// last place; below exp(-87) the result is 0.
+__device__ inline float expOf(float x) {
+  x = x < -200.0f ? -200.0f : x;  // minus infinity has no second part
+  const float t = x * 1.44269502f, r = __builtin_fmaf(x, 1.92596299e-8f, __builtin_fmaf(x, 1.44269502f, -t));
+  const float y = __builtin_amdgcn_exp2f(t);
+  return __builtin_fmaf(y, r * 0.693147182f, y);
+}
+__device__ inline double expOf(double x) { return exp(x); }
+// Without the second part: x log2(e) is rounded, an error of |x| 2^-24 relative to the result, which is that of a difference x
+// already. For terms of a sum, where it is weighted with exp(x), and for results of 16 bits.
+__device__ inline float expTerm(float x) { return __builtin_amdgcn_exp2f(x * 1.44269502f); }
+__device__ inline double expTerm(double x) { return exp(x); }
+__device__ inline float logOf(float x) { return logf(x); }
+__device__ inline double logOf(double x) { return log(x); }
+
+// ---- host side ------------------------------------------------------------------------------------------------------
+
+[[noreturn]] inline void refuse(const std::string& what) { throw std::runtime_error(what); }
+
+inline void launched(const char* what) {
+  const hipError_t e = hipGetLastError();
+  if (e != hipSuccess) refuse(std::string(what) + " launch: " + hipGetErrorString(e));
+}
+
+inline size_t elementBytes(int dtype) {
+  switch (dtype) {
+    case SPNC_HIP_FLOAT32: return 4;
+    case SPNC_HIP_FLOAT64: return 8;
+    case SPNC_HIP_FLOAT16:
+    case SPNC_HIP_BFLOAT16: return 2;
+  }
+  refuse("unknown element type " + std::to_string(dtype));
+}
+
+// calls fn(T()) for the element type
+template <typename Fn>
+void withType(int dtype, Fn&& fn) {
+  switch (dtype) {
+    case SPNC_HIP_FLOAT32: return fn(float());
+    case SPNC_HIP_FLOAT64: return fn(double());
+    case SPNC_HIP_FLOAT16: return fn(_Float16());
+    case SPNC_HIP_BFLOAT16: return fn(__bf16());
+  }
+  refuse("unknown element type " + std::to_string(dtype));
+}
+
+// the widest piece, in bytes, that a row of rowBytes at these addresses and strides consists of; `least` at the least
+inline unsigned pieceBytes(unsigned least, std::initializer_list<uintptr_t> addresses) {
+  uintptr_t bits = 16;
+  for (uintptr_t a : addresses) bits |= a;
+  const unsigned widest = unsigned(bits & (~bits + 1));
+  return widest < least ? 0 : widest;
+}
+
+inline uintptr_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
+
+inline void checkAligned(unsigned piece, const char* what) {
+  if (piece == 0) refuse(std::string(what) + ": pointers are not aligned to the element type");
+}
+
+inline void checkExperts(unsigned experts) {
+  if (experts == 0 || experts > SPNC_HIP_MAX_EXPERTS) refuse("experts must be between 1 and " + std::to_string(SPNC_HIP_MAX_EXPERTS));
+}
+
+}  // namespace
+}  // namespace spnc_hip

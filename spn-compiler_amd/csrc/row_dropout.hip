@@ -1,0 +1,141 @@
+// Dropout whose mask is a function of the element's number: it is computed where it is needed and never stored.
+#include "philox.h"
+#include "row_common.h"
+
+namespace spnc_hip {
+namespace {
+
+template <typename R>
+struct Dropout {
+  uint64_t threshold;
+  R scale, fill;
+  uint64_t seed, offset;
+  const uint64_t* offsetDevice;
+
+  __device__ Philox4 words(size_t block, uint64_t at) const {
+    return philox4x32(uint32_t(block), uint32_t(block >> 32), uint32_t(at), uint32_t(at >> 32), uint32_t(seed), uint32_t(seed >> 32));
+  }
+  template <typename T>
+  __device__ T apply(uint32_t word, T x) const {
+    return T(word >= threshold ? R(x) * scale : fill);
+  }
+};
+
+template <typename T> constexpr int DROPOUT_UNIT = sizeof(T) == 2 ? 8 : 4;  // elements of 16 bytes, at least the four of one counter
+constexpr unsigned DROPOUT_UNITS = 2;                                       // of a thread
+
+// Contiguous elements; VEC: read and written 16 bytes at a time.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(BLOCK) void dropoutFlatKernel(const T* x, size_t elements, T* out, Dropout<wide_t<T>> d) {
+  constexpr int E = DROPOUT_UNIT<T>;
+  using P = Pack<T, E>;
+  const uint64_t at = d.offsetDevice ? *d.offsetDevice : d.offset;
+  const size_t units = (elements + E - 1) / E, tiles = (units + DROPOUT_UNITS * BLOCK - 1) / (DROPOUT_UNITS * BLOCK);
+  for (size_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
+    const size_t first = tile * (DROPOUT_UNITS * BLOCK) + threadIdx.x;
+    P v[DROPOUT_UNITS];
+#pragma unroll
+    for (unsigned i = 0; i < DROPOUT_UNITS; ++i) {
+      const size_t e = (first + i * BLOCK) * E;
+      if (VEC && e + E <= elements) v[i] = *reinterpret_cast<const P*>(x + e);
+      else
+#pragma unroll
+        for (int q = 0; q < E; ++q)
+          if (e + q < elements) v[i].v[q] = x[e + q];
+    }
+#pragma unroll
+    for (unsigned i = 0; i < DROPOUT_UNITS; ++i) {
+      const size_t e = (first + i * BLOCK) * E;
+      if (e >= elements) continue;
+#pragma unroll
+      for (int b = 0; b < E / 4; ++b) {
+        const Philox4 r = d.words(e / 4 + b, at);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v[i].v[4 * b + q] = d.apply(r.w[q], v[i].v[4 * b + q]);
+      }
+      if (VEC && e + E <= elements) *reinterpret_cast<P*>(out + e) = v[i];
+      else
+#pragma unroll
+        for (int q = 0; q < E; ++q)
+          if (e + q < elements) out[e + q] = v[i].v[q];
+    }
+  }
+}
+
+// Rows that are not adjacent; VEC: widths, strides and addresses in multiples of four elements, so that a counter's four
+// elements are neighbours. Otherwise a counter whose elements lie in two rows is computed for both.
+template <typename T, bool VEC>
+__global__ __launch_bounds__(BLOCK) void dropoutRowsKernel(const T* x, size_t n, size_t width, size_t stride, T* out, size_t outStride, RowShape shape,
+                                                           Dropout<wide_t<T>> d) {
+  const uint64_t at = d.offsetDevice ? *d.offsetDevice : d.offset;
+  const unsigned lane = threadIdx.x & ((1u << shape.shift) - 1);
+  forTiles(shape.tiles, gridDim.x, [&](size_t tile) {
+    const size_t row = tile * (BLOCK >> shape.shift) + (threadIdx.x >> shape.shift);
+    if (row >= n) return;
+    const size_t begin = row * width, end = begin + width;
+    const T* from = x + row * stride;
+    T* to = out + row * outStride;
+    for (size_t b = begin / 4 + lane; 4 * b < end; b += size_t(1) << shape.shift) {
+      const Philox4 r = d.words(b, at);
+      if constexpr (VEC) {
+        Pack<T, 4> v = *reinterpret_cast<const Pack<T, 4>*>(from + (4 * b - begin));
+#pragma unroll
+        for (int q = 0; q < 4; ++q) v.v[q] = d.apply(r.w[q], v.v[q]);
+        *reinterpret_cast<Pack<T, 4>*>(to + (4 * b - begin)) = v;
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const size_t e = 4 * b + q;
+          if (e >= begin && e < end) to[e - begin] = d.apply(r.w[q], from[e - begin]);
+        }
+      }
+    }
+  });
+}
+
+}  // namespace
+}  // namespace spnc_hip
+
+using namespace spnc_hip;
+
+extern "C" {
+
+int spnc_hip_dropout(const void* x, int dtype, size_t n, size_t width, size_t stride, void* out, size_t out_stride, double p, int mode,
+                     uint64_t seed, uint64_t offset, const uint64_t* offset_device, void* stream) {
+  return guarded([&] {
+    elementBytes(dtype);
+    if (!(p >= 0.0 && p <= 1.0)) refuse("the probability of dropping an element must be between 0 and 1");
+    if (mode < SPNC_HIP_DROPOUT_ZERO || mode > SPNC_HIP_DROPOUT_MASK) refuse("unknown dropout mode " + std::to_string(mode));
+    if (n > 1 && (stride < width || out_stride < width)) refuse("rows overlap");
+    if (n == 0 || width == 0) return;
+    if (!x || !out) refuse("null argument");
+    const uint64_t threshold = uint64_t(std::llrint(p * 4294967296.0));
+    const double scale = mode != SPNC_HIP_DROPOUT_ZERO ? 1.0 : threshold >> 32 ? 0.0 : 1.0 / (1.0 - p);
+    const double fill = mode == SPNC_HIP_DROPOUT_MARGINAL ? NAN : 0.0;
+    const hipStream_t s = static_cast<hipStream_t>(stream);
+    withType(dtype, [&](auto t) {
+      using T = decltype(t);
+      using R = wide_t<T>;
+      const Dropout<R> d{threshold, R(scale), R(fill), seed, offset, offset_device};
+      const uintptr_t bits = address(x) | address(out);
+      if (n == 1 || (stride == width && out_stride == width)) {
+        constexpr int E = DROPOUT_UNIT<T>;
+        const size_t elements = n * width, units = (elements + E - 1) / E, blocks = (units + DROPOUT_UNITS * BLOCK - 1) / (DROPOUT_UNITS * BLOCK);
+        const unsigned grid = unsigned(blocks < MAX_GRID ? blocks : MAX_GRID);
+        if (bits % (sizeof(Pack<T, E>) < 16 ? sizeof(Pack<T, E>) : 16) == 0)
+          dropoutFlatKernel<T, true><<<grid, BLOCK, 0, s>>>(static_cast<const T*>(x), elements, static_cast<T*>(out), d);
+        else
+          dropoutFlatKernel<T, false><<<grid, BLOCK, 0, s>>>(static_cast<const T*>(x), elements, static_cast<T*>(out), d);
+      } else {
+        const RowShape shape = rowShape(n, (width + 3) / 4, 1);
+        if (((width | stride | out_stride) % 4 | bits % (4 * sizeof(T) < 16 ? 4 * sizeof(T) : 16)) == 0)
+          dropoutRowsKernel<T, true><<<tileGrid(shape.tiles), BLOCK, 0, s>>>(static_cast<const T*>(x), n, width, stride, static_cast<T*>(out), out_stride, shape, d);
+        else
+          dropoutRowsKernel<T, false><<<tileGrid(shape.tiles), BLOCK, 0, s>>>(static_cast<const T*>(x), n, width, stride, static_cast<T*>(out), out_stride, shape, d);
+      }
+    });
+    launched("dropout");
+  });
+}
+
+}  // extern "C"

@@ -1,356 +1,9 @@
-// Operators on device-resident rows around compiled kernels (include/spnc_hip_rows.h): gate, routing, combination,
-// dropout. Device code, launch shapes and the extern "C" entry points.
-#include <hip/hip_runtime.h>
-
-#include <cmath>
-#include <cstdint>
-#include <stdexcept>
-#include <string>
-#include <type_traits>
-
-#include "../../include/spnc_hip_rows.h"
-#include "guard.h"
-#include "philox.h"
+// Rows sorted by expert and back: the sort, the copy into its order, the weighted sum and the log-sum-exp back in row order,
+// and their gradients.
+#include "row_common.h"
 
 namespace spnc_hip {
 namespace {
-
-constexpr unsigned WAVE = 64;
-constexpr unsigned BLOCK = 256;
-constexpr unsigned XCDS = 8;             // blocks go to the chip's dies in turn
-constexpr size_t MAX_GRID = 1u << 22;    // a launch must stay below 2^32 threads
-
-template <typename T> struct Wide { using type = float; };
-template <> struct Wide<double> { using type = double; };
-template <typename T> using wide_t = typename Wide<T>::type;
-
-template <typename T, int N>
-struct alignas(sizeof(T) * N < 16 ? sizeof(T) * N : 16) Pack {
-  T v[N];
-};
-
-// Accesses that are not kept in the caches. A piece of another size than 16 bytes goes the ordinary way.
-typedef uint32_t Words4 __attribute__((ext_vector_type(4)));
-
-template <typename P>
-__device__ inline P streamLoad(const P* p) {
-  if constexpr (sizeof(P) == 16) return __builtin_bit_cast(P, __builtin_nontemporal_load(reinterpret_cast<const Words4*>(p)));
-  else return *p;
-}
-
-template <typename P>
-__device__ inline void streamStore(P* p, const P& v) {
-  if constexpr (sizeof(P) == 16) __builtin_nontemporal_store(__builtin_bit_cast(Words4, v), reinterpret_cast<Words4*>(p));
-  else *p = v;
-}
-
-// Neighbouring tiles of rows go to one die: rows that are neighbours in the sorted buffer come from neighbouring rows,
-// and a cache line of narrow rows is then filled or read within one L2.
-template <typename Body>
-__device__ inline void forTiles(size_t tiles, unsigned grid, Body&& body) {
-  const size_t perDie = (tiles + XCDS - 1) / XCDS, first = size_t(blockIdx.x % XCDS) * perDie;
-  for (size_t t = blockIdx.x / XCDS; t < perDie; t += grid / XCDS)
-    if (first + t < tiles) body(first + t);
-}
-
-unsigned tileGrid(size_t tiles) {
-  const size_t g = (tiles + XCDS - 1) / XCDS * XCDS;
-  return unsigned(g < MAX_GRID ? g : MAX_GRID);
-}
-
-// ---- lanes ----------------------------------------------------------------------------------------------------------
-
-// For a lane, its word and that of the lane it is paired with at distance D, in an order that is the same for both lanes or
-// does not matter to a symmetric operation. D = 4 and 8 mirror instead of exchanging: all lanes at smaller distances must hold the
-// same already. Vector instructions throughout (DPP, and row swaps of gfx950 for 16 and 32), no LDS.
-template <int D>
-__device__ inline void lanePair(uint32_t x, uint32_t& a, uint32_t& b) {
-  if constexpr (D <= 8) {
-    constexpr int control = D == 1 ? 0xB1 : D == 2 ? 0x4E : D == 4 ? 0x141 : 0x140;  // quad_perm, half row and row mirror
-    a = x;
-    b = uint32_t(__builtin_amdgcn_update_dpp(0, int(x), control, 0xF, 0xF, true));
-  } else if constexpr (D == 16) {
-    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
-    a = r[0], b = r[1];
-  } else {
-    const auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
-    a = r[0], b = r[1];
-  }
-}
-
-template <int D, int G, typename R, typename Op>
-__device__ inline R groupFrom(R x, Op op) {
-  if constexpr (D >= G) {
-    return x;
-  } else {
-    R a, b;
-    if constexpr (sizeof(R) == 4) {
-      uint32_t wa, wb;
-      lanePair<D>(__builtin_bit_cast(uint32_t, x), wa, wb);
-      a = __builtin_bit_cast(R, wa), b = __builtin_bit_cast(R, wb);
-    } else {
-      const uint64_t w = __builtin_bit_cast(uint64_t, x);
-      uint32_t la, lb, ha, hb;
-      lanePair<D>(uint32_t(w), la, lb);
-      lanePair<D>(uint32_t(w >> 32), ha, hb);
-      a = __builtin_bit_cast(R, uint64_t(ha) << 32 | la), b = __builtin_bit_cast(R, uint64_t(hb) << 32 | lb);
-    }
-    return groupFrom<D * 2, G>(op(a, b), op);
-  }
-}
-
-// The sum, maximum or minimum over a group of G lanes, in all of them.
-template <int G, typename R> __device__ inline R groupSum(R x) {
-  return groupFrom<1, G>(x, [](R a, R b) { return a + b; });
-}
-template <int G, typename R> __device__ inline R groupMax(R x) {
-  return groupFrom<1, G>(x, [](R a, R b) { return a > b ? a : b; });
-}
-template <int G, typename R> __device__ inline R groupMin(R x) {
-  return groupFrom<1, G>(x, [](R a, R b) { return a < b ? a : b; });
-}
-
-// exp(x): x log2(e) in two parts, the hardware's exp2 of the first, the second as a factor 1 + r ln 2. Within two units in the
-// last place; below exp(-87) the result is 0.
-__device__ inline float expOf(float x) {
-  x = x < -200.0f ? -200.0f : x;  // minus infinity has no second part
-  const float t = x * 1.44269502f, r = __builtin_fmaf(x, 1.92596299e-8f, __builtin_fmaf(x, 1.44269502f, -t));
-  const float y = __builtin_amdgcn_exp2f(t);
-  return __builtin_fmaf(y, r * 0.693147182f, y);
-}
-__device__ inline double expOf(double x) { return exp(x); }
-__device__ inline float logOf(float x) { return logf(x); }
-__device__ inline double logOf(double x) { return log(x); }
-
-// ---- gate -----------------------------------------------------------------------------------------------------------
-
-// Unsigned keys in the order of the values: NaN above everything, both zeros the same, 0 for "no value". Keys of 16-bit types
-// carry the expert below the value, descending, so that one maximum finds both; 26 bits in all.
-template <typename T> struct GateKey;
-template <> struct GateKey<float> {
-  using key = uint32_t;
-  static constexpr bool packed = false;
-  __device__ static key of(float x, unsigned) {
-    const uint32_t u = __float_as_uint(x + 0.0f);
-    return x != x ? 0xFFFFFFFFu : (u & 0x80000000u) ? ~u : u | 0x80000000u;
-  }
-  __device__ static float value(key k) {
-    return k == 0xFFFFFFFFu ? __uint_as_float(0x7FC00000u) : __uint_as_float((k & 0x80000000u) ? k ^ 0x80000000u : ~k);
-  }
-  __device__ static bool open(key k) { return k > 0x007FFFFFu; }  // above minus infinity
-};
-template <> struct GateKey<double> {
-  using key = uint64_t;
-  static constexpr bool packed = false;
-  __device__ static key of(double x, unsigned) {
-    const uint64_t u = uint64_t(__double_as_longlong(x + 0.0));
-    return x != x ? ~0ull : (u >> 63) ? ~u : u | (1ull << 63);
-  }
-  __device__ static double value(key k) {
-    if (k == ~0ull) return __longlong_as_double(0x7FF8000000000000ll);
-    return __longlong_as_double((long long)((k >> 63) ? k ^ (1ull << 63) : ~k));
-  }
-  __device__ static bool open(key k) { return k > 0x000FFFFFFFFFFFFFull; }
-};
-template <typename T, uint32_t INF> struct GateKey16 {
-  using key = uint32_t;
-  static constexpr bool packed = true;
-  __device__ static key of(T x, unsigned e) {
-    uint32_t u = __builtin_bit_cast(uint16_t, x);
-    const bool nan = (u & 0x7FFFu) > INF;
-    u = u == 0x8000u ? 0u : u;
-    u = nan ? 0xFFFFu : (u & 0x8000u) ? u ^ 0xFFFFu : u | 0x8000u;
-    return u << 10 | (1023u - e);
-  }
-  __device__ static float value(key k) {
-    const uint32_t u = k >> 10;
-    const float x = float(__builtin_bit_cast(T, uint16_t((u & 0x8000u) ? u ^ 0x8000u : u ^ 0xFFFFu)));
-    return u == 0xFFFFu ? __uint_as_float(0x7FC00000u) : x;
-  }
-  __device__ static bool open(key k) { return k >> 10 > (INF ^ 0x7FFFu); }
-};
-template <> struct GateKey<__bf16> : GateKey16<__bf16, 0x7F80u> {};
-template <> struct GateKey<_Float16> : GateKey16<_Float16, 0x7C00u> {};
-
-// The expert of a lane's i-th logit. VEC: read four at a time.
-template <int G, bool VEC>
-__device__ inline unsigned gateExpert(int i, unsigned lane) {
-  return VEC ? (i / 4) * (4 * G) + 4 * lane + i % 4 : i * G + lane;
-}
-
-template <typename T, int G, int V, bool VEC>
-__device__ inline void gateLoad(const T* row, unsigned experts, unsigned lane, T (&z)[V]) {
-#pragma unroll
-  for (int i = 0; i < V; i += VEC ? 4 : 1) {
-    const unsigned e = gateExpert<G, VEC>(i, lane);
-    if constexpr (VEC) {
-      if (e < experts) {
-        const Pack<T, 4> p = *reinterpret_cast<const Pack<T, 4>*>(row + e);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) z[i + q] = p.v[q];
-      }
-    } else if (e < experts) {
-      z[i] = row[e];
-    }
-  }
-}
-
-// G lanes hold a row, V logits each. k rounds: the largest key of the group, the lowest expert that has it, and out it goes; lane
-// j keeps the choice of round j. The whole row is in registers, so the logits are read once.
-template <typename T, int G, int V, bool VEC>
-__global__ __launch_bounds__(BLOCK) void gateKernel(const T* __restrict__ logits, size_t n, unsigned experts, size_t stride, unsigned k,
-                                                    unsigned flags, int32_t* __restrict__ index, wide_t<T>* __restrict__ weight) {
-  using R = wide_t<T>;
-  using O = GateKey<T>;
-  using K = typename O::key;
-  const unsigned lane = threadIdx.x % G;
-  forTiles((n + BLOCK / G - 1) / (BLOCK / G), gridDim.x, [&](size_t tile) {
-    const size_t row = tile * (BLOCK / G) + threadIdx.x / G;
-    if (row >= n) return;  // whole groups leave; lanes are paired inside a group
-    T z[V];
-    K key[V];
-    gateLoad<T, G, V, VEC>(logits + row * stride, experts, lane, z);
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-      const unsigned e = gateExpert<G, VEC>(i, lane);
-      key[i] = e < experts ? O::of(z[i], e) : K(0);
-    }
-    K myKey = 0, topKey = 0, last = 0;
-    unsigned myIndex = 0;
-    R total = 0;
-    for (unsigned j = 0; j < k; ++j) {
-      K best = 0;
-      unsigned at = 0;
-      if constexpr (O::packed) {
-        // Keys are distinct and have 26 bits: modulo 2^32, key - last is above 2^31 for keys below the last choice and below 2^26
-        // for the others, so its maximum belongs to the largest key below, and nothing has to be taken out.
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const K below = j == 0 ? key[i] : key[i] - last;
-          best = below > best ? below : best;
-        }
-        best = groupMax<G>(best);
-        best = j == 0 ? best : best >> 31 ? best + last : K(0);
-        last = best ? best : last;
-        at = 1023u - (best & 1023u);
-      } else {
-#pragma unroll
-        for (int i = 0; i < V; ++i) best = key[i] > best ? key[i] : best;
-        best = groupMax<G>(best);
-        at = ~0u;
-#pragma unroll
-        for (int i = V - 1; i >= 0; --i) at = key[i] == best ? gateExpert<G, VEC>(i, lane) : at;
-        at = groupMin<G>(at);
-#pragma unroll
-        for (int i = 0; i < V; ++i)
-          if (gateExpert<G, VEC>(i, lane) == at) key[i] = 0;
-      }
-      if (j == 0) {
-        topKey = best;
-        if ((flags & SPNC_HIP_GATE_ALL) && O::open(best)) {
-          const R top = O::value(best);
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            const unsigned e = gateExpert<G, VEC>(i, lane);
-            if (e < experts && R(z[i]) != -INFINITY) total += expOf(R(z[i]) - top);
-          }
-          total = groupSum<G>(total);
-        }
-      }
-      if (lane == j) myKey = best, myIndex = at;
-    }
-    const bool open = lane < k && O::open(myKey);
-    const R shifted = open ? O::value(myKey) - O::value(topKey) : R(0);
-    const R e = open ? expOf(shifted) : R(0);
-    if (!(flags & SPNC_HIP_GATE_ALL)) total = groupSum<G>(e);
-    if (lane < k) {
-      index[row * k + lane] = open ? int32_t(myIndex) : -1;
-      weight[row * k + lane] = (flags & SPNC_HIP_GATE_LOG) ? (open ? shifted - logOf(total) : R(-INFINITY)) : open ? e / total : R(0);
-    }
-  });
-}
-
-// dz_e of the experts that were not chosen is 0, or -p_e times the sum over the slots under "all"; the k chosen ones get their
-// slot's term on top, through LDS: every lane has V of the row's entries in registers, and a slot's expert may be any of them.
-template <typename T, int G, int V, bool VEC>
-__global__ __launch_bounds__(BLOCK) void gateBackwardKernel(const T* __restrict__ logits, size_t n, unsigned experts, size_t stride, unsigned k,
-                                                            unsigned flags, const int32_t* __restrict__ index, const wide_t<T>* __restrict__ weight,
-                                                            const wide_t<T>* __restrict__ gradWeight, T* __restrict__ gradLogits) {
-  using R = wide_t<T>;
-  __shared__ R entries[BLOCK / G][V * G];
-  const unsigned lane = threadIdx.x % G;
-  R* const mine = entries[threadIdx.x / G];
-  const bool all = flags & SPNC_HIP_GATE_ALL, logs = flags & SPNC_HIP_GATE_LOG;
-  forTiles((n + BLOCK / G - 1) / (BLOCK / G), gridDim.x, [&](size_t tile) {
-    const size_t row = tile * (BLOCK / G) + threadIdx.x / G;
-    if (row >= n) return;
-    int32_t at = -1;
-    R d = 0, w = 0;
-    if (lane < k) {
-      at = index[row * k + lane];
-      if (at >= int32_t(experts)) at = -1;
-      if (at >= 0) {
-        d = gradWeight[row * k + lane];
-        w = weight[row * k + lane];
-        if (logs) w = w == -INFINITY ? R(0) : expOf(w);
-        else d *= w;
-      }
-    }
-    R dz[V] = {};
-    R top = -INFINITY, total = 0;
-    if (all) {
-      T z[V];
-      gateLoad<T, G, V, VEC>(logits + row * stride, experts, lane, z);
-      int bad = 0;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        dz[i] = gateExpert<G, VEC>(i, lane) < experts ? R(z[i]) : R(-INFINITY);
-        bad |= dz[i] != dz[i];
-        top = dz[i] > top ? dz[i] : top;
-      }
-      top = groupMax<G>(top);
-      if (groupMax<G>(bad)) top = NAN;
-#pragma unroll
-      for (int i = 0; i < V; ++i) {
-        dz[i] = dz[i] == -INFINITY ? R(0) : expOf(dz[i] - top);
-        total += dz[i];
-      }
-      total = groupSum<G>(total);
-    }
-    const R common = groupSum<G>(d);
-    if (!all) d -= w * common;
-    const R factor = total == 0 ? R(0) : -common / total;
-#pragma unroll
-    for (int i = 0; i < V; i += VEC ? 4 : 1) {
-      const unsigned e = gateExpert<G, VEC>(i, lane);
-      if constexpr (VEC) {
-        Pack<R, 4> p;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) p.v[q] = dz[i + q] * factor;
-        *reinterpret_cast<Pack<R, 4>*>(mine + e) = p;
-      } else {
-        mine[e] = dz[i] * factor;
-      }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the group is part of one wave, whose LDS accesses stay in order
-    if (at >= 0) mine[at] += d;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-#pragma unroll
-    for (int i = 0; i < V; i += VEC ? 4 : 1) {
-      const unsigned e = gateExpert<G, VEC>(i, lane);
-      if constexpr (VEC) {
-        const Pack<R, 4> p = *reinterpret_cast<const Pack<R, 4>*>(mine + e);
-        Pack<T, 4> o;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) o.v[q] = T(p.v[q]);
-        if (e < experts) *reinterpret_cast<Pack<T, 4>*>(gradLogits + row * experts + e) = o;
-      } else if (e < experts) {
-        gradLogits[row * experts + e] = T(mine[e]);
-      }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  });
-}
 
 // ---- routing --------------------------------------------------------------------------------------------------------
 
@@ -479,30 +132,6 @@ __global__ __launch_bounds__(ROUTE_BLOCK) void routeKernel(const int32_t* __rest
 }
 
 // ---- rows there and back --------------------------------------------------------------------------------------------
-
-// A group of 2^shift lanes handles a row, a piece of up to 16 bytes a lane at a time.
-//
-// Rows that are written to scattered places bypass the caches where they consist of whole 64-byte halves of cache lines: 1 M rows
-// of 64 bytes to two places each take 36 us instead of 50, of 2 KB to four places 52 instead of 67 (a consumer that reads
-// them next loses up to half of that where they would have fit the last-level cache). Rows that share their halves must not: 48
-// bytes take 87 us instead of 61, since each piece goes to memory by itself.
-struct RowShape {
-  unsigned pieces;  // of a row
-  unsigned shift;
-  size_t tiles;
-  bool stream;      // scattered rows are written past the caches
-};
-
-RowShape rowShape(size_t n, size_t rowBytes, unsigned pieceBytes, const void* scattered = nullptr) {
-  RowShape s;
-  s.pieces = unsigned(rowBytes / pieceBytes);
-  s.shift = 0;
-  while (s.shift < 6 && (1u << s.shift) < s.pieces) ++s.shift;
-  const size_t rows = BLOCK >> s.shift;
-  s.tiles = (n + rows - 1) / rows;
-  s.stream = pieceBytes == 16 && rowBytes % 64 == 0 && reinterpret_cast<uintptr_t>(scattered) % 64 == 0;
-  return s;
-}
 
 // Rows of the sorted buffer that belong to no segment, cleared by blocks of their own behind the rowBlocks that write the
 // others: a wave for what follows each segment, all of them for what follows the last one.
@@ -803,140 +432,7 @@ __global__ __launch_bounds__(BLOCK) void combineLogBackwardKernel(const R* __res
   });
 }
 
-// ---- dropout --------------------------------------------------------------------------------------------------------
-
-template <typename R>
-struct Dropout {
-  uint64_t threshold;
-  R scale, fill;
-  uint64_t seed, offset;
-  const uint64_t* offsetDevice;
-
-  __device__ Philox4 words(size_t block, uint64_t at) const {
-    return philox4x32(uint32_t(block), uint32_t(block >> 32), uint32_t(at), uint32_t(at >> 32), uint32_t(seed), uint32_t(seed >> 32));
-  }
-  template <typename T>
-  __device__ T apply(uint32_t word, T x) const {
-    return T(word >= threshold ? R(x) * scale : fill);
-  }
-};
-
-template <typename T> constexpr int DROPOUT_UNIT = sizeof(T) == 2 ? 8 : 4;  // elements of 16 bytes, at least the four of one counter
-constexpr unsigned DROPOUT_UNITS = 2;                                       // of a thread
-
-// Contiguous elements; VEC: read and written 16 bytes at a time.
-template <typename T, bool VEC>
-__global__ __launch_bounds__(BLOCK) void dropoutFlatKernel(const T* x, size_t elements, T* out, Dropout<wide_t<T>> d) {
-  constexpr int E = DROPOUT_UNIT<T>;
-  using P = Pack<T, E>;
-  const uint64_t at = d.offsetDevice ? *d.offsetDevice : d.offset;
-  const size_t units = (elements + E - 1) / E, tiles = (units + DROPOUT_UNITS * BLOCK - 1) / (DROPOUT_UNITS * BLOCK);
-  for (size_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const size_t first = tile * (DROPOUT_UNITS * BLOCK) + threadIdx.x;
-    P v[DROPOUT_UNITS];
-#pragma unroll
-    for (unsigned i = 0; i < DROPOUT_UNITS; ++i) {
-      const size_t e = (first + i * BLOCK) * E;
-      if (VEC && e + E <= elements) v[i] = *reinterpret_cast<const P*>(x + e);
-      else
-#pragma unroll
-        for (int q = 0; q < E; ++q)
-          if (e + q < elements) v[i].v[q] = x[e + q];
-    }
-#pragma unroll
-    for (unsigned i = 0; i < DROPOUT_UNITS; ++i) {
-      const size_t e = (first + i * BLOCK) * E;
-      if (e >= elements) continue;
-#pragma unroll
-      for (int b = 0; b < E / 4; ++b) {
-        const Philox4 r = d.words(e / 4 + b, at);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) v[i].v[4 * b + q] = d.apply(r.w[q], v[i].v[4 * b + q]);
-      }
-      if (VEC && e + E <= elements) *reinterpret_cast<P*>(out + e) = v[i];
-      else
-#pragma unroll
-        for (int q = 0; q < E; ++q)
-          if (e + q < elements) out[e + q] = v[i].v[q];
-    }
-  }
-}
-
-// Rows that are not adjacent; VEC: widths, strides and addresses in multiples of four elements, so that a counter's four
-// elements are neighbours. Otherwise a counter whose elements lie in two rows is computed for both.
-template <typename T, bool VEC>
-__global__ __launch_bounds__(BLOCK) void dropoutRowsKernel(const T* x, size_t n, size_t width, size_t stride, T* out, size_t outStride, RowShape shape,
-                                                           Dropout<wide_t<T>> d) {
-  const uint64_t at = d.offsetDevice ? *d.offsetDevice : d.offset;
-  const unsigned lane = threadIdx.x & ((1u << shape.shift) - 1);
-  forTiles(shape.tiles, gridDim.x, [&](size_t tile) {
-    const size_t row = tile * (BLOCK >> shape.shift) + (threadIdx.x >> shape.shift);
-    if (row >= n) return;
-    const size_t begin = row * width, end = begin + width;
-    const T* from = x + row * stride;
-    T* to = out + row * outStride;
-    for (size_t b = begin / 4 + lane; 4 * b < end; b += size_t(1) << shape.shift) {
-      const Philox4 r = d.words(b, at);
-      if constexpr (VEC) {
-        Pack<T, 4> v = *reinterpret_cast<const Pack<T, 4>*>(from + (4 * b - begin));
-#pragma unroll
-        for (int q = 0; q < 4; ++q) v.v[q] = d.apply(r.w[q], v.v[q]);
-        *reinterpret_cast<Pack<T, 4>*>(to + (4 * b - begin)) = v;
-      } else {
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const size_t e = 4 * b + q;
-          if (e >= begin && e < end) to[e - begin] = d.apply(r.w[q], from[e - begin]);
-        }
-      }
-    }
-  });
-}
-
 // ---- host side ------------------------------------------------------------------------------------------------------
-
-[[noreturn]] void refuse(const std::string& what) { throw std::runtime_error(what); }
-
-void launched(const char* what) {
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) refuse(std::string(what) + " launch: " + hipGetErrorString(e));
-}
-
-size_t elementBytes(int dtype) {
-  switch (dtype) {
-    case SPNC_HIP_FLOAT32: return 4;
-    case SPNC_HIP_FLOAT64: return 8;
-    case SPNC_HIP_FLOAT16:
-    case SPNC_HIP_BFLOAT16: return 2;
-  }
-  refuse("unknown element type " + std::to_string(dtype));
-}
-
-// calls fn(T()) for the element type
-template <typename Fn>
-void withType(int dtype, Fn&& fn) {
-  switch (dtype) {
-    case SPNC_HIP_FLOAT32: return fn(float());
-    case SPNC_HIP_FLOAT64: return fn(double());
-    case SPNC_HIP_FLOAT16: return fn(_Float16());
-    case SPNC_HIP_BFLOAT16: return fn(__bf16());
-  }
-  refuse("unknown element type " + std::to_string(dtype));
-}
-
-// the widest piece, in bytes, that a row of rowBytes at these addresses and strides consists of; `least` at the least
-unsigned pieceBytes(unsigned least, std::initializer_list<uintptr_t> addresses) {
-  uintptr_t bits = 16;
-  for (uintptr_t a : addresses) bits |= a;
-  const unsigned widest = unsigned(bits & (~bits + 1));
-  return widest < least ? 0 : widest;
-}
-
-uintptr_t address(const void* p) { return reinterpret_cast<uintptr_t>(p); }
-
-void checkAligned(unsigned piece, const char* what) {
-  if (piece == 0) refuse(std::string(what) + ": pointers are not aligned to the element type");
-}
 
 void checkSlots(size_t n, unsigned k, size_t capacity) {
   if (k == 0) refuse("k must be at least 1");
@@ -944,44 +440,9 @@ void checkSlots(size_t n, unsigned k, size_t capacity) {
   if (capacity >= (size_t(1) << 31)) refuse("too many rows: the capacity must be below 2^31");
 }
 
-void checkExperts(unsigned experts) {
-  if (experts == 0 || experts > SPNC_HIP_MAX_EXPERTS) refuse("experts must be between 1 and " + std::to_string(SPNC_HIP_MAX_EXPERTS));
-}
-
 void checkWeightType(int dtype, int weightDtype) {
   if (weightDtype != SPNC_HIP_FLOAT32 && !(weightDtype == SPNC_HIP_FLOAT64 && dtype == SPNC_HIP_FLOAT64))
     refuse("weights must be float32, or float64 with float64 values");
-}
-
-// calls fn(G, V, VEC): a row's logits in G lanes of V; at least as many lanes as choices, four logits a lane until 64 lanes are used
-template <typename T, typename Fn>
-void withGateShape(unsigned experts, unsigned k, size_t stride, uintptr_t addresses, Fn&& fn) {
-  unsigned group = 1;
-  while (group < WAVE && (4 * group < experts || group < k)) group *= 2;
-  const bool vec = (experts | stride) % 4 == 0 && addresses % alignof(Pack<T, 4>) == 0;
-  auto shape = [&](auto g, auto v) { vec ? fn(g, v, std::true_type()) : fn(g, v, std::false_type()); };
-#define SPN_GATE_SHAPE(G, V) return shape(std::integral_constant<int, G>(), std::integral_constant<int, V>())
-  switch (group) {
-    case 1: SPN_GATE_SHAPE(1, 4);
-    case 2: SPN_GATE_SHAPE(2, 4);
-    case 4: SPN_GATE_SHAPE(4, 4);
-    case 8: SPN_GATE_SHAPE(8, 4);
-    case 16: SPN_GATE_SHAPE(16, 4);
-    case 32: SPN_GATE_SHAPE(32, 4);
-  }
-  if (experts <= 256) SPN_GATE_SHAPE(64, 4);
-  if (experts <= 512) SPN_GATE_SHAPE(64, 8);
-  SPN_GATE_SHAPE(64, 16);
-#undef SPN_GATE_SHAPE
-}
-
-void checkGate(int dtype, size_t n, unsigned experts, size_t stride, unsigned k, unsigned flags) {
-  elementBytes(dtype);
-  checkExperts(experts);
-  if (k == 0 || k > experts || k > SPNC_HIP_MAX_CHOICES)
-    refuse("k must be between 1 and the number of experts, at most " + std::to_string(SPNC_HIP_MAX_CHOICES));
-  if (n > 1 && stride < experts) refuse("rows of logits overlap");
-  if (flags & ~unsigned(SPNC_HIP_GATE_ALL | SPNC_HIP_GATE_LOG)) refuse("unknown gate flags");
 }
 
 template <typename Fn>
@@ -1072,45 +533,6 @@ void withLogTypes(int dtype, int weightDtype, Fn&& fn) {
 using namespace spnc_hip;
 
 extern "C" {
-
-int spnc_hip_gate(const void* logits, int dtype, size_t n, unsigned experts, size_t stride, unsigned k, unsigned flags, int32_t* index,
-                  void* weight, void* stream) {
-  return guarded([&] {
-    checkGate(dtype, n, experts, stride, k, flags);
-    if (n == 0) return;
-    if (!logits || !index || !weight) refuse("null argument");
-    withType(dtype, [&](auto t) {
-      using T = decltype(t);
-      withGateShape<T>(experts, k, stride, address(logits), [&](auto g, auto v, auto vec) {
-        constexpr int G = decltype(g)::value, V = decltype(v)::value;
-        gateKernel<T, G, V, decltype(vec)::value><<<tileGrid((n + BLOCK / G - 1) / (BLOCK / G)), BLOCK, 0, static_cast<hipStream_t>(stream)>>>(
-            static_cast<const T*>(logits), n, experts, stride, k, flags, index, static_cast<wide_t<T>*>(weight));
-      });
-    });
-    launched("gate");
-  });
-}
-
-int spnc_hip_gate_backward(const void* logits, int dtype, size_t n, unsigned experts, size_t stride, unsigned k, unsigned flags,
-                           const int32_t* index, const void* weight, const void* grad_weight, void* grad_logits, void* stream) {
-  return guarded([&] {
-    checkGate(dtype, n, experts, stride, k, flags);
-    if (n == 0) return;
-    if ((!logits && (flags & SPNC_HIP_GATE_ALL)) || !index || !weight || !grad_weight || !grad_logits) refuse("null argument");
-    withType(dtype, [&](auto t) {
-      using T = decltype(t);
-      using R = wide_t<T>;
-      withGateShape<T>(experts, k, (flags & SPNC_HIP_GATE_ALL) ? stride : experts,
-                       address(grad_logits) | ((flags & SPNC_HIP_GATE_ALL) ? address(logits) : 0), [&](auto g, auto v, auto vec) {
-        constexpr int G = decltype(g)::value, V = decltype(v)::value;
-        gateBackwardKernel<T, G, V, decltype(vec)::value><<<tileGrid((n + BLOCK / G - 1) / (BLOCK / G)), BLOCK, 0, static_cast<hipStream_t>(stream)>>>(
-            static_cast<const T*>(logits), n, experts, stride, k, flags, index, static_cast<const R*>(weight), static_cast<const R*>(grad_weight),
-            static_cast<T*>(grad_logits));
-      });
-    });
-    launched("gate gradient");
-  });
-}
 
 size_t spnc_hip_route_workspace(size_t slots, unsigned experts) {
   const RouteShape shape = routeShape(slots, experts);
@@ -1287,44 +709,6 @@ int spnc_hip_combine_log_backward(const void* values, int dtype, size_t capacity
       });
     });
     launched("combine_log gradient");
-  });
-}
-
-int spnc_hip_dropout(const void* x, int dtype, size_t n, size_t width, size_t stride, void* out, size_t out_stride, double p, int mode,
-                     uint64_t seed, uint64_t offset, const uint64_t* offset_device, void* stream) {
-  return guarded([&] {
-    elementBytes(dtype);
-    if (!(p >= 0.0 && p <= 1.0)) refuse("the probability of dropping an element must be between 0 and 1");
-    if (mode < SPNC_HIP_DROPOUT_ZERO || mode > SPNC_HIP_DROPOUT_MASK) refuse("unknown dropout mode " + std::to_string(mode));
-    if (n > 1 && (stride < width || out_stride < width)) refuse("rows overlap");
-    if (n == 0 || width == 0) return;
-    if (!x || !out) refuse("null argument");
-    const uint64_t threshold = uint64_t(std::llrint(p * 4294967296.0));
-    const double scale = mode != SPNC_HIP_DROPOUT_ZERO ? 1.0 : threshold >> 32 ? 0.0 : 1.0 / (1.0 - p);
-    const double fill = mode == SPNC_HIP_DROPOUT_MARGINAL ? NAN : 0.0;
-    const hipStream_t s = static_cast<hipStream_t>(stream);
-    withType(dtype, [&](auto t) {
-      using T = decltype(t);
-      using R = wide_t<T>;
-      const Dropout<R> d{threshold, R(scale), R(fill), seed, offset, offset_device};
-      const uintptr_t bits = address(x) | address(out);
-      if (n == 1 || (stride == width && out_stride == width)) {
-        constexpr int E = DROPOUT_UNIT<T>;
-        const size_t elements = n * width, units = (elements + E - 1) / E, blocks = (units + DROPOUT_UNITS * BLOCK - 1) / (DROPOUT_UNITS * BLOCK);
-        const unsigned grid = unsigned(blocks < MAX_GRID ? blocks : MAX_GRID);
-        if (bits % (sizeof(Pack<T, E>) < 16 ? sizeof(Pack<T, E>) : 16) == 0)
-          dropoutFlatKernel<T, true><<<grid, BLOCK, 0, s>>>(static_cast<const T*>(x), elements, static_cast<T*>(out), d);
-        else
-          dropoutFlatKernel<T, false><<<grid, BLOCK, 0, s>>>(static_cast<const T*>(x), elements, static_cast<T*>(out), d);
-      } else {
-        const RowShape shape = rowShape(n, (width + 3) / 4, 1);
-        if (((width | stride | out_stride) % 4 | bits % (4 * sizeof(T) < 16 ? 4 * sizeof(T) : 16)) == 0)
-          dropoutRowsKernel<T, true><<<tileGrid(shape.tiles), BLOCK, 0, s>>>(static_cast<const T*>(x), n, width, stride, static_cast<T*>(out), out_stride, shape, d);
-        else
-          dropoutRowsKernel<T, false><<<tileGrid(shape.tiles), BLOCK, 0, s>>>(static_cast<const T*>(x), n, width, stride, static_cast<T*>(out), out_stride, shape, d);
-      }
-    });
-    launched("dropout");
   });
 }
 

@@ -221,6 +221,39 @@ def test_gate(native, dtype, over, log):
         assert (_host(got)[~np.isfinite(_host(z))] == 0).all()      # closed experts have no gradient
 
 
+@pytest.mark.parametrize("over,log", [("chosen", True), ("chosen", False), ("all", True), ("all", False)])
+def test_oracles_of_the_gate_agree(over, log):
+    z = _gate_logits(40, 12, "float32", seed=2).double().numpy()
+    grad = np.random.default_rng(3).normal(size=(40, 5))
+    index, weight = om.gate(z, 5, over, log)
+    many = om.gate_many(z, 5, over, log, grad)
+    assert np.array_equal(index, many[0]) and np.allclose(weight, many[1], rtol=1e-13, atol=1e-13)
+    assert np.allclose(om.gate_gradient(z, index, grad, over, log), many[2], rtol=1e-12, atol=1e-13)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "float64", "float16", "bfloat16"])
+@pytest.mark.parametrize("experts,k", [(3, 2), (10, 2), (33, 1), (64, 4), (67, 4), (96, 20), (130, 8), (256, 4), (509, 8), (511, 3), (512, 6), (1023, 2), (1024, 40)])
+def test_gate_of_many_rows(native, dtype, experts, k):
+    """From 8192 rows on a row is held by fewer lanes. Tolerances as in test_gate."""
+    torch = _torch()
+    from spnc import mixture as m
+    n, u = 8192 + 61, HALF["float64" if dtype == "float64" else "float32"]
+    z = _gate_logits(n, experts, dtype, seed=experts, masked=0.3)
+    grad = torch.randn(n, k, dtype=torch.float64 if dtype == "float64" else torch.float32, generator=torch.Generator().manual_seed(n))
+    wide = torch.zeros(n, experts + 7, dtype=z.dtype, device="cuda")
+    wide[:, 3:experts + 3] = z.cuda()
+    for over, log, dev in (("all", True, z.cuda()), ("chosen", False, z.cuda()), ("all", False, wide[:, 3:experts + 3])):
+        dev = dev.detach().requires_grad_()
+        index, weight = m.gate(dev, k, over=over, log=log)
+        got, = torch.autograd.grad(weight, dev, grad.cuda())
+        want_index, want, want_grad = om.gate_many(z.double().numpy(), k, over, log, _host(grad))
+        assert np.array_equal(_host(index), want_index)
+        _near(weight, want, (24 + experts) * u * (np.maximum(1.0, np.abs(np.where(np.isfinite(want), want, 0))) if log else np.maximum(np.abs(want), 1e-30)))
+        scale = np.abs(_host(grad)).sum(axis=1, keepdims=True)
+        _near(got, want_grad, (24 + experts + 2 * k) * u * scale + HALF[dtype] * np.abs(want_grad) + (2.0 ** -25 if dtype == "float16" else 0))
+
+
 @pytest.mark.gpu
 def test_gate_of_nan_and_infinity(native):
     torch = _torch()
@@ -232,6 +265,8 @@ def test_gate_of_nan_and_infinity(native):
             index, weight = m.gate(z.to(dtype).cuda(), 2, over=over)
             assert index.tolist() == [[1, 3], [0, 2], [2, 1], [3, -1]], (dtype, over)
             assert torch.isnan(weight[0]).all() and torch.isnan(weight[2]).all() and weight[3].tolist() == [1.0, 0.0]
+            many = m.gate(z.repeat(3000, 1).to(dtype).cuda(), 2, over=over)
+            assert torch.equal(many[0], index.repeat(3000, 1)) and torch.equal(many[1].nan_to_num(7.0), weight.repeat(3000, 1).nan_to_num(7.0))
 
 
 @pytest.mark.gpu
