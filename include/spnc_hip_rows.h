@@ -33,7 +33,7 @@ enum {
 /* logits [n, experts], rows `stride` elements apart -> index int32 [n, k], weight [n, k] (float64 for float64 logits,
  * else float32): the k largest logits of a row in descending order, equal ones by ascending index, NaN above everything.
  * Minus infinity closes an expert to a row: it is never chosen, and slots left over hold index -1 and weight 0 (log
- * weight minus infinity). 1 <= k <= min(experts, SPNC_HIP_MAX_CHOICES), experts <= SPNC_HIP_MAX_EXPERTS. */
+ * weight minus infinity). 1 <= k <= min(experts, SPNC_HIP_MAX_CHOICES), experts <= SPNC_HIP_MAX_EXPERTS, stride < 2^20. */
 SPNC_HIP_API int spnc_hip_gate(const void* logits, int dtype, size_t n, unsigned experts, size_t stride, unsigned k, unsigned flags,
                                int32_t* index, void* weight, void* stream);
 

@@ -5,7 +5,8 @@ namespace spnc_hip {
 namespace {
 
 // Unsigned keys in the order of the values: NaN above everything, both zeros the same, 0 for "taken out". Keys of 16-bit types
-// carry the expert below the value, descending, so that one maximum finds both; 29 bits in all.
+// carry the expert below the value, descending, so that one maximum finds both. They have 29 bits and bit 30, which makes them
+// normal positive floats in the same order: v_med3_f32 sorts them into lists.
 template <typename T> struct GateKey;
 template <> struct GateKey<float> {
   using key = uint32_t;
@@ -40,14 +41,14 @@ struct GateKey16 {
   // As float these have at most 19 leading bits that are not zero.
   __device__ static key of(float x, int e) {
     const uint32_t u = GateKey<float>::of(x, e);
-    return ((u >> 3) & 0x1FFFFC00u) | ((1023u - unsigned(e)) & 1023u);
+    return ((u >> 3) & 0x1FFFFC00u) | (0x40000000u | ((1023u - unsigned(e)) & 1023u));
   }
-  __device__ static key ofNan(int e) { return 0x1FFFFC00u | ((1023u - unsigned(e)) & 1023u); }
+  __device__ static key ofNan(int e) { return 0x5FFFFC00u | ((1023u - unsigned(e)) & 1023u); }
   __device__ static float value(key k) {
-    const uint32_t u = k >> 10 << 13;
-    return (k >> 10) == 0x7FFFFu ? __uint_as_float(0x7FC00000u) : __uint_as_float((u & 0x80000000u) ? u ^ 0x80000000u : ~(u | 0x1FFFu));
+    const uint32_t u = (k << 3) & 0xFFFFE000u;
+    return u == 0xFFFFE000u ? __uint_as_float(0x7FC00000u) : __uint_as_float((u & 0x80000000u) ? u ^ 0x80000000u : ~(u | 0x1FFFu));
   }
-  __device__ static bool open(key k) { return k >> 10 > 0x007FFFFFu >> 13; }
+  __device__ static bool open(key k) { return k > 0x400FFFFFu; }  // above minus infinity, whose value is 0x3FF
 };
 template <> struct GateKey<__bf16> : GateKey16 {};
 template <> struct GateKey<_Float16> : GateKey16 {};
@@ -69,43 +70,88 @@ __device__ inline int gateExpert(int i, int lane, int odd) {
   return i / STEP * (STEP * G) + STEP * lane + i % STEP - (LAYOUT == GATE_PAIRS ? odd : 0);
 }
 
-// A row's logits, minus infinity in places without an expert. All loads are unconditional (a place past the end reads the last
-// one), so that they are under way together. A word at the border of a row reaches into the row beside it, which the first and
-// the last row do not have: `edge` reads those one by one.
+// The rows of a block as a buffer: loads beyond its end return zero without touching memory, so places without an expert need
+// no care, and one address with a constant per load serves a lane. Its size is rounded down to `unit` bytes.
+typedef __amdgpu_buffer_rsrc_t GateRows;
+
+template <typename T>
+__device__ inline GateRows gateRows(const T* first, size_t elements, unsigned unit) {
+  const size_t bytes = elements * sizeof(T) / unit * unit;
+  // word 3: 32-bit data, no stride
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(first), 0, int(bytes < 0x7FFFFFF0u ? bytes : 0x7FFFFFF0u), 0x00027000);
+}
+
+// Steps whose places are experts in every lane: the same for the whole kernel. Opaque, or the comparisons with it would be
+// kept from one tile to the next in registers that are not there.
+template <int G, int LAYOUT>
+__device__ inline int gateWholeSteps(int experts) {
+  int steps = experts / (gateStep(LAYOUT) * G);
+  asm volatile("" : "+s"(steps));
+  return steps;
+}
+template <int LAYOUT>
+__device__ inline bool gateWhole(int i, int steps) {
+  return (LAYOUT != GATE_PAIRS || i > 0) && i / gateStep(LAYOUT) < steps;
+}
+
+// A row's logits, minus infinity in places without an expert. `at` is where it begins, in elements from the buffer's start.
 template <typename T, int G, int V, int LAYOUT>
-__device__ inline void gateLoad(const T* row, int experts, int lane, int odd, bool edge, wide_t<T> (&z)[V]) {
-  T raw[V];
-  auto single = [&](int i) {
-    const int e = gateExpert<G, LAYOUT>(i, lane, odd);
-    raw[i] = row[e < 0 ? 0 : e < experts ? e : experts - 1];
-  };
-  if constexpr (LAYOUT == GATE_FOURS) {
+__device__ inline void gateLoad(GateRows rows, const T* row, unsigned at, int experts, int lane, int odd, bool last, wide_t<T> (&z)[V]) {
+  constexpr int STEP = gateStep(LAYOUT);
+  constexpr unsigned BYTES = STEP * sizeof(T);
+  const int from = int((at + STEP * lane - (LAYOUT == GATE_PAIRS ? odd : 0)) * sizeof(T));
+  Pack<T, STEP> raw[V / STEP];
 #pragma unroll
-    for (int i = 0; i < V; i += 4) {
-      const int e = gateExpert<G, LAYOUT>(i, lane, odd);
-      const Pack<T, 4> p = *reinterpret_cast<const Pack<T, 4>*>(row + (e < experts ? e : experts - 4));
-#pragma unroll
-      for (int q = 0; q < 4; ++q) raw[i + q] = p.v[q];
+  for (int i = 0; i < V / STEP; ++i) {
+    const int offset = from + i * int(BYTES * G);
+    if constexpr (BYTES == 2) raw[i] = __builtin_bit_cast(Pack<T, STEP>, __builtin_amdgcn_raw_buffer_load_b16(rows, offset, 0, 0));
+    if constexpr (BYTES == 4) raw[i] = __builtin_bit_cast(Pack<T, STEP>, __builtin_amdgcn_raw_buffer_load_b32(rows, offset, 0, 0));
+    if constexpr (BYTES == 8) raw[i] = __builtin_bit_cast(Pack<T, STEP>, __builtin_amdgcn_raw_buffer_load_b64(rows, offset, 0, 0));
+    if constexpr (BYTES == 16) raw[i] = __builtin_bit_cast(Pack<T, STEP>, __builtin_amdgcn_raw_buffer_load_b128(rows, offset, 0, 0));
+    if constexpr (BYTES == 32) {
+      const Words4 words[2] = {__builtin_amdgcn_raw_buffer_load_b128(rows, offset, 0, 0), __builtin_amdgcn_raw_buffer_load_b128(rows, offset + 16, 0, 0)};
+      raw[i] = __builtin_bit_cast(Pack<T, STEP>, words);
     }
-  } else if constexpr (LAYOUT == GATE_PAIRS) {
-    if (edge) {
-#pragma unroll
-      for (int i = 0; i < V; ++i) single(i);
-    } else {
-      const int last = ((experts - 1 + odd) & ~1) - odd;
-#pragma unroll
-      for (int i = 0; i < V; i += 2) {
-        const int e = gateExpert<G, LAYOUT>(i, lane, odd);
-        const Pack<T, 2> p = *reinterpret_cast<const Pack<T, 2>*>(row + (e < last ? e : last));
-        raw[i] = p.v[0], raw[i + 1] = p.v[1];
-      }
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < V; ++i) single(i);
   }
 #pragma unroll
-  for (int i = 0; i < V; ++i) z[i] = unsigned(gateExpert<G, LAYOUT>(i, lane, odd)) < unsigned(experts) ? wide_t<T>(raw[i]) : wide_t<T>(-INFINITY);
+  for (int i = 0; i < V; ++i) z[i] = wide_t<T>(raw[i / STEP].v[i % STEP]);
+  const int steps = gateWholeSteps<G, LAYOUT>(experts);
+#pragma unroll
+  for (int i = 0; i < V; i += STEP)
+    if (!gateWhole<LAYOUT>(i, steps)) {
+#pragma unroll
+      for (int q = 0; q < STEP; ++q) {
+        const int e = gateExpert<G, LAYOUT>(i + q, lane, odd);
+        if (unsigned(e) >= unsigned(experts)) z[i + q] = -INFINITY;
+        else if (LAYOUT == GATE_PAIRS && last && e == experts - 1) z[i + q] = wide_t<T>(row[e]);  // half a word at the buffer's end
+      }
+    }
+}
+
+// exp(z - top) for many z as 2^(z log2(e) - top log2(e)): one fused multiply-add and the hardware's exp2. The exponent is rounded
+// once, an error of |z - top| 2^-24 relative to the term. `off` is by how much the rounded top log2(e) is too small: the terms are
+// too large by a factor of 2^off, all alike, and a sum that has to be right by itself is multiplied by 2^-off.
+struct TermsFloat {
+  float shift, off;
+  __device__ explicit TermsFloat(float top) : shift(top * 1.44269502f), off(__builtin_fmaf(top, 1.44269502f, -(top * 1.44269502f))) {}
+  __device__ float term(float z) const { return __builtin_amdgcn_exp2f(__builtin_fmaf(z, 1.44269502f, -shift)); }
+  __device__ float sum(float total) const { return total * __builtin_amdgcn_exp2f(-off); }
+};
+struct TermsDouble {
+  double top;
+  __device__ explicit TermsDouble(double t) : top(t) {}
+  __device__ double term(double z) const { return exp(z - top); }
+  __device__ double sum(double total) const { return total; }
+};
+template <typename R> using Terms = typename std::conditional<std::is_same<R, double>::value, TermsDouble, TermsFloat>::type;
+
+// The largest keys of a lane in descending order, 0 where there are none.
+template <int DEPTH>
+__device__ inline void gateInsert(uint32_t (&list)[4], uint32_t key) {
+#pragma unroll
+  for (int d = DEPTH - 1; d > 0; --d)  // the middle of two neighbours and the new key, which is one or the other or the new one
+    list[d] = __float_as_uint(__builtin_amdgcn_fmed3f(__uint_as_float(list[d - 1]), __uint_as_float(list[d]), __uint_as_float(key)));
+  list[0] = key > list[0] ? key : list[0];
 }
 
 // G lanes hold a row, V logits each. k rounds: the largest key of the group, the lowest expert that has it, and out it goes; lane
@@ -122,8 +168,10 @@ __global__ __launch_bounds__(BLOCK) void gateKernel(const T* __restrict__ logits
     if (row >= n) return;  // whole groups leave; lanes are paired inside a group
     const T* const from = logits + row * stride;
     const int odd = LAYOUT == GATE_PAIRS ? gateOdd(from) : 0;
+    const size_t first = tile * (BLOCK / G);
+    const GateRows rows = gateRows(logits + first * stride, (n - 1 - first) * stride + experts, gateStep(LAYOUT) * sizeof(T));
     R z[V];
-    gateLoad<T, G, V, LAYOUT>(from, experts, lane, odd, row == 0 || row == n - 1, z);
+    gateLoad<T, G, V, LAYOUT>(rows, from, unsigned(threadIdx.x / G) * unsigned(stride), experts, lane, odd, row == n - 1, z);
     K key[V];
     bool nan = false;
 #pragma unroll
@@ -136,24 +184,34 @@ __global__ __launch_bounds__(BLOCK) void gateKernel(const T* __restrict__ logits
       for (int i = 0; i < V; ++i)
         if (z[i] != z[i]) key[i] = O::ofNan(gateExpert<G, LAYOUT>(i, lane, odd));
     }
-    K myKey = 0, topKey = 0, last = 0;
+    K myKey = 0, topKey = 0;
     int myIndex = 0;
     R total = 0;
+    [[maybe_unused]] uint32_t list[4] = {};
+    if constexpr (O::packed) {
+      // Every lane's four largest (two, if no more are asked for): four instructions a logit, after which a round only looks at the
+      // lists' heads. A lane that has more of the k largest than its list holds makes a new one of what is below.
+      if (k > 2) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) gateInsert<4>(list, key[i]);
+      } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) gateInsert<2>(list, key[i]);
+      }
+    }
     for (int j = 0; j < int(k); ++j) {
       K best = 0;
       int at = 0;
       if constexpr (O::packed) {
-        // Keys are distinct and have 29 bits: modulo 2^32, key - last is above 2^31 for keys below the last choice and below 2^29
-        // for the others, so its maximum belongs to the largest key below, and nothing has to be taken out.
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-          const K below = j == 0 ? key[i] : key[i] - last;
-          best = below > best ? below : best;
-        }
-        best = groupMax<G>(best);
-        best = j == 0 ? best : best >> 31 ? best + last : K(0);
-        last = best ? best : last;
+        best = groupMax<G>(list[0]);
         at = 1023 - int(best & 1023u);
+        if (list[0] == best) {  // keys are distinct: one lane
+          list[0] = list[1], list[1] = list[2], list[2] = list[3], list[3] = 0;
+          if (V > 4 && list[0] == 0 && j + 1 < int(k)) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) gateInsert<4>(list, key[i] < best ? key[i] : 0u);
+          }
+        }
       } else {
 #pragma unroll
         for (int i = 0; i < V; ++i) best = key[i] > best ? key[i] : best;
@@ -169,10 +227,10 @@ __global__ __launch_bounds__(BLOCK) void gateKernel(const T* __restrict__ logits
       if (j == 0) {
         topKey = best;
         if ((flags & SPNC_HIP_GATE_ALL) && O::open(best)) {
-          const R top = O::value(best);
+          const Terms<R> terms(O::value(best));
 #pragma unroll
-          for (int i = 0; i < V; ++i) total += expTerm(z[i] - top);
-          total = groupSum<G>(total);
+          for (int i = 0; i < V; ++i) total += terms.term(z[i]);
+          total = terms.sum(groupSum<G>(total));
         }
       }
       if (lane == j) myKey = best, myIndex = at;
@@ -189,91 +247,100 @@ __global__ __launch_bounds__(BLOCK) void gateKernel(const T* __restrict__ logits
 }
 
 // dz_e of the experts that were not chosen is 0, or -p_e times the sum over the slots under "all"; the k chosen ones get their
-// slot's term on top, through LDS: every lane has V of the row's entries in registers, and a slot's expert may be any of them.
+// slot's term on top. A block's rows are one stretch of the output. It is put together in LDS, the chosen entries over the others,
+// and goes out 16 bytes a lane whatever the width of a row: 65537 rows of 509 bfloat16 take 30 us, 40 if every group
+// writes its own row.
 template <typename T, int G, int V, int LAYOUT>
 __global__ __launch_bounds__(BLOCK) void gateBackwardKernel(const T* __restrict__ logits, size_t n, unsigned experts, size_t stride, unsigned k,
                                                             unsigned flags, const int32_t* __restrict__ index, const wide_t<T>* __restrict__ weight,
                                                             const wide_t<T>* __restrict__ gradWeight, T* __restrict__ gradLogits) {
   using R = wide_t<T>;
-  __shared__ R entries[BLOCK / G][V * G];
-  const int lane = threadIdx.x % G;
-  R* const mine = entries[threadIdx.x / G];
+  constexpr int ROWS = BLOCK / G, E16 = 16 / sizeof(T);
+  __shared__ alignas(16) T stretch[ROWS * V * G + E16];
+  const int lane = threadIdx.x % G, local = threadIdx.x / G;
   const bool all = flags & SPNC_HIP_GATE_ALL, logs = flags & SPNC_HIP_GATE_LOG;
-  forTiles((n + BLOCK / G - 1) / (BLOCK / G), gridDim.x, [&](size_t tile) {
-    const size_t row = tile * (BLOCK / G) + threadIdx.x / G;
-    if (row >= n) return;
-    int32_t at = -1;
-    R d = 0, w = 0;
-    if (lane < int(k)) {
-      at = index[row * k + lane];
-      if (at >= int32_t(experts)) at = -1;
-      if (at >= 0) {
-        d = gradWeight[row * k + lane];
-        w = weight[row * k + lane];
-        if (logs) w = w == -INFINITY ? R(0) : expOf(w);
-        else d *= w;
+  forTiles((n + ROWS - 1) / ROWS, gridDim.x, [&](size_t tile) {
+    const size_t row = tile * ROWS + local;
+    const int rows = n - tile * ROWS < size_t(ROWS) ? int(n - tile * ROWS) : ROWS;
+    T* const to = gradLogits + tile * ROWS * experts;
+    const int skew = int(reinterpret_cast<uintptr_t>(to) % 16 / sizeof(T));  // LDS is aligned as the output is
+    T* const mine = stretch + skew + local * int(experts);
+    if (row < n) {
+      int32_t at = -1;
+      R d = 0, w = 0;
+      if (lane < int(k)) {
+        at = index[row * k + lane];
+        if (at >= int32_t(experts)) at = -1;
+        if (at >= 0) {
+          d = gradWeight[row * k + lane];
+          w = weight[row * k + lane];
+          if (logs) w = expOf(w);
+          else d *= w;
+        }
       }
-    }
-    R dz[V] = {};
-    R total = 0;
-    int odd = 0;  // any layout of the entries will do without logits
-    const int32_t first = all ? index[row * k] : -1;  // the largest logit's, or NaN's; none: closed altogether
-    if (first >= 0 && first < int32_t(experts)) {
-      const T* const from = logits + row * stride;
-      const R top = R(from[first]);
-      if (LAYOUT == GATE_PAIRS) odd = gateOdd(from);
-      gateLoad<T, G, V, LAYOUT>(from, experts, lane, odd, row == 0 || row == n - 1, dz);
+      const R common = groupSum<G>(d);
+      if (all) {
+        R z[V];
+        const T* const from = logits + row * stride;
+        const int32_t first = index[row * k];  // the largest logit's, or NaN's; none: closed altogether
+        const bool any = first >= 0 && first < int32_t(experts);
+        const int odd = LAYOUT == GATE_PAIRS ? gateOdd(from) : 0;
+        const GateRows buffer = gateRows(logits + tile * ROWS * stride, (n - 1 - tile * ROWS) * stride + experts, gateStep(LAYOUT) * sizeof(T));
+        gateLoad<T, G, V, LAYOUT>(buffer, from, unsigned(local) * unsigned(stride), experts, lane, odd, row == n - 1, z);
+        const R top = any ? R(from[first]) : R(0);
+        const Terms<R> terms(top);
+        R total = 0;
 #pragma unroll
-      for (int i = 0; i < V; ++i) {
-        dz[i] = sizeof(T) == 2 ? expTerm(dz[i] - top) : expOf(dz[i] - top);
-        total += dz[i];
+        for (int i = 0; i < V; ++i) {
+          z[i] = sizeof(T) == 4 ? expOf(z[i] - top) : terms.term(z[i]);
+          total += z[i];
+        }
+        total = groupSum<G>(total);
+        const R factor = total == 0 ? R(0) : -common / total;
+        const int steps = gateWholeSteps<G, LAYOUT>(experts);
+#pragma unroll
+        for (int i = 0; i < V; i += gateStep(LAYOUT)) {
+          const int e = gateExpert<G, LAYOUT>(i, lane, odd);
+          if constexpr (LAYOUT == GATE_FOURS) {
+            const Pack<T, 4> p{{T(z[i] * factor), T(z[i + 1] * factor), T(z[i + 2] * factor), T(z[i + 3] * factor)}};
+            if (e < int(experts)) *reinterpret_cast<Pack<T, 4>*>(mine + e) = p;
+          } else if (gateWhole<LAYOUT>(i, steps)) {
+#pragma unroll
+            for (int q = 0; q < gateStep(LAYOUT); ++q) mine[e + q] = T(z[i + q] * factor);
+          } else {
+#pragma unroll
+            for (int q = 0; q < gateStep(LAYOUT); ++q)
+              if (unsigned(e + q) < experts) mine[e + q] = T(z[i + q] * factor);
+          }
+        }
+      } else {
+        constexpr int STEP = LAYOUT == GATE_FOURS ? 4 : 1;
+#pragma unroll
+        for (int i = 0; i < V; i += STEP) {
+          const int e = i * G + STEP * lane;
+          if (e < int(experts)) *reinterpret_cast<Pack<T, STEP>*>(mine + e) = Pack<T, STEP>{};
+        }
       }
-      total = groupSum<G>(total);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the group is part of one wave, whose LDS accesses stay in order
+      if (at >= 0) mine[at] = T(d - w * common);
     }
-    const R common = groupSum<G>(d);
-    if (!all) d -= w * common;
-    const R factor = total == 0 ? R(0) : -common / total;
-#pragma unroll
-    for (int i = 0; i < V; i += gateStep(LAYOUT)) {
-      const int e = gateExpert<G, LAYOUT>(i, lane, odd);
-      if constexpr (LAYOUT == GATE_FOURS) {
-        Pack<R, 4> p;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) p.v[q] = dz[i + q] * factor;
-        *reinterpret_cast<Pack<R, 4>*>(mine + e) = p;
+    __syncthreads();
+    const int begin = skew, end = skew + rows * int(experts);
+    for (int i = int(threadIdx.x) * E16; i < end; i += BLOCK * E16) {
+      if (i >= begin && i + E16 <= end) {
+        *reinterpret_cast<Pack<T, E16>*>(to + (i - skew)) = *reinterpret_cast<const Pack<T, E16>*>(stretch + i);
       } else {
 #pragma unroll
-        for (int q = 0; q < gateStep(LAYOUT); ++q)
-          if (unsigned(e + q) < experts) mine[e + q] = dz[i + q] * factor;
+        for (int q = 0; q < E16; ++q)
+          if (i + q >= begin && i + q < end) to[i + q - skew] = stretch[i + q];
       }
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the group is part of one wave, whose LDS accesses stay in order
-    if (at >= 0) mine[at] += d;
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    T* const to = gradLogits + row * experts;
-    if (LAYOUT == GATE_PAIRS) odd = gateOdd(to);
-#pragma unroll
-    for (int i = 0; i < V; i += gateStep(LAYOUT)) {
-      const int e = gateExpert<G, LAYOUT>(i, lane, odd);
-      if constexpr (LAYOUT == GATE_FOURS) {
-        const Pack<R, 4> p = *reinterpret_cast<const Pack<R, 4>*>(mine + e);
-        Pack<T, 4> o;
-#pragma unroll
-        for (int q = 0; q < 4; ++q) o.v[q] = T(p.v[q]);
-        if (e < int(experts)) *reinterpret_cast<Pack<T, 4>*>(to + e) = o;
-      } else if constexpr (LAYOUT == GATE_PAIRS) {
-        if (e >= 0 && e + 1 < int(experts)) *reinterpret_cast<Pack<T, 2>*>(to + e) = Pack<T, 2>{{T(mine[e]), T(mine[e + 1])}};
-        else if (unsigned(e) < experts) to[e] = T(mine[e]);
-        else if (unsigned(e + 1) < experts) to[e + 1] = T(mine[e + 1]);
-      } else if (e < int(experts)) {
-        to[e] = T(mine[e]);
-      }
-    }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __syncthreads();
   });
 }
 
 constexpr size_t GATE_MANY_ROWS = 8192;
+constexpr size_t GATE_MAX_STRIDE = 1u << 20;  // a block's rows, 256 at the most, lie within 2^31 bytes
 
 // calls fn(G, V, LAYOUT): a row's logits in G lanes of V, at least as many lanes as choices. A round costs a wave about 5 V + 14
 // instructions (3 V / 2 + 14 with packed keys) for 64 / G rows, so with many rows few lanes of many logits are cheapest, as far as the
@@ -282,7 +349,7 @@ template <typename T, typename Fn>
 void withGateShape(size_t n, unsigned experts, unsigned k, size_t stride, uintptr_t addresses, Fn&& fn) {
   constexpr bool packed = sizeof(T) == 2;
   const bool fours = (experts | stride) % 4 == 0 && addresses % alignof(Pack<T, 4>) == 0;
-  const bool pairs = packed && !fours && experts >= 16 && experts < SPNC_HIP_MAX_EXPERTS;
+  const bool pairs = packed && !fours && experts >= 16 && experts < SPNC_HIP_MAX_EXPERTS && addresses % 4 == 0;
   const unsigned places = experts + (pairs ? 1 : 0);  // an odd row's first word begins a place earlier
   unsigned group = 0, logits = 0, best = ~0u;
   for (unsigned v : {4u, 8u, 16u, 32u}) {
@@ -333,6 +400,7 @@ void checkGate(int dtype, size_t n, unsigned experts, size_t stride, unsigned k,
   if (k == 0 || k > experts || k > SPNC_HIP_MAX_CHOICES)
     refuse("k must be between 1 and the number of experts, at most " + std::to_string(SPNC_HIP_MAX_CHOICES));
   if (n > 1 && stride < experts) refuse("rows of logits overlap");
+  if (stride >= GATE_MAX_STRIDE) refuse("rows of logits must be less than 2^20 elements apart");
   if (flags & ~unsigned(SPNC_HIP_GATE_ALL | SPNC_HIP_GATE_LOG)) refuse("unknown gate flags");
 }
 

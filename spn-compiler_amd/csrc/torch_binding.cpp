@@ -103,9 +103,15 @@ Plan planOf(const Tensor& position, const Tensor& starts, const Tensor& counts, 
 
 // ---- gate -----------------------------------------------------------------------------------------------------------
 
+// Rows of logits a million elements and more apart are copied.
+Tensor logitsOf(const Tensor& t) {
+  const Tensor rows = rowsOf(t);
+  return rowStride(rows) < 1 << 20 ? rows : rows.contiguous();
+}
+
 std::pair<Tensor, Tensor> gateForward(const Tensor& given, int64_t k, int64_t flags) {
   c10::DeviceGuard guard(given.device());
-  const Tensor logits = rowsOf(given);
+  const Tensor logits = logitsOf(given);
   const int64_t n = logits.size(0);
   Tensor index = at::empty({n, k}, logits.options().dtype(at::kInt).requires_grad(false));
   Tensor weight = at::empty({n, k}, index.options().dtype(logits.scalar_type() == at::kDouble ? at::kDouble : at::kFloat));
@@ -128,7 +134,7 @@ struct Gate : torch::autograd::Function<Gate> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &index = saved[1], &weight = saved[2];
     c10::DeviceGuard guard(index.device());
-    const Tensor logits = saved[0].defined() ? rowsOf(saved[0]) : Tensor(), grad = grads[1].contiguous();
+    const Tensor logits = saved[0].defined() ? logitsOf(saved[0]) : Tensor(), grad = grads[1].contiguous();
     const int64_t flags = ctx->saved_data["flags"].toInt(), experts = ctx->saved_data["experts"].toInt();
     const auto type = at::ScalarType(ctx->saved_data["type"].toInt());
     Tensor result = at::empty({index.size(0), experts}, weight.options().dtype(type).requires_grad(false));
