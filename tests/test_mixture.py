@@ -141,6 +141,8 @@ def test_c_entry_points_refuse(native):
     refused(lib.spnc_hip_dropout(p, 0, 2, 4, 4, p, 4, float("nan"), 0, 0, 0, None, None), "probability")
     refused(lib.spnc_hip_dropout(p, 0, 2, 4, 3, p, 4, 0.5, 0, 0, 0, None, None), "overlap")
     refused(lib.spnc_hip_dropout(p, 0, 2, 4, 4, p, 4, 0.5, 3, 0, 0, None, None), "unknown dropout mode")
+    assert lib.spnc_hip_route_workspace(100000, 0) == 0 and lib.spnc_hip_route_workspace(100000, 70000) == 0
+    assert lib.spnc_hip_route_workspace(8192, 10) == 0 and lib.spnc_hip_route_workspace(100000, 10) > 0
     # nothing to do is no error
     assert lib.spnc_hip_gate(None, 0, 0, 3, 3, 1, 0, None, None, None) == 0
     assert lib.spnc_hip_combine(None, 0, 0, 4, 4, None, 0, 2, None, 0, None, None) == 0
