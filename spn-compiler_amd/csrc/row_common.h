@@ -45,13 +45,14 @@ __device__ inline void streamStore(P* p, const P& v) {
   else *p = v;
 }
 
-// Neighbouring tiles of rows go to one die: rows that are neighbours in the sorted buffer come from neighbouring rows,
-// and a cache line of narrow rows is then filled or read within one L2.
+// Tiles of rows, one a block at a time. byDie: neighbouring tiles go to one die (blocks are dealt to the dies in turn): rows that are
+// neighbours in the sorted buffer come from neighbouring rows, and a cache line of narrow rows is then filled or read within one L2.
 template <typename Body>
-__device__ inline void forTiles(size_t tiles, unsigned grid, Body&& body) {
-  const size_t perDie = (tiles + XCDS - 1) / XCDS, first = size_t(blockIdx.x % XCDS) * perDie;
-  for (size_t t = blockIdx.x / XCDS; t < perDie; t += grid / XCDS)
-    if (first + t < tiles) body(first + t);
+__device__ inline void forTiles(size_t tiles, unsigned grid, bool byDie, Body&& body) {
+  const size_t perDie = (tiles + XCDS - 1) / XCDS;
+  const size_t first = byDie ? size_t(blockIdx.x % XCDS) * perDie : 0, begin = byDie ? blockIdx.x / XCDS : blockIdx.x;
+  const size_t end = byDie ? (first + perDie < tiles ? perDie : tiles > first ? tiles - first : 0) : tiles, step = byDie ? grid / XCDS : grid;
+  for (size_t t = begin; t < end; t += step) body(first + t);
 }
 
 inline unsigned tileGrid(size_t tiles) {
@@ -70,6 +71,7 @@ struct RowShape {
   unsigned shift;
   size_t tiles;
   bool stream;      // scattered rows are written past the caches
+  bool byDie;
 };
 
 inline RowShape rowShape(size_t n, size_t rowBytes, unsigned pieceBytes, const void* scattered = nullptr) {
@@ -79,6 +81,9 @@ inline RowShape rowShape(size_t n, size_t rowBytes, unsigned pieceBytes, const v
   while (s.shift < 6 && (1u << s.shift) < s.pieces) ++s.shift;
   const size_t rows = BLOCK >> s.shift;
   s.tiles = (n + rows - 1) / rows;
+  // In the order of the blocks from 1 KB on: 4 x 32769 rows of 2 KB are combined in 59 us instead of 61. Of 8 bytes, 4 x 2 M rows take 32
+  // instead of 26 that way, of 24 bytes 78 instead of 67.
+  s.byDie = rowBytes < 1024;
   s.stream = pieceBytes == 16 && rowBytes % 64 == 0 && reinterpret_cast<uintptr_t>(scattered) % 64 == 0;
   return s;
 }

@@ -69,7 +69,7 @@ __global__ __launch_bounds__(BLOCK) void dropoutRowsKernel(const T* x, size_t n,
                                                            Dropout<wide_t<T>> d) {
   const uint64_t at = d.offsetDevice ? *d.offsetDevice : d.offset;
   const unsigned lane = threadIdx.x & ((1u << shape.shift) - 1);
-  forTiles(shape.tiles, gridDim.x, [&](size_t tile) {
+  forTiles(shape.tiles, gridDim.x, false, [&](size_t tile) {
     const size_t row = tile * (BLOCK >> shape.shift) + (threadIdx.x >> shape.shift);
     if (row >= n) return;
     const size_t begin = row * width, end = begin + width;

@@ -163,7 +163,7 @@ __global__ __launch_bounds__(BLOCK) void gateKernel(const T* __restrict__ logits
   using O = GateKey<T>;
   using K = typename O::key;
   const int lane = threadIdx.x % G;
-  forTiles((n + BLOCK / G - 1) / (BLOCK / G), gridDim.x, [&](size_t tile) {
+  forTiles((n + BLOCK / G - 1) / (BLOCK / G), gridDim.x, false, [&](size_t tile) {
     const size_t row = tile * (BLOCK / G) + threadIdx.x / G;
     if (row >= n) return;  // whole groups leave; lanes are paired inside a group
     const T* const from = logits + row * stride;
@@ -259,7 +259,7 @@ __global__ __launch_bounds__(BLOCK) void gateBackwardKernel(const T* __restrict_
   __shared__ alignas(16) T stretch[ROWS * V * G + E16];
   const int lane = threadIdx.x % G, local = threadIdx.x / G;
   const bool all = flags & SPNC_HIP_GATE_ALL, logs = flags & SPNC_HIP_GATE_LOG;
-  forTiles((n + ROWS - 1) / ROWS, gridDim.x, [&](size_t tile) {
+  forTiles((n + ROWS - 1) / ROWS, gridDim.x, false, [&](size_t tile) {
     const size_t row = tile * ROWS + local;
     const int rows = n - tile * ROWS < size_t(ROWS) ? int(n - tile * ROWS) : ROWS;
     T* const to = gradLogits + tile * ROWS * experts;

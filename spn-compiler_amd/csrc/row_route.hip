@@ -236,23 +236,35 @@ __global__ __launch_bounds__(BLOCK) void dispatchKernel(const unsigned char* __r
                                                         Unused unused) {
   if (blockIdx.x >= unused.rowBlocks) return clearUnused(unused);
   const unsigned lane = threadIdx.x & ((1u << shape.shift) - 1);
-  forTiles(shape.tiles, unused.rowBlocks, [&](size_t tile) {
+  forTiles(shape.tiles, unused.rowBlocks, shape.byDie, [&](size_t tile) {
     const size_t row = tile * (BLOCK >> shape.shift) + (threadIdx.x >> shape.shift);
     if (row >= n) return;
     const P* source = reinterpret_cast<const P*>(rows + row * strideBytes);
     for (unsigned first = 0; first < k; first += KB) {
       int32_t at[KB];
       loadPositions<KB>(position, row, k, first, capacity, at);
-      for (unsigned c = lane; c < shape.pieces; c += 1u << shape.shift) {
-        const P piece = source[c];
+      // H pieces a lane at a time, H - 1 of which may lie behind the row's end
+      auto copy = [&](auto h) {
+        constexpr unsigned H = decltype(h)::value;
+        for (unsigned c = lane; c < shape.pieces; c += H << shape.shift) {
+          P piece[H];
 #pragma unroll
-        for (int j = 0; j < KB; ++j)
-          if (at[j] >= 0) {
-            P* const to = &out[size_t(at[j]) * shape.pieces + c];
-            if constexpr (STREAM) streamStore(to, piece);
-            else *to = piece;
-          }
-      }
+          for (unsigned i = 0; i < H; ++i)
+            if (i == 0 || c + (i << shape.shift) < shape.pieces) piece[i] = source[c + (i << shape.shift)];
+#pragma unroll
+          for (unsigned i = 0; i < H; ++i)
+            if (i == 0 || c + (i << shape.shift) < shape.pieces)
+#pragma unroll
+              for (int j = 0; j < KB; ++j)
+                if (at[j] >= 0) {
+                  P* const to = &out[size_t(at[j]) * shape.pieces + c + (i << shape.shift)];
+                  if constexpr (STREAM) streamStore(to, piece[i]);
+                  else *to = piece[i];
+                }
+        }
+      };
+      if (shape.pieces > 1u << shape.shift) copy(std::integral_constant<unsigned, 2>());
+      else copy(std::integral_constant<unsigned, 1>());
     }
   });
 }
@@ -260,14 +272,15 @@ __global__ __launch_bounds__(BLOCK) void dispatchKernel(const unsigned char* __r
 // Slots are read KB at a time, all loads before the first product; a slot that is not routed reads row 0 and drops it. Results
 // bypass the caches, which leaves the values there for the backward pass (32769 x 4 rows of 2 KB, forward and backward: 164 us
 // instead of 191), and so do values without weights: gradients of dispatch, whose last use this is (139 instead of 150 us for the
-// whole of routing, dispatch and its gradient at that size).
+// whole of routing, dispatch and its gradient at that size). Two pieces a lane at a time, where a row has them for all
+// lanes: 59 us instead of 69.
 template <typename T, int N, typename W, int KB, bool ONE, bool WEIGHTED>
 __global__ __launch_bounds__(BLOCK) void combineKernel(const T* __restrict__ values, size_t capacity, size_t stride, RowShape shape,
                                                        const int32_t* __restrict__ position, size_t n, unsigned k, const W* __restrict__ weight,
                                                        Pack<T, N>* __restrict__ out) {
   using R = wide_t<T>;
   const unsigned lane = threadIdx.x & ((1u << shape.shift) - 1);
-  forTiles(shape.tiles, gridDim.x, [&](size_t tile) {
+  forTiles(shape.tiles, gridDim.x, shape.byDie, [&](size_t tile) {
     const size_t row = tile * (BLOCK >> shape.shift) + (threadIdx.x >> shape.shift);
     if (row >= n) return;
     int32_t at[KB];
@@ -276,30 +289,42 @@ __global__ __launch_bounds__(BLOCK) void combineKernel(const T* __restrict__ val
       loadPositions<KB>(position, row, k, 0, capacity, at);
       loadWeights<KB>(WEIGHTED ? weight : nullptr, row, k, 0, w);
     }
-    for (unsigned c = lane; c < shape.pieces; c += 1u << shape.shift) {
-      R sum[N] = {};
-      for (unsigned first = 0; first < (ONE ? 1 : k); first += KB) {
-        if (!ONE) {
-          loadPositions<KB>(position, row, k, first, capacity, at);
-          loadWeights<KB>(WEIGHTED ? weight : nullptr, row, k, first, w);
-        }
-        Pack<T, N> v[KB];
-#pragma unroll
-        for (int j = 0; j < KB; ++j)
-          if (capacity) {
-            const Pack<T, N>* from = reinterpret_cast<const Pack<T, N>*>(values + size_t(at[j] >= 0 ? at[j] : 0) * stride + size_t(c) * N);
-            v[j] = WEIGHTED ? *from : streamLoad(from);
+    auto join = [&](auto h) {
+      constexpr unsigned H = decltype(h)::value;
+      for (unsigned c = lane; c < shape.pieces; c += H << shape.shift) {
+        const unsigned place[2] = {c, c + (1u << shape.shift)};
+        R sum[H][N] = {};
+        for (unsigned first = 0; first < (ONE ? 1 : k); first += KB) {
+          if (!ONE) {
+            loadPositions<KB>(position, row, k, first, capacity, at);
+            loadWeights<KB>(WEIGHTED ? weight : nullptr, row, k, first, w);
           }
+          Pack<T, N> v[H][KB];
 #pragma unroll
-        for (int j = 0; j < KB; ++j)
+          for (unsigned q = 0; q < H; ++q)
 #pragma unroll
-          for (int i = 0; i < N; ++i) sum[i] += at[j] >= 0 ? w[j] * R(v[j].v[i]) : R(0);
+            for (int j = 0; j < KB; ++j) {
+              const Pack<T, N>* from = reinterpret_cast<const Pack<T, N>*>(values + size_t(at[j] >= 0 ? at[j] : 0) * stride + size_t(place[q]) * N);
+              v[q][j] = WEIGHTED ? *from : streamLoad(from);
+            }
+#pragma unroll
+          for (unsigned q = 0; q < H; ++q)
+#pragma unroll
+            for (int j = 0; j < KB; ++j)
+#pragma unroll
+              for (int i = 0; i < N; ++i) sum[q][i] += at[j] >= 0 ? w[j] * R(v[q][j].v[i]) : R(0);
+        }
+#pragma unroll
+        for (unsigned q = 0; q < H; ++q) {
+          Pack<T, N> o;
+#pragma unroll
+          for (int i = 0; i < N; ++i) o.v[i] = T(sum[q][i]);
+          streamStore(&out[row * shape.pieces + place[q]], o);
+        }
       }
-      Pack<T, N> o;
-#pragma unroll
-      for (int i = 0; i < N; ++i) o.v[i] = T(sum[i]);
-      streamStore(&out[row * shape.pieces + c], o);
-    }
+    };
+    if (shape.pieces % (2u << shape.shift) == 0) join(std::integral_constant<unsigned, 2>());
+    else join(std::integral_constant<unsigned, 1>());
   });
 }
 
@@ -311,7 +336,7 @@ __global__ __launch_bounds__(BLOCK) void combineBackwardKernel(const T* __restri
   using R = wide_t<T>;
   if (blockIdx.x >= unused.rowBlocks) return clearUnused(unused);
   const unsigned group = 1u << shape.shift, lane = threadIdx.x & (group - 1);
-  forTiles(shape.tiles, unused.rowBlocks, [&](size_t tile) {
+  forTiles(shape.tiles, unused.rowBlocks, shape.byDie, [&](size_t tile) {
     const size_t row = tile * (BLOCK >> shape.shift) + (threadIdx.x >> shape.shift);
     if (row >= n) return;
     for (unsigned first = 0; first < k; first += KB) {
@@ -428,7 +453,7 @@ __device__ inline void logSum(const LogTerms<R, W, K>& terms, size_t row, R& pea
 template <typename R, typename W, int K>
 __global__ __launch_bounds__(BLOCK) void combineLogKernel(const R* __restrict__ values, size_t capacity, const int32_t* __restrict__ position,
                                                           const W* __restrict__ logWeight, size_t n, unsigned k, R* __restrict__ out) {
-  forTiles((n + BLOCK - 1) / BLOCK, gridDim.x, [&](size_t tile) {
+  forTiles((n + BLOCK - 1) / BLOCK, gridDim.x, true, [&](size_t tile) {
     const size_t row = tile * BLOCK + threadIdx.x;
     if (row >= n) return;
     LogTerms<R, W, K> terms{values, capacity, position, logWeight, k};
@@ -444,7 +469,7 @@ __global__ __launch_bounds__(BLOCK) void combineLogBackwardKernel(const R* __res
                                                                   const W* __restrict__ logWeight, size_t n, unsigned k, const R* __restrict__ gradOut,
                                                                   R* __restrict__ gradValues, W* __restrict__ gradLogWeight, Unused unused) {
   if (blockIdx.x >= unused.rowBlocks) return clearUnused(unused);
-  forTiles((n + BLOCK - 1) / BLOCK, unused.rowBlocks, [&](size_t tile) {
+  forTiles((n + BLOCK - 1) / BLOCK, unused.rowBlocks, true, [&](size_t tile) {
     const size_t row = tile * BLOCK + threadIdx.x;
     if (row >= n) return;
     LogTerms<R, W, K> terms{values, capacity, position, logWeight, k};
@@ -659,6 +684,7 @@ int spnc_hip_combine(const void* values, int dtype, size_t capacity, size_t widt
     if (width * bytes >> 32) refuse("a row must be shorter than 4 GiB");
     if (n == 0 || width == 0) return;
     if ((capacity && !values) || !position || !out) refuse("null argument");
+    if (capacity == 0) values = out, stride = width;  // no slot is routed; there has to be a row to read and drop
     const unsigned piece = pieceBytes(unsigned(bytes), {address(values), address(out), width * bytes, stride * bytes});
     checkAligned(piece, "combine");
     const RowShape shape = rowShape(n, width * bytes, piece);
