@@ -381,121 +381,191 @@ __global__ __launch_bounds__(BLOCK) void combineBackwardKernel(const T* __restri
 
 // The largest value of the row's slots is taken out before its log weight is added: values of some thousands differ by
 // little, and the difference is exact where the sum would be rounded. Shares are computed from the same terms, not from the
-// rounded result.
+// rounded result. A slot that is not routed or has log weight minus infinity is left out, whatever value stands there.
+//
+// K slots a row in registers, EXACT: k of them, positions and weights one piece each; otherwise the last ones may be missing. Bound by
+// the gather of single values: lanes next to each other hold rows of different experts, so nearly every lane is an access of its own.
+// Two rows a thread keep more of them under way.
+template <typename R, typename W, int K, bool EXACT>
+struct LogRow {
+  int32_t at[K];
+  R weight[K], term[K];  // term: the value, then exp(log weight + (value - peak) - shift)
+  R peak, shift, total;  // the largest value, the largest log weight + (value - peak), the sum of the terms
 
-// A row's slots. K > 0: held in registers, read as one piece each of positions and weights; K = 0: read again for every use.
-template <typename R, typename W, int K>
-struct LogTerms {
+  __device__ void slots(const int32_t* position, const W* logWeight, size_t row, unsigned k, size_t capacity) {
+    Pack<int32_t, K> p;
+    Pack<W, K> w;
+    if constexpr (EXACT) {
+      p = *reinterpret_cast<const Pack<int32_t, K>*>(position + row * K);
+      w = *reinterpret_cast<const Pack<W, K>*>(logWeight + row * K);
+    } else {
+#pragma unroll
+      for (int j = 0; j < K; ++j) {
+        p.v[j] = j < int(k) ? position[row * k + j] : -1;
+        w.v[j] = j < int(k) ? logWeight[row * k + j] : W(0);
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      at[j] = p.v[j] >= 0 && size_t(p.v[j]) < capacity ? p.v[j] : -1;
+      weight[j] = at[j] >= 0 ? R(w.v[j]) : R(-INFINITY);
+    }
+  }
+  __device__ void values(const R* from) {
+#pragma unroll
+    for (int j = 0; j < K; ++j) term[j] = from[at[j] >= 0 ? at[j] : 0];
+  }
+  __device__ void solve() {
+    peak = shift = -INFINITY;
+    total = 0;
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      if (weight[j] == -INFINITY) term[j] = -INFINITY;
+      peak = term[j] > peak || term[j] != term[j] ? term[j] : peak;
+    }
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      term[j] = weight[j] + (term[j] - peak);
+      shift = term[j] > shift || term[j] != term[j] ? term[j] : shift;
+    }
+#pragma unroll
+    for (int j = 0; j < K; ++j) {
+      term[j] = expOf(term[j] - shift);
+      total += term[j];
+    }
+  }
+  __device__ R result() const { return peak == -INFINITY || peak == INFINITY ? peak : peak + (shift + logOf(total)); }
+  __device__ R share(int j, R g) const { return weight[j] == -INFINITY || peak == -INFINITY ? R(0) : g * (term[j] / total); }
+};
+
+template <int K> constexpr int LOG_ROWS = K <= 2 ? 2 : 1;  // of a thread
+
+template <typename R, typename W, int K, bool EXACT>
+__global__ __launch_bounds__(BLOCK) void combineLogKernel(const R* __restrict__ values, size_t capacity, const int32_t* __restrict__ position,
+                                                          const W* __restrict__ logWeight, size_t n, unsigned k, R* __restrict__ out) {
+  constexpr int ROWS = LOG_ROWS<K>;
+  forTiles((n + ROWS * BLOCK - 1) / (ROWS * BLOCK), gridDim.x, true, [&](size_t tile) {
+    const size_t first = tile * (ROWS * BLOCK) + threadIdx.x;
+    LogRow<R, W, K, EXACT> r[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) r[i].slots(position, logWeight, first + i * BLOCK < n ? first + i * BLOCK : n - 1, k, capacity);
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) r[i].values(values);
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      r[i].solve();
+      if (first + i * BLOCK < n) out[first + i * BLOCK] = r[i].result();
+    }
+  });
+}
+
+template <typename R, typename W, int K, bool EXACT>
+__global__ __launch_bounds__(BLOCK) void combineLogBackwardKernel(const R* __restrict__ values, size_t capacity, const int32_t* __restrict__ position,
+                                                                  const W* __restrict__ logWeight, size_t n, unsigned k, const R* __restrict__ gradOut,
+                                                                  R* __restrict__ gradValues, W* __restrict__ gradLogWeight, Unused unused) {
+  if (blockIdx.x >= unused.rowBlocks) return clearUnused(unused);
+  constexpr int ROWS = LOG_ROWS<K>;
+  forTiles((n + ROWS * BLOCK - 1) / (ROWS * BLOCK), unused.rowBlocks, true, [&](size_t tile) {
+    const size_t first = tile * (ROWS * BLOCK) + threadIdx.x;
+    LogRow<R, W, K, EXACT> r[ROWS];
+    R g[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const size_t row = first + i * BLOCK < n ? first + i * BLOCK : n - 1;
+      r[i].slots(position, logWeight, row, k, capacity);
+      g[i] = gradOut[row];
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) r[i].values(values);
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+      const size_t row = first + i * BLOCK;
+      if (row >= n) continue;
+      r[i].solve();
+      Pack<W, K> o;
+#pragma unroll
+      for (int j = 0; j < K; ++j) {
+        const R share = r[i].share(j, g[i]);
+        if (gradValues && r[i].at[j] >= 0) gradValues[r[i].at[j]] = share;
+        o.v[j] = W(share);
+      }
+      if (gradLogWeight) {
+        if constexpr (EXACT) {
+          *reinterpret_cast<Pack<W, K>*>(gradLogWeight + row * K) = o;
+        } else {
+#pragma unroll
+          for (int j = 0; j < K; ++j)
+            if (j < int(k)) gradLogWeight[row * k + j] = o.v[j];
+        }
+      }
+    }
+  });
+}
+
+// Any number of slots, read again for every use.
+template <typename R, typename W>
+struct LogSlots {
   const R* values;
   size_t capacity;
   const int32_t* position;
   const W* logWeight;
   unsigned k;
-  int32_t at[K > 0 ? K : 1];
-  R value[K > 0 ? K : 1], weight[K > 0 ? K : 1];
+  R peak, shift, total;
 
-  __device__ unsigned count() const { return K > 0 ? K : k; }
-  // false: the slot is left out
-  __device__ bool read(size_t s, R& v, R& lw, int32_t& p) const {
-    p = position[s];
-    if (p >= 0 && size_t(p) >= capacity) p = -1;
-    lw = p >= 0 ? R(logWeight[s]) : R(-INFINITY);
+  __device__ bool read(size_t s, R& v, R& lw, int32_t& at) const {
+    at = position[s];
+    if (at >= 0 && size_t(at) >= capacity) at = -1;
+    lw = at >= 0 ? R(logWeight[s]) : R(-INFINITY);
     if (lw == -INFINITY) return false;
-    v = values[p];
+    v = values[at];
     return true;
   }
-  __device__ void load(size_t row) {
-    if constexpr (K > 0) {
-      const Pack<int32_t, K> p = *reinterpret_cast<const Pack<int32_t, K>*>(position + row * K);
-      const Pack<W, K> w = *reinterpret_cast<const Pack<W, K>*>(logWeight + row * K);
-#pragma unroll
-      for (int j = 0; j < K; ++j) {
-        at[j] = p.v[j] >= 0 && size_t(p.v[j]) < capacity ? p.v[j] : -1;
-        weight[j] = at[j] >= 0 ? R(w.v[j]) : R(-INFINITY);
-        value[j] = capacity ? values[at[j] >= 0 ? at[j] : 0] : R(0);
+  __device__ void solve(size_t row) {
+    peak = shift = -INFINITY;
+    total = 0;
+    R v, lw;
+    int32_t at;
+    for (unsigned j = 0; j < k; ++j)
+      if (read(row * k + j, v, lw, at)) peak = v > peak || v != v ? v : peak;
+    if (peak == -INFINITY) return;  // nothing possible
+    for (unsigned j = 0; j < k; ++j)
+      if (read(row * k + j, v, lw, at)) {
+        const R t = lw + (v - peak);
+        shift = t > shift || t != t ? t : shift;
       }
-    }
-  }
-  __device__ bool slot(size_t row, unsigned j, R& v, R& lw) const {
-    if constexpr (K > 0) {
-      v = value[j];
-      lw = weight[j];
-      return lw != -INFINITY;
-    } else {
-      int32_t p;
-      return read(row * k + j, v, lw, p);
-    }
+    for (unsigned j = 0; j < k; ++j)
+      if (read(row * k + j, v, lw, at)) total += expOf(lw + (v - peak) - shift);
   }
 };
 
-// peak: the largest value; shift: the largest log weight + (value - peak); total: sum of exp(that - shift)
-template <typename R, typename W, int K>
-__device__ inline void logSum(const LogTerms<R, W, K>& terms, size_t row, R& peak, R& shift, R& total) {
-  peak = -INFINITY;
-  R v, lw;
-#pragma unroll
-  for (unsigned j = 0; j < terms.count(); ++j)
-    if (terms.slot(row, j, v, lw)) peak = v > peak || v != v ? v : peak;
-  shift = -INFINITY;
-  total = 0;
-  if (peak == -INFINITY) return;  // nothing possible
-#pragma unroll
-  for (unsigned j = 0; j < terms.count(); ++j)
-    if (terms.slot(row, j, v, lw)) {
-      const R t = lw + (v - peak);
-      shift = t > shift || t != t ? t : shift;
-    }
-#pragma unroll
-  for (unsigned j = 0; j < terms.count(); ++j)
-    if (terms.slot(row, j, v, lw)) total += expOf(lw + (v - peak) - shift);
-}
-
-template <typename R, typename W, int K>
-__global__ __launch_bounds__(BLOCK) void combineLogKernel(const R* __restrict__ values, size_t capacity, const int32_t* __restrict__ position,
-                                                          const W* __restrict__ logWeight, size_t n, unsigned k, R* __restrict__ out) {
+template <typename R, typename W>
+__global__ __launch_bounds__(BLOCK) void combineLogManyKernel(LogSlots<R, W> given, size_t n, R* __restrict__ out) {
   forTiles((n + BLOCK - 1) / BLOCK, gridDim.x, true, [&](size_t tile) {
     const size_t row = tile * BLOCK + threadIdx.x;
     if (row >= n) return;
-    LogTerms<R, W, K> terms{values, capacity, position, logWeight, k};
-    terms.load(row);
-    R peak, shift, total;
-    logSum(terms, row, peak, shift, total);
-    out[row] = peak == -INFINITY || peak == INFINITY ? peak : peak + (shift + logOf(total));
+    LogSlots<R, W> r = given;
+    r.solve(row);
+    out[row] = r.peak == -INFINITY || r.peak == INFINITY ? r.peak : r.peak + (r.shift + logOf(r.total));
   });
 }
 
-template <typename R, typename W, int K>
-__global__ __launch_bounds__(BLOCK) void combineLogBackwardKernel(const R* __restrict__ values, size_t capacity, const int32_t* __restrict__ position,
-                                                                  const W* __restrict__ logWeight, size_t n, unsigned k, const R* __restrict__ gradOut,
-                                                                  R* __restrict__ gradValues, W* __restrict__ gradLogWeight, Unused unused) {
+template <typename R, typename W>
+__global__ __launch_bounds__(BLOCK) void combineLogManyBackwardKernel(LogSlots<R, W> given, size_t n, const R* __restrict__ gradOut,
+                                                                      R* __restrict__ gradValues, W* __restrict__ gradLogWeight, Unused unused) {
   if (blockIdx.x >= unused.rowBlocks) return clearUnused(unused);
   forTiles((n + BLOCK - 1) / BLOCK, unused.rowBlocks, true, [&](size_t tile) {
     const size_t row = tile * BLOCK + threadIdx.x;
     if (row >= n) return;
-    LogTerms<R, W, K> terms{values, capacity, position, logWeight, k};
-    terms.load(row);
-    R peak, shift, total;
-    logSum(terms, row, peak, shift, total);
+    LogSlots<R, W> r = given;
+    r.solve(row);
     const R g = gradOut[row];
-    if constexpr (K > 0) {
-      Pack<W, K> o;
-#pragma unroll
-      for (int j = 0; j < K; ++j) {
-        R v, lw, share = 0;
-        if (peak != -INFINITY && terms.slot(row, j, v, lw)) share = g * (expOf(lw + (v - peak) - shift) / total);
-        if (gradValues && terms.at[j] >= 0) gradValues[terms.at[j]] = share;
-        o.v[j] = W(share);
-      }
-      if (gradLogWeight) *reinterpret_cast<Pack<W, K>*>(gradLogWeight + row * K) = o;
-    } else {
-      for (unsigned j = 0; j < k; ++j) {
-        const size_t s = row * k + j;
-        R v, lw, share = 0;
-        int32_t p;
-        if (terms.read(s, v, lw, p) && peak != -INFINITY) share = g * (expOf(lw + (v - peak) - shift) / total);
-        if (gradValues && p >= 0) gradValues[p] = share;
-        if (gradLogWeight) gradLogWeight[s] = W(share);
-      }
+    for (unsigned j = 0; j < r.k; ++j) {
+      const size_t s = row * r.k + j;
+      R v, lw, share = 0;
+      int32_t at;
+      if (r.read(s, v, lw, at) && r.peak != -INFINITY) share = g * (expOf(lw + (v - r.peak) - r.shift) / r.total);
+      if (gradValues && at >= 0) gradValues[at] = share;
+      if (gradLogWeight) gradLogWeight[s] = W(share);
     }
   });
 }
@@ -580,15 +650,23 @@ void checkSegments(const int32_t* starts, const int32_t* counts, unsigned expert
   if (!starts || !counts) refuse("null argument");
 }
 
-// calls fn(K): K slots a row read as one piece each of positions and weights, or 0 for any number and alignment
+// calls fn(K, EXACT), see LogRow; K = 0 for more than eight
 template <typename W, typename Fn>
 void withLogChoices(unsigned k, const void* position, const void* weight, const void* gradWeight, Fn&& fn) {
-  const uintptr_t bits = address(position) | address(weight) | address(gradWeight);
-  if (k == 1) return fn(std::integral_constant<int, 1>());
-  if (k == 2 && bits % (2 * sizeof(W)) == 0) return fn(std::integral_constant<int, 2>());
-  if (k == 4 && bits % 16 == 0) return fn(std::integral_constant<int, 4>());
-  if (k == 8 && bits % 16 == 0) return fn(std::integral_constant<int, 8>());
-  fn(std::integral_constant<int, 0>());
+  const size_t piece = k * sizeof(W) < 16 ? k * sizeof(W) : 16;
+  const bool exact = (k & (k - 1)) == 0 && (address(position) | address(weight) | address(gradWeight)) % piece == 0;
+  auto choose = [&](auto kb) { exact ? fn(kb, std::true_type()) : fn(kb, std::false_type()); };
+  if (k == 1) return fn(std::integral_constant<int, 1>(), std::true_type());
+  if (k == 2) return choose(std::integral_constant<int, 2>());
+  if (k <= 4) return choose(std::integral_constant<int, 4>());
+  if (k <= 8) return choose(std::integral_constant<int, 8>());
+  fn(std::integral_constant<int, 0>(), std::false_type());
+}
+
+// the blocks of the kernel that withLogChoices picks
+inline unsigned logGrid(size_t n, unsigned k) {
+  const size_t rows = BLOCK * (k <= 2 ? LOG_ROWS<2> : 1);
+  return tileGrid((n + rows - 1) / rows);
 }
 
 void checkLogTypes(int dtype, int weightDtype) {
@@ -754,12 +832,18 @@ int spnc_hip_combine_log(const void* values, int dtype, size_t capacity, const i
     checkSlots(n, k, capacity);
     if (n == 0) return;
     if ((capacity && !values) || !position || !log_weight || !out) refuse("null argument");
+    if (capacity == 0) values = out;  // no slot is routed; there has to be a value to read and drop
     withLogTypes(dtype, weight_dtype, [&](auto r, auto w) {
       using R = decltype(r);
       using W = decltype(w);
-      withLogChoices<W>(k, position, log_weight, nullptr, [&](auto kb) {
-        combineLogKernel<R, W, decltype(kb)::value><<<tileGrid((n + BLOCK - 1) / BLOCK), BLOCK, 0, static_cast<hipStream_t>(stream)>>>(
-            static_cast<const R*>(values), capacity, position, static_cast<const W*>(log_weight), n, k, static_cast<R*>(out));
+      withLogChoices<W>(k, position, log_weight, nullptr, [&](auto kb, auto exact) {
+        constexpr int K = decltype(kb)::value;
+        if constexpr (K > 0)
+          combineLogKernel<R, W, K, decltype(exact)::value><<<logGrid(n, k), BLOCK, 0, static_cast<hipStream_t>(stream)>>>(
+              static_cast<const R*>(values), capacity, position, static_cast<const W*>(log_weight), n, k, static_cast<R*>(out));
+        else
+          combineLogManyKernel<R, W><<<logGrid(n, k), BLOCK, 0, static_cast<hipStream_t>(stream)>>>(
+              LogSlots<R, W>{static_cast<const R*>(values), capacity, position, static_cast<const W*>(log_weight), k}, n, static_cast<R*>(out));
       });
     });
     launched("combine_log");
@@ -776,16 +860,23 @@ int spnc_hip_combine_log_backward(const void* values, int dtype, size_t capacity
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (!grad_values && !grad_log_weight) return;
     if (n && ((capacity && !values) || !position || !log_weight || !grad_out)) refuse("null argument");
+    if (capacity == 0) values = grad_out;
     const Unused unused =
-        unusedRows(tileGrid((n + BLOCK - 1) / BLOCK), starts, counts, experts, capacity, elementBytes(dtype), grad_values);
+        unusedRows(logGrid(n, k), starts, counts, experts, capacity, elementBytes(dtype), grad_values);
     if (unused.rowBlocks + unused.blocks == 0) return;
     withLogTypes(dtype, weight_dtype, [&](auto r, auto w) {
       using R = decltype(r);
       using W = decltype(w);
-      withLogChoices<W>(k, position, log_weight, grad_log_weight, [&](auto kb) {
-        combineLogBackwardKernel<R, W, decltype(kb)::value><<<unused.rowBlocks + unused.blocks, BLOCK, 0, s>>>(
-            static_cast<const R*>(values), capacity, position, static_cast<const W*>(log_weight), n, k, static_cast<const R*>(grad_out),
-            static_cast<R*>(grad_values), static_cast<W*>(grad_log_weight), unused);
+      withLogChoices<W>(k, position, log_weight, grad_log_weight, [&](auto kb, auto exact) {
+        constexpr int K = decltype(kb)::value;
+        if constexpr (K > 0)
+          combineLogBackwardKernel<R, W, K, decltype(exact)::value><<<unused.rowBlocks + unused.blocks, BLOCK, 0, s>>>(
+              static_cast<const R*>(values), capacity, position, static_cast<const W*>(log_weight), n, k, static_cast<const R*>(grad_out),
+              static_cast<R*>(grad_values), static_cast<W*>(grad_log_weight), unused);
+        else
+          combineLogManyBackwardKernel<R, W><<<unused.rowBlocks + unused.blocks, BLOCK, 0, s>>>(
+              LogSlots<R, W>{static_cast<const R*>(values), capacity, position, static_cast<const W*>(log_weight), k}, n,
+              static_cast<const R*>(grad_out), static_cast<R*>(grad_values), static_cast<W*>(grad_log_weight), unused);
       });
     });
     launched("combine_log gradient");
