@@ -22,54 +22,43 @@ struct Dropout {
   }
 };
 
-template <typename T> constexpr int DROPOUT_UNIT = sizeof(T) == 2 ? 8 : 4;  // elements of 16 bytes, at least the four of one counter
-constexpr unsigned DROPOUT_UNITS = 2;                                       // of a thread
+template <typename T> constexpr int DROPOUT_UNIT = sizeof(T) == 2 ? 8 : 4;  // elements of a thread: 16 bytes, at least the four of one counter
 
-// Contiguous elements; VEC: read and written 16 bytes at a time. For 16-bit types bound by the generator: eighteen 32-bit products at a
-// quarter of the rate for four elements. 33 M bfloat16 take xx us (31 with two exclusive ors an instruction each and the
-// counter's upper half a lane's own), 64 M float32 94 us or 5.7 TB/s, which is what a copy of that size reaches. Results stay on the ordinary way through the
-// caches: past them the kernel takes 90 us, but what reads them next is 6 us slower than that saves.
+// Contiguous elements; VEC: read and written 16 bytes at a time. One unit a thread: 4 M x 16 float32 take 88 us or 6.1 TB/s (95 with two,
+// 98 with four), which is what a copy of that size reaches. For 16-bit types the generator counts, eighteen 32-bit products at a quarter of
+// the rate for four elements: 33 M bfloat16 take 27 us, 23 without it (31 with two exclusive ors an instruction each and a counter
+// whose upper half is a lane's own). Results stay on the ordinary way through the caches: past them the kernel alone is a
+// few us faster, but what reads them next loses more than that.
 template <typename T, bool VEC>
 __global__ __launch_bounds__(BLOCK) void dropoutFlatKernel(const T* x, size_t elements, T* out, Dropout<wide_t<T>> d) {
-  constexpr int E = DROPOUT_UNIT<T>;
-  constexpr uint32_t COUNTERS = DROPOUT_UNITS * BLOCK * (E / 4);  // of a tile
+  constexpr uint32_t E = DROPOUT_UNIT<T>, TILE = BLOCK * E;  // elements; TILE / 4 divides 2^32, so a tile's counters have one upper half
   using P = Pack<T, E>;
   const uint64_t at = d.offsetDevice ? *d.offsetDevice : d.offset;
-  const size_t units = (elements + E - 1) / E, tiles = (units + DROPOUT_UNITS * BLOCK - 1) / (DROPOUT_UNITS * BLOCK);
+  const size_t tiles = (elements + TILE - 1) / TILE;
   for (size_t tile = blockIdx.x; tile < tiles; tile += gridDim.x) {
-    const T* const from = x + tile * COUNTERS * 4;
-    T* const to = out + tile * COUNTERS * 4;
-    const size_t left = elements - tile * COUNTERS * 4;
-    const uint32_t here = left < COUNTERS * 4 ? uint32_t(left) : COUNTERS * 4;  // elements of this tile
-    P v[DROPOUT_UNITS];
+    const T* const from = x + tile * TILE;
+    T* const to = out + tile * TILE;
+    const size_t left = elements - tile * TILE;
+    const uint32_t here = left < TILE ? uint32_t(left) : TILE, e = threadIdx.x * E;
+    if (e >= here) continue;
+    P v;
+    if (VEC && e + E <= here) v = *reinterpret_cast<const P*>(from + e);
+    else
 #pragma unroll
-    for (unsigned i = 0; i < DROPOUT_UNITS; ++i) {
-      const uint32_t e = (threadIdx.x + i * BLOCK) * E;
-      if (VEC && e + E <= here) v[i] = *reinterpret_cast<const P*>(from + e);
-      else
+      for (uint32_t q = 0; q < E; ++q)
+        if (e + q < here) v.v[q] = from[e + q];
+    const uint64_t counter = uint64_t(tile) * (TILE / 4);
 #pragma unroll
-        for (int q = 0; q < E; ++q)
-          if (e + q < here) v[i].v[q] = from[e + q];
+    for (uint32_t b = 0; b < E / 4; ++b) {
+      const Philox4 r = d.words(uint32_t(counter) + e / 4 + b, uint32_t(counter >> 32), at);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) v.v[4 * b + q] = d.apply(r.w[q], v.v[4 * b + q]);
     }
-    // COUNTERS divides 2^32: the upper half is the same for the tile
-    const uint64_t counter = uint64_t(tile) * COUNTERS;
-    const uint32_t high = uint32_t(counter >> 32);
+    if (VEC && e + E <= here) *reinterpret_cast<P*>(to + e) = v;
+    else
 #pragma unroll
-    for (unsigned i = 0; i < DROPOUT_UNITS; ++i) {
-      const uint32_t e = (threadIdx.x + i * BLOCK) * E;
-      if (e >= here) continue;
-#pragma unroll
-      for (int b = 0; b < E / 4; ++b) {
-        const Philox4 r = d.words(uint32_t(counter) + e / 4 + b, high, at);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) v[i].v[4 * b + q] = d.apply(r.w[q], v[i].v[4 * b + q]);
-      }
-      if (VEC && e + E <= here) *reinterpret_cast<P*>(to + e) = v[i];
-      else
-#pragma unroll
-        for (int q = 0; q < E; ++q)
-          if (e + q < here) to[e + q] = v[i].v[q];
-    }
+      for (uint32_t q = 0; q < E; ++q)
+        if (e + q < here) to[e + q] = v.v[q];
   }
 }
 
@@ -131,7 +120,7 @@ int spnc_hip_dropout(const void* x, int dtype, size_t n, size_t width, size_t st
       const uintptr_t bits = address(x) | address(out);
       if (n == 1 || (stride == width && out_stride == width)) {
         constexpr int E = DROPOUT_UNIT<T>;
-        const size_t elements = n * width, units = (elements + E - 1) / E, blocks = (units + DROPOUT_UNITS * BLOCK - 1) / (DROPOUT_UNITS * BLOCK);
+        const size_t elements = n * width, blocks = (elements + BLOCK * E - 1) / (BLOCK * E);
         const unsigned grid = unsigned(blocks < MAX_GRID ? blocks : MAX_GRID);
         if (bits % (sizeof(Pack<T, E>) < 16 ? sizeof(Pack<T, E>) : 16) == 0)
           dropoutFlatKernel<T, true><<<grid, BLOCK, 0, s>>>(static_cast<const T*>(x), elements, static_cast<T*>(out), d);

@@ -63,7 +63,7 @@ def gate(logits, k, *, over="chosen", log=False):
 class Plan:
     """Where every slot (row i, choice j) stands in the buffer sorted by expert.
 
-    position : int32 [n, k], the slot's row of the sorted buffer, -1 where it is not routed.
+    position : int32 [n, k], the slot's row of the sorted buffer, -1 where it is not routed; a row of the buffer belongs to one slot.
     starts   : int32 [experts + 1], first row of every expert's segment; the last entry is where the last segment ends.
     counts   : int32 [experts], rows of every segment.
     capacity : rows of the sorted buffer.

@@ -442,6 +442,56 @@ def test_combine_of_views_and_one_gradient(native):
     alone, = torch.autograd.grad(m.combine(base, plan, w).sum(), w)                                                # the weights' alone
     assert torch.equal(alone, torch.autograd.grad(m.combine(both, plan, w).sum(), (both, w))[1])
     assert m.combine(base[:, :0], plan, weights).shape == (50, 0)
+    one = torch.rand(50, 1, device="cuda").requires_grad_()                                                        # a weight for all slots of a row
+    shared, = torch.autograd.grad(m.combine(base, plan, one.expand(50, 2)).sum(), one)
+    w = one.detach().expand(50, 2).contiguous().requires_grad_()
+    assert torch.equal(shared, torch.autograd.grad(m.combine(base, plan, w).sum(), w)[0].sum(dim=1, keepdim=True))
+
+
+@pytest.mark.gpu
+def test_plans_without_rows(native):
+    """A buffer of no rows: everything that comes back is empty sums, nothing is read."""
+    torch = _torch()
+    from spnc import mixture as m
+    i32 = dict(dtype=torch.int32, device="cuda")
+    for n in (0, 5):
+        plan = m.Plan(torch.full((n, 2), 3, **i32), torch.zeros(4, **i32), torch.zeros(3, **i32), 0)     # positions behind the buffer: not routed
+        w = torch.rand(n, 2, device="cuda", requires_grad=True)
+        rows = torch.empty(0, 6, device="cuda", requires_grad=True)
+        y = m.combine(rows, plan, w)
+        assert y.shape == (n, 6) and bool((y == 0).all())
+        gr, gw = torch.autograd.grad(y, (rows, w), torch.ones_like(y))
+        assert gr.shape == (0, 6) and bool((gw == 0).all()) and gw.shape == (n, 2)
+        v = torch.empty(0, device="cuda", requires_grad=True)
+        z = m.combine_log(v, plan, w)
+        assert z.shape == (n,) and bool((z == -float("inf")).all())
+        gv, gw = torch.autograd.grad(z, (v, w), torch.ones_like(z))
+        assert gv.shape == (0,) and bool((gw == 0).all())
+        assert m.dispatch(torch.rand(n, 6, device="cuda"), plan).shape == (0, 6)
+
+
+@pytest.mark.gpu
+def test_captured_small_calls(native):
+    """The serving form of each operator, captured and replayed with new data; a thousand experts need more LDS than a kernel has unasked."""
+    torch = _torch()
+    from spnc import mixture as m
+    z, x, v = torch.randn(3, 1000, device="cuda"), torch.randn(3, 40, device="cuda").bfloat16(), torch.randn(6, device="cuda")
+
+    def step():
+        index, w = m.gate(z, 2, log=True)
+        plan = m.route(index, 1000)
+        return index, plan.position, m.dispatch(x, plan), m.combine(m.dispatch(x, plan), plan, w.exp()), m.combine_log(v, plan, w), m.dropout(x, 0.5, 3)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for _ in range(3):
+        z.normal_(), x.normal_(), v.normal_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(captured, step()))
 
 
 LOG = [(1, 1, 2, 1), (1, 2, 10, 1), (77, 3, 5, 4), (1031, 2, 16, 1), (300, 8, 9, 1), (130, 11, 6, 2), (70, 64, 100, 1)]
