@@ -154,8 +154,10 @@ __device__ inline void gateInsert(uint32_t (&list)[4], uint32_t key) {
   list[0] = key > list[0] ? key : list[0];
 }
 
-// G lanes hold a row, V logits each. k rounds: the largest key of the group, the lowest expert that has it, and out it goes; lane
-// j keeps the choice of round j. The whole row is in registers, so the logits are read once.
+// G lanes hold a row, V logits each, so the logits are read once. k rounds: the largest key of the group, the lowest expert that has it, and
+// out it goes; lane j keeps the choice of round j, and the softmax is computed by the lanes that have one. Bound by instructions: 262144
+// rows of 64 float32, four choices, take 18 us (76 MB, 4.3 TB/s), 65537 of 509 bfloat16, eight choices over all, 26 us (71 MB; 800
+// vector instructions a wave of four rows are 21 us of issue).
 template <typename T, int G, int V, int LAYOUT>
 __global__ __launch_bounds__(BLOCK) void gateKernel(const T* __restrict__ logits, size_t n, unsigned experts, size_t stride, unsigned k,
                                                     unsigned flags, int32_t* __restrict__ index, wide_t<T>* __restrict__ weight) {

@@ -230,6 +230,9 @@ __device__ inline void loadWeights(const W* weight, size_t row, unsigned k, unsi
   for (int j = 0; j < KB; ++j) w[j] = !weight ? R(1) : first + j < k ? R(weight[row * k + first + j]) : R(0);
 }
 
+// out[position_ij] = x_i: a row is read once and written to all its places. Bound by the writes: 1 M rows of 64 bytes to two places
+// take 36 us, 5.6 TB/s; 32769 rows of 2 KB to four, 52 us, 6.3 TB/s. Rows that share cache lines with rows of other blocks cost more: of 24
+// bytes, 2 M to two places 31 us, 4.9 TB/s, to four of 64 experts' places 98 us, 2.6 TB/s.
 template <typename P, int KB, bool STREAM>
 __global__ __launch_bounds__(BLOCK) void dispatchKernel(const unsigned char* __restrict__ rows, size_t n, size_t strideBytes, RowShape shape,
                                                         const int32_t* __restrict__ position, unsigned k, size_t capacity, P* __restrict__ out,
@@ -269,11 +272,11 @@ __global__ __launch_bounds__(BLOCK) void dispatchKernel(const unsigned char* __r
   });
 }
 
-// Slots are read KB at a time, all loads before the first product; a slot that is not routed reads row 0 and drops it. Results
-// bypass the caches, which leaves the values there for the backward pass (32769 x 4 rows of 2 KB, forward and backward: 164 us
-// instead of 191), and so do values without weights: gradients of dispatch, whose last use this is (139 instead of 150 us for the
-// whole of routing, dispatch and its gradient at that size). Two pieces a lane at a time, where a row has them for all
-// lanes: 59 us instead of 69.
+// out[i] = sum_j w_ij v[position_ij] in the order of j. Bound by memory: 32769 rows of four slots of 2 KB take 59 us, 5.5 TB/s. Slots
+// are read KB at a time, all loads before the first product (a slot that is not routed reads row 0 and drops it), and two pieces a
+// lane at a time where a row has them for all lanes, which is 10 us of these. Results go past the caches, which leaves the
+// values there for the backward pass (both together are 27 us shorter at that size), and so do values without weights: gradients of
+// dispatch, whose last use this is (54 us; 11 us of routing, dispatch and gradient together).
 template <typename T, int N, typename W, int KB, bool ONE, bool WEIGHTED>
 __global__ __launch_bounds__(BLOCK) void combineKernel(const T* __restrict__ values, size_t capacity, size_t stride, RowShape shape,
                                                        const int32_t* __restrict__ position, size_t n, unsigned k, const W* __restrict__ weight,
@@ -328,6 +331,8 @@ __global__ __launch_bounds__(BLOCK) void combineKernel(const T* __restrict__ val
   });
 }
 
+// dv[position_ij] = w_ij g_i and dw_ij = <g_i, v[position_ij]> in one pass over the values. Bound by memory: 32769 rows of four slots
+// of 2 KB take 94 us, 6.3 TB/s; the gradient of the output is read past the caches, where it has no further use (8 us).
 template <typename T, int N, typename W, int KB, bool STREAM>
 __global__ __launch_bounds__(BLOCK) void combineBackwardKernel(const T* __restrict__ values, size_t capacity, size_t stride, RowShape shape,
                                                                const int32_t* __restrict__ position, size_t n, unsigned k,
@@ -385,7 +390,8 @@ __global__ __launch_bounds__(BLOCK) void combineBackwardKernel(const T* __restri
 //
 // K slots a row in registers, EXACT: k of them, positions and weights one piece each; otherwise the last ones may be missing. Bound by
 // the gather of single values: lanes next to each other hold rows of different experts, so nearly every lane is an access of its own.
-// Two rows a thread keep more of them under way.
+// Two rows a thread keep more of them under way. 4 M rows of two slots take 26 us, 4.5 TB/s, their gradient 41 us, 4.5 TB/s: the
+// address units, which take a lane a cycle here, are busy for three quarters of that.
 template <typename R, typename W, int K, bool EXACT>
 struct LogRow {
   int32_t at[K];
