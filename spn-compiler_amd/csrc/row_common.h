@@ -163,6 +163,11 @@ __device__ inline float expOf(float x) {
   return __builtin_fmaf(y, r * 0.693147182f, y);
 }
 __device__ inline double expOf(double x) { return exp(x); }
+// Without the second part: x log2(e) is rounded, an error of |x| 2^-24 relative to the result, which is that of a difference x
+// already. For terms of a sum, where it is weighted with exp(x), and for results of 16 bits. The difference is taken first: a logit of
+// the type's lowest value, times log2(e), would be infinite.
+__device__ inline float expTerm(float x) { return __builtin_amdgcn_exp2f(x * 1.44269502f); }
+__device__ inline double expTerm(double x) { return exp(x); }
 __device__ inline float logOf(float x) { return logf(x); }
 __device__ inline double logOf(double x) { return log(x); }
 

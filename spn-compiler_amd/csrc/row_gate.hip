@@ -128,23 +128,6 @@ __device__ inline void gateLoad(GateRows rows, const T* row, unsigned at, int ex
     }
 }
 
-// exp(z - top) for many z as 2^(z log2(e) - top log2(e)): one fused multiply-add and the hardware's exp2. The exponent is rounded
-// once, an error of |z - top| 2^-24 relative to the term. `off` is by how much the rounded top log2(e) is too small: the terms are
-// too large by a factor of 2^off, all alike, and a sum that has to be right by itself is multiplied by 2^-off.
-struct TermsFloat {
-  float shift, off;
-  __device__ explicit TermsFloat(float top) : shift(top * 1.44269502f), off(__builtin_fmaf(top, 1.44269502f, -(top * 1.44269502f))) {}
-  __device__ float term(float z) const { return __builtin_amdgcn_exp2f(__builtin_fmaf(z, 1.44269502f, -shift)); }
-  __device__ float sum(float total) const { return total * __builtin_amdgcn_exp2f(-off); }
-};
-struct TermsDouble {
-  double top;
-  __device__ explicit TermsDouble(double t) : top(t) {}
-  __device__ double term(double z) const { return exp(z - top); }
-  __device__ double sum(double total) const { return total; }
-};
-template <typename R> using Terms = typename std::conditional<std::is_same<R, double>::value, TermsDouble, TermsFloat>::type;
-
 // The largest keys of a lane in descending order, 0 where there are none.
 template <int DEPTH>
 __device__ inline void gateInsert(uint32_t (&list)[4], uint32_t key) {
@@ -229,10 +212,10 @@ __global__ __launch_bounds__(BLOCK) void gateKernel(const T* __restrict__ logits
       if (j == 0) {
         topKey = best;
         if ((flags & SPNC_HIP_GATE_ALL) && O::open(best)) {
-          const Terms<R> terms(O::value(best));
+          const R top = O::value(best);
 #pragma unroll
-          for (int i = 0; i < V; ++i) total += terms.term(z[i]);
-          total = terms.sum(groupSum<G>(total));
+          for (int i = 0; i < V; ++i) total += expTerm(z[i] - top);
+          total = groupSum<G>(total);
         }
       }
       if (lane == j) myKey = best, myIndex = at;
@@ -290,11 +273,10 @@ __global__ __launch_bounds__(BLOCK) void gateBackwardKernel(const T* __restrict_
         const GateRows buffer = gateRows(logits + tile * ROWS * stride, (n - 1 - tile * ROWS) * stride + experts, gateStep(LAYOUT) * sizeof(T));
         gateLoad<T, G, V, LAYOUT>(buffer, from, unsigned(local) * unsigned(stride), experts, lane, odd, row == n - 1, z);
         const R top = any ? R(from[first]) : R(0);
-        const Terms<R> terms(top);
         R total = 0;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-          z[i] = sizeof(T) == 4 ? expOf(z[i] - top) : terms.term(z[i]);
+          z[i] = sizeof(T) == 2 ? expTerm(z[i] - top) : expOf(z[i] - top);
           total += z[i];
         }
         total = groupSum<G>(total);

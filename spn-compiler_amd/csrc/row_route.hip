@@ -190,15 +190,17 @@ __device__ inline void clearUnused(const Unused& u) {
   const unsigned lane = threadIdx.x % WAVE;
   const size_t wave = size_t(blockIdx.x - u.rowBlocks) * (BLOCK / WAVE) + threadIdx.x / WAVE, waves = size_t(u.blocks) * (BLOCK / WAVE);
   auto clear = [&](size_t from, size_t to, size_t first, size_t step) {  // bytes; pointers may have any alignment
-    if (((reinterpret_cast<uintptr_t>(u.out) | from | to) & 15) == 0) {
-      Pack<uint32_t, 4>* words = reinterpret_cast<Pack<uint32_t, 4>*>(u.out);
-      for (size_t i = from / 16 + first; i < to / 16; i += step) words[i] = Pack<uint32_t, 4>{};
-    } else if (((reinterpret_cast<uintptr_t>(u.out) | from | to) & 3) == 0) {
-      uint32_t* words = reinterpret_cast<uint32_t*>(u.out);
-      for (size_t i = from / 4 + first; i < to / 4; i += step) words[i] = 0;
-    } else {
-      for (size_t i = from + first; i < to; i += step) u.out[i] = 0;
+    unsigned char *const begin = u.out + from, *const end = u.out + to;
+    const uintptr_t low = (reinterpret_cast<uintptr_t>(begin) + 15) & ~uintptr_t(15), high = reinterpret_cast<uintptr_t>(end) & ~uintptr_t(15);
+    if (low >= high) {
+      for (size_t i = first; i < to - from; i += step) begin[i] = 0;
+      return;
     }
+    Pack<uint32_t, 4>* const pieces = reinterpret_cast<Pack<uint32_t, 4>*>(low);
+    for (size_t i = first; i < (high - low) / 16; i += step) pieces[i] = Pack<uint32_t, 4>{};
+    unsigned char* const tail = reinterpret_cast<unsigned char*>(high);
+    if (first < low - reinterpret_cast<uintptr_t>(begin)) begin[first] = 0;  // fewer than 16 bytes, of which there are as many lanes
+    if (first < reinterpret_cast<uintptr_t>(end) - high) tail[first] = 0;
   };
   for (size_t e = wave; e < u.experts; e += waves) {
     size_t from = size_t(u.starts[e]) + size_t(u.counts[e]), to = size_t(u.starts[e + 1]);
@@ -736,7 +738,7 @@ int spnc_hip_dispatch(const void* rows, size_t n, size_t row_bytes, size_t strid
                       const int32_t* starts, const int32_t* counts, unsigned experts, int zero_unused, void* out, void* stream) {
   return guarded([&] {
     checkSlots(n, k, capacity);
-    if (row_bytes >> 32) refuse("a row must be shorter than 4 GiB");
+    if (row_bytes >> 31) refuse("a row must be shorter than 2 GiB");
     if (zero_unused) checkSegments(starts, counts, experts);
     if (capacity == 0 || row_bytes == 0) return;
     if (!out || (n && (!rows || !position))) refuse("null argument");
@@ -765,7 +767,7 @@ int spnc_hip_combine(const void* values, int dtype, size_t capacity, size_t widt
     const size_t bytes = elementBytes(dtype);
     checkSlots(n, k, capacity);
     if (weight) checkWeightType(dtype, weight_dtype);
-    if (width * bytes >> 32) refuse("a row must be shorter than 4 GiB");
+    if (width >> 31 || width * bytes >> 31) refuse("a row must be shorter than 2 GiB");
     if (n == 0 || width == 0) return;
     if ((capacity && !values) || !position || !out) refuse("null argument");
     if (capacity == 0) values = out, stride = width;  // no slot is routed; there has to be a row to read and drop
@@ -800,7 +802,7 @@ int spnc_hip_combine_backward(const void* values, int dtype, size_t capacity, si
     const size_t bytes = elementBytes(dtype);
     checkSlots(n, k, capacity);
     checkWeightType(dtype, weight_dtype);
-    if (width * bytes >> 32) refuse("a row must be shorter than 4 GiB");
+    if (width >> 31 || width * bytes >> 31) refuse("a row must be shorter than 2 GiB");
     if (grad_values) checkSegments(starts, counts, experts);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (!grad_values && !grad_weight) return;

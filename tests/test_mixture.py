@@ -129,7 +129,8 @@ def test_c_entry_points_refuse(native):
     refused(lib.spnc_hip_dispatch(p, 2, 4, 4, p, 0, 4, None, None, 0, 0, p, None), "k must be")
     refused(lib.spnc_hip_dispatch(p, big, 4, 4, p, 2, 4, None, None, 0, 0, p, None), "too many slots")
     refused(lib.spnc_hip_dispatch(p, 2, 4, 4, p, 2, 4, None, None, 3, 1, p, None), "null argument")
-    refused(lib.spnc_hip_dispatch(p, 2, 1 << 32, 1 << 32, p, 2, 4, None, None, 0, 0, p, None), "4 GiB")
+    refused(lib.spnc_hip_dispatch(p, 2, 1 << 31, 1 << 31, p, 2, 4, None, None, 0, 0, p, None), "2 GiB")
+    refused(lib.spnc_hip_combine(p, 0, 4, 1 << 62, 1 << 62, p, 2, 2, p, 0, p, None), "2 GiB")
     refused(lib.spnc_hip_combine(p, 0, big, 4, 4, p, 2, 2, p, 0, p, None), "too many rows")
     refused(lib.spnc_hip_combine(p, 0, 4, 4, 4, p, 2, 2, p, 1, p, None), "weights must be float32")
     refused(lib.spnc_hip_combine(ctypes.c_void_p(18), 0, 4, 4, 4, p, 2, 2, p, 0, p, None), "not aligned")
@@ -254,6 +255,41 @@ def test_gate_of_many_rows(native, dtype, experts, k):
         _near(weight, want, (24 + experts) * u * (np.maximum(1.0, np.abs(np.where(np.isfinite(want), want, 0))) if log else np.maximum(np.abs(want), 1e-30)))
         scale = np.abs(_host(grad)).sum(axis=1, keepdims=True)
         _near(got, want_grad, (24 + experts + 2 * k) * u * scale + HALF[dtype] * np.abs(want_grad) + (2.0 ** -25 if dtype == "float16" else 0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "float64", "float16", "bfloat16"])
+def test_gate_of_the_types_limits(native, dtype):
+    """Masks of the type's lowest value, whole rows of it among them, and its largest: finite logits like others. Weights of 1, 1/2,
+    1/7 and 0 within the rounding of one quotient and of exp and a sum of seven, three units each."""
+    torch = _torch()
+    from spnc import mixture as m
+    info = torch.finfo(getattr(torch, dtype))
+    z = torch.tensor([[info.min] * 7, [info.min, 0.5, info.min, info.min, 0.5, info.min, info.min], [info.max] + [0.0] * 6, [info.max] * 7,
+                      [info.min] * 6 + [-float("inf")], [info.max, info.min] + [-float("inf")] * 5], dtype=torch.float64).to(getattr(torch, dtype))
+    u = HALF["float64" if dtype == "float64" else "float32"]
+    for repeat in (1, 2000):                          # rows over many lanes and over few
+        dev = z.repeat(repeat, 1).cuda().requires_grad_()
+        for over in ("chosen", "all"):
+            index, weight = m.gate(dev, 2, over=over)
+            assert index[:6].tolist() == [[0, 1], [1, 4], [0, 1], [0, 1], [0, 1], [0, 1]]
+            half, seventh, sixth = 0.5, 0.5 if over == "chosen" else 1 / 7, 0.5 if over == "chosen" else 1 / 6
+            want = np.array([[seventh, seventh], [half, half], [1, 0], [seventh, seventh], [sixth, sixth], [1, 0]])
+            _near(weight[-6:], want, 16 * u)
+            grad = torch.zeros_like(weight)
+            grad[:, 0] = 1.0
+            got, = torch.autograd.grad(weight, dev, grad)
+            p = np.where(z.double().numpy() == z.double().max(dim=1, keepdim=True).values.numpy(), 1.0, 0.0)
+            if over == "chosen":
+                p = np.zeros_like(p)
+                np.put_along_axis(p, index[:6].cpu().numpy().astype(np.int64), want, axis=1)
+            p /= p.sum(axis=1, keepdims=True)
+            first = index[:6, 0].cpu().numpy()
+            one = np.zeros_like(p)
+            one[np.arange(6), first] = 1.0
+            _near(got[-6:], p[np.arange(6), first][:, None] * (one - p), 32 * u + 2 * HALF[dtype])
+            logs = m.gate(dev, 2, over=over, log=True)[1][-6:]
+            _near(logs[[0, 1, 3, 4]], np.log(want[[0, 1, 3, 4]]), 32 * u)
 
 
 @pytest.mark.gpu
