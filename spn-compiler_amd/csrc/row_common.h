@@ -60,7 +60,7 @@ inline unsigned tileGrid(size_t tiles) {
   return unsigned(g < MAX_GRID ? g : MAX_GRID);
 }
 
-// A group of 2^shift lanes handles a row, a piece of up to 16 bytes a lane at a time.
+// A group of 2^shift lanes, a wave or with few rows up to a block, handles a row, a piece of up to 16 bytes a lane at a time.
 //
 // Rows that are written to scattered places bypass the caches where they consist of whole 64-byte halves of cache lines: 1 M rows
 // of 64 bytes to two places each take 36 us instead of 50, of 2 KB to four places 52 instead of 67 (a consumer that reads
@@ -74,11 +74,11 @@ struct RowShape {
   bool byDie;
 };
 
-inline RowShape rowShape(size_t n, size_t rowBytes, unsigned pieceBytes, const void* scattered = nullptr) {
+inline RowShape rowShape(size_t n, size_t rowBytes, unsigned pieceBytes, const void* scattered = nullptr, unsigned most = 6) {
   RowShape s;
   s.pieces = unsigned(rowBytes / pieceBytes);
   s.shift = 0;
-  while (s.shift < 6 && (1u << s.shift) < s.pieces) ++s.shift;
+  while (s.shift < most && (1u << s.shift) < s.pieces) ++s.shift;
   const size_t rows = BLOCK >> s.shift;
   s.tiles = (n + rows - 1) / rows;
   // In the order of the blocks from 1 KB on: 4 x 32769 rows of 2 KB are combined in 59 us instead of 61. Of 8 bytes, 4 x 2 M rows take 32

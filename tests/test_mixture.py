@@ -380,7 +380,7 @@ def test_dispatch_and_its_gradient(native, dtype, width):
     """A copy, and the sum of k copies: k - 1 additions of 32 (64) bits, then the type's own rounding."""
     torch = _torch()
     from spnc import mixture as m
-    for n, k, experts, align in [(1, 1, 2, 1), (77, 3, 5, 4), (1031, 2, 16, 1)]:
+    for n, k, experts, align in [(1, 1, 2, 1), (77, 3, 5, 4), (1031, 2, 16, 1), (2100, 2, 7, 1)]:      # from 2048 rows on a wave a row
         index = _index(n, k, experts, seed=width + n)
         plan = m.route(index.cuda(), experts, align=align)
         position, _, _ = om.route(index.numpy(), experts, align)
@@ -433,7 +433,7 @@ def test_combine(native, dtype, width, weight):
         weight = "float32"
     u = HALF["float64" if dtype == "float64" else "float32"]
     tiny = 2.0 ** -25 if dtype == "float16" else 0.0
-    for n, k, experts, align in [(1, 1, 2, 1), (1, 4, 9, 1), (77, 3, 5, 4), (531, 8, 16, 1), (40, 11, 6, 1)]:
+    for n, k, experts, align in [(1, 1, 2, 1), (1, 4, 9, 1), (77, 3, 5, 4), (531, 8, 16, 1), (40, 11, 6, 1), (2100, 2, 7, 1)]:
         index = _index(n, k, experts, seed=width + n)
         plan = m.route(index.cuda(), experts, align=align)
         position = _host(plan.position)
