@@ -337,10 +337,10 @@ void withGateShape(size_t n, unsigned experts, unsigned k, size_t stride, uintpt
   const unsigned places = experts + (pairs ? 1 : 0);  // an odd row's first word begins a place earlier
   unsigned group = 0, logits = 0, best = ~0u;
   for (unsigned v : {4u, 8u, 16u, 32u}) {
-    if ((v == 8 && places <= 256) || (v > 16 && !packed) || (v > 4 && (sizeof(T) == 8 || n < GATE_MANY_ROWS) && places <= 256)) continue;
+    if ((v > 16 && !packed) || (v > 4 && (sizeof(T) == 8 || n < GATE_MANY_ROWS) && places <= 256)) continue;
     unsigned g = 1;
     while (g < WAVE && (v * g < places || g < k)) g *= 2;
-    if (v * g < places || (v == 8 && g < WAVE) || (v == 16 && g < (sizeof(T) == 8 ? WAVE : 2)) || (v == 32 && (g < 4 || g > 32))) continue;
+    if (v * g < places || (v == 8 && (g < 2 || sizeof(T) == 8) && g < WAVE) || (v == 16 && g < (sizeof(T) == 8 ? WAVE : 2)) || (v == 32 && (g < 4 || g > 32))) continue;
     const unsigned cost = n < GATE_MANY_ROWS ? v : packed ? g * (3 * v + 28) : g * (10 * v + 28);
     if (cost < best) group = g, logits = v, best = cost;
   }
@@ -362,6 +362,11 @@ void withGateShape(size_t n, unsigned experts, unsigned k, size_t stride, uintpt
   SPN_GATE_SHAPE(64, 8);
   SPN_GATE_SHAPE(64, 16);
   if constexpr (sizeof(T) < 8) {
+    SPN_GATE_SHAPE(2, 8);
+    SPN_GATE_SHAPE(4, 8);
+    SPN_GATE_SHAPE(8, 8);
+    SPN_GATE_SHAPE(16, 8);
+    SPN_GATE_SHAPE(32, 8);
     SPN_GATE_SHAPE(2, 16);
     SPN_GATE_SHAPE(4, 16);
     SPN_GATE_SHAPE(8, 16);
