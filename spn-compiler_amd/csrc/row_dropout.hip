@@ -109,6 +109,7 @@ int spnc_hip_dropout(const void* x, int dtype, size_t n, size_t width, size_t st
     if (n > 1 && (stride < width || out_stride < width)) refuse("rows overlap");
     if (n == 0 || width == 0) return;
     if (!x || !out) refuse("null argument");
+    if ((address(x) | address(out)) % elementBytes(dtype)) refuse("dropout: pointers are not aligned to the element type");
     const uint64_t threshold = uint64_t(std::llrint(p * 4294967296.0));
     const double scale = mode != SPNC_HIP_DROPOUT_ZERO ? 1.0 : threshold >> 32 ? 0.0 : 1.0 / (1.0 - p);
     const double fill = mode == SPNC_HIP_DROPOUT_MARGINAL ? NAN : 0.0;

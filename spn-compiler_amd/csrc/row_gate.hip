@@ -406,6 +406,7 @@ int spnc_hip_gate(const void* logits, int dtype, size_t n, unsigned experts, siz
     checkGate(dtype, n, experts, stride, k, flags);
     if (n == 0) return;
     if (!logits || !index || !weight) refuse("null argument");
+    if (address(logits) % elementBytes(dtype)) refuse("gate: pointers are not aligned to the element type");
     withType(dtype, [&](auto t) {
       using T = decltype(t);
       withGateShape<T>(n, experts, k, stride, address(logits), [&](auto g, auto v, auto layout) {
@@ -424,6 +425,7 @@ int spnc_hip_gate_backward(const void* logits, int dtype, size_t n, unsigned exp
     checkGate(dtype, n, experts, stride, k, flags);
     if (n == 0) return;
     if ((!logits && (flags & SPNC_HIP_GATE_ALL)) || !index || !weight || !grad_weight || !grad_logits) refuse("null argument");
+    if ((address(logits) | address(grad_logits)) % elementBytes(dtype)) refuse("gate gradient: pointers are not aligned to the element type");
     withType(dtype, [&](auto t) {
       using T = decltype(t);
       using R = wide_t<T>;

@@ -715,6 +715,7 @@ int spnc_hip_route(const int32_t* index, size_t slots, unsigned experts, unsigne
     if ((slots && (!index || !position)) || !starts || !counts) refuse("null argument");
     const RouteShape shape = routeShape(slots, experts);
     const size_t need = spnc_hip_route_workspace(slots, experts);
+    if (address(workspace) % sizeof(uint32_t)) refuse("the workspace must be aligned to 4 bytes");
     if (workspace_bytes < need || (need && !workspace)) refuse("the workspace must hold " + std::to_string(need) + " bytes");
     unsigned bits = 0;
     while ((1u << bits) < experts) ++bits;

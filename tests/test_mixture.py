@@ -121,6 +121,10 @@ def test_c_entry_points_refuse(native):
     refused(lib.spnc_hip_gate(p, 0, 2, 3, 2, 1, 0, p, p, None), "rows of logits overlap")
     refused(lib.spnc_hip_gate(p, 0, 2, 3, 3, 1, 4, p, p, None), "unknown gate flags")
     refused(lib.spnc_hip_gate(None, 0, 2, 3, 3, 1, 0, p, p, None), "null argument")
+    refused(lib.spnc_hip_gate(ctypes.c_void_p(18), 0, 2, 3, 3, 1, 0, p, p, None), "not aligned")
+    refused(lib.spnc_hip_gate(p, 0, 2, 3, 1 << 20, 1, 0, p, p, None), "2^20")
+    refused(lib.spnc_hip_dropout(ctypes.c_void_p(17), 3, 2, 4, 4, p, 4, 0.5, 0, 0, 0, None, None), "not aligned")
+    refused(lib.spnc_hip_route(p, 100000, 3, 1, p, p, p, ctypes.c_void_p(18), 1 << 20, None), "aligned to 4 bytes")
     refused(lib.spnc_hip_gate_backward(None, 0, 2, 3, 3, 1, 1, p, p, p, p, None), "null argument")
     refused(lib.spnc_hip_route(p, 4, 3, 0, p, p, p, None, 0, None), "align")
     refused(lib.spnc_hip_route(p, big, 3, 1, p, p, p, None, 0, None), "too many slots")
