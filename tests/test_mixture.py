@@ -765,6 +765,37 @@ def test_mixture_of_kernels(native, options):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", ["auto", "interpreter"])
+def test_mixture_on_several_streams(native, kind):
+    """Six segments run beside each other, two of them under one kernel: the same bits as one kernel after the other, call after call
+    and from two streams at once."""
+    torch = _torch()
+    from spnc import mixture as m
+    from spnc.hip import HIPCompiler
+    with quiet():
+        mix = HIPCompiler(**{"hip-kernel": kind}).compile_mixture(_experts(), "float32")
+    try:
+        mix = m.Mixture(mix.kernels + mix.kernels[:1])
+        x, z = torch.randn(30011, 6, device="cuda"), torch.randn(30011, 6, device="cuda")
+        index, lw = m.gate(z, 2, log=True)
+        each = torch.stack([torch.from_numpy(k.execute(30011, x.cpu().numpy())).cuda() for k in mix.kernels], 1)
+        plan = m.Plan(torch.arange(60022, dtype=torch.int32, device="cuda").view(-1, 2), torch.tensor([0, 60022], dtype=torch.int32, device="cuda"),
+                      torch.tensor([60022], dtype=torch.int32, device="cuda"), 60022)
+        want = m.combine_log(each.gather(1, index.long()).flatten(), plan, lw)
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        torch.cuda.synchronize()
+        got = []
+        for call in range(6):
+            with torch.cuda.stream(streams[call % 2]):
+                got.append(mix.log_likelihood(x, z, 2))
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, want) for g in got)
+    finally:
+        for k in mix.kernels[:5]:
+            os.remove(k.fileName())
+
+
+@pytest.mark.gpu
 def test_mixture_of_integer_kernels_is_aligned(native):
     """Rows of 6 x 4 bytes: a segment that began at an odd row would not be aligned for the kernel."""
     torch = _torch()
