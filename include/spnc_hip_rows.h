@@ -76,15 +76,17 @@ SPNC_HIP_API int spnc_hip_combine_backward(const void* values, int dtype, size_t
 
 /* out[i] = log sum over j of exp(log_weight[i * k + j] + values[position[i * k + j]]): values [capacity] and out [n] float32 or
  * float64, log_weight float32 or float64. Slots that are not routed or whose log weight is minus infinity are left out, whatever
- * value stands there; a row without slots becomes minus infinity, as a sum node whose children are all impossible. */
+ * value stands there; a row without slots becomes minus infinity, as a sum node whose children are all impossible. share [n, k] of the values'
+ * type, if not NULL, receives every slot's part of its row's sum for spnc_hip_combine_log_backward: 0 for slots that are left out and in
+ * rows whose sum is empty. */
 SPNC_HIP_API int spnc_hip_combine_log(const void* values, int dtype, size_t capacity, const int32_t* position, size_t n, unsigned k,
-                                      const void* log_weight, int weight_dtype, void* out, void* stream);
+                                      const void* log_weight, int weight_dtype, void* out, void* share, void* stream);
 
-/* grad_out [n] -> grad_values [capacity] (0 in rows of no segment) and grad_log_weight [n, k]; either may be NULL. Both are the
- * output's gradient times the share of the slot in the sum; 0 in rows whose sum is empty. */
-SPNC_HIP_API int spnc_hip_combine_log_backward(const void* values, int dtype, size_t capacity, const int32_t* position, size_t n, unsigned k,
-                                               const void* log_weight, int weight_dtype, const void* grad_out, const int32_t* starts,
-                                               const int32_t* counts, unsigned experts, void* grad_values, void* grad_log_weight, void* stream);
+/* grad_out [n] -> grad_values [capacity] (0 in rows of no segment) and grad_log_weight [n, k] of weight_dtype; either may be NULL. Both
+ * are the output's gradient times the slot's share, 0 where that is 0. position is read for grad_values only. */
+SPNC_HIP_API int spnc_hip_combine_log_backward(const void* share, int dtype, size_t capacity, const int32_t* position, size_t n, unsigned k,
+                                               int weight_dtype, const void* grad_out, const int32_t* starts, const int32_t* counts,
+                                               unsigned experts, void* grad_values, void* grad_log_weight, void* stream);
 
 /* What a dropped element becomes. */
 enum {

@@ -392,8 +392,8 @@ __global__ __launch_bounds__(BLOCK) void combineBackwardKernel(const T* __restri
 //
 // K slots a row in registers, EXACT: k of them, positions and weights one piece each; otherwise the last ones may be missing. Bound by
 // the gather of single values: lanes next to each other hold rows of different experts, so nearly every lane is an access of its own.
-// Two rows a thread keep more of them under way. 4 M rows of two slots take 26 us, 4.5 TB/s, their gradient 41 us, 4.5 TB/s: the
-// address units, which take a lane a cycle here, are busy for three quarters of that.
+// Two rows a thread keep more of them under way. 4 M rows of two slots take 26 us, 4.5 TB/s, and 30 with the shares for a backward pass: the address
+// units, which take a lane a cycle here, are busy for three quarters of that.
 template <typename R, typename W, int K, bool EXACT>
 struct LogRow {
   int32_t at[K];
@@ -443,14 +443,26 @@ struct LogRow {
     }
   }
   __device__ R result() const { return peak == -INFINITY || peak == INFINITY ? peak : peak + (shift + logOf(total)); }
-  __device__ R share(int j, R g) const { return weight[j] == -INFINITY || peak == -INFINITY ? R(0) : g * (term[j] / total); }
+  __device__ R share(int j) const { return weight[j] == -INFINITY || peak == -INFINITY ? R(0) : term[j] / total; }
 };
+
+template <typename T, int K, bool EXACT>
+__device__ inline void storeSlots(T* to, size_t row, unsigned k, const Pack<T, K>& v) {
+  if constexpr (EXACT) {
+    *reinterpret_cast<Pack<T, K>*>(to + row * K) = v;
+  } else {
+#pragma unroll
+    for (int j = 0; j < K; ++j)
+      if (j < int(k)) to[row * k + j] = v.v[j];
+  }
+}
 
 template <int K> constexpr int LOG_ROWS = K <= 2 ? 2 : 1;  // of a thread
 
 template <typename R, typename W, int K, bool EXACT>
 __global__ __launch_bounds__(BLOCK) void combineLogKernel(const R* __restrict__ values, size_t capacity, const int32_t* __restrict__ position,
-                                                          const W* __restrict__ logWeight, size_t n, unsigned k, R* __restrict__ out) {
+                                                          const W* __restrict__ logWeight, size_t n, unsigned k, R* __restrict__ out,
+                                                          R* __restrict__ shares) {
   constexpr int ROWS = LOG_ROWS<K>;
   forTiles((n + ROWS * BLOCK - 1) / (ROWS * BLOCK), gridDim.x, true, [&](size_t tile) {
     const size_t first = tile * (ROWS * BLOCK) + threadIdx.x;
@@ -461,51 +473,64 @@ __global__ __launch_bounds__(BLOCK) void combineLogKernel(const R* __restrict__ 
     for (int i = 0; i < ROWS; ++i) r[i].values(values);
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
+      const size_t row = first + i * BLOCK;
+      if (row >= n) continue;
       r[i].solve();
-      if (first + i * BLOCK < n) out[first + i * BLOCK] = r[i].result();
+      out[row] = r[i].result();
+      if (shares) {
+        Pack<R, K> o;
+#pragma unroll
+        for (int j = 0; j < K; ++j) o.v[j] = r[i].share(j);
+        storeSlots<R, K, EXACT>(shares, row, k, o);
+      }
     }
   });
 }
 
+// dv[position_ij] = dl_ij = g_i times the share that the forward pass wrote: nothing is gathered again. A share of 0 passes no gradient
+// whatever g is: its slot may have been left out. 4 M rows of two slots take 34 us, bound by
+// the scatter, and 16 us, 5.2 TB/s, without the values' gradient (compiled kernels want none); 41 where values and weights are read again.
 template <typename R, typename W, int K, bool EXACT>
-__global__ __launch_bounds__(BLOCK) void combineLogBackwardKernel(const R* __restrict__ values, size_t capacity, const int32_t* __restrict__ position,
-                                                                  const W* __restrict__ logWeight, size_t n, unsigned k, const R* __restrict__ gradOut,
-                                                                  R* __restrict__ gradValues, W* __restrict__ gradLogWeight, Unused unused) {
+__global__ __launch_bounds__(BLOCK) void combineLogBackwardKernel(const R* __restrict__ shares, const int32_t* __restrict__ position, size_t n, unsigned k,
+                                                                  size_t capacity, const R* __restrict__ gradOut, R* __restrict__ gradValues,
+                                                                  W* __restrict__ gradLogWeight, Unused unused) {
   if (blockIdx.x >= unused.rowBlocks) return clearUnused(unused);
   constexpr int ROWS = LOG_ROWS<K>;
   forTiles((n + ROWS * BLOCK - 1) / (ROWS * BLOCK), unused.rowBlocks, true, [&](size_t tile) {
     const size_t first = tile * (ROWS * BLOCK) + threadIdx.x;
-    LogRow<R, W, K, EXACT> r[ROWS];
+    Pack<R, K> share[ROWS];
+    int32_t at[ROWS][K];
     R g[ROWS];
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
       const size_t row = first + i * BLOCK < n ? first + i * BLOCK : n - 1;
-      r[i].slots(position, logWeight, row, k, capacity);
       g[i] = gradOut[row];
-    }
+      Pack<int32_t, K> p;
+      if constexpr (EXACT) {
+        share[i] = *reinterpret_cast<const Pack<R, K>*>(shares + row * K);
+        if (gradValues) p = *reinterpret_cast<const Pack<int32_t, K>*>(position + row * K);
+      } else {
 #pragma unroll
-    for (int i = 0; i < ROWS; ++i) r[i].values(values);
+        for (int j = 0; j < K; ++j) {
+          share[i].v[j] = j < int(k) ? shares[row * k + j] : R(0);
+          if (gradValues) p.v[j] = j < int(k) ? position[row * k + j] : -1;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < K; ++j) at[i][j] = gradValues && p.v[j] >= 0 && size_t(p.v[j]) < capacity ? p.v[j] : -1;
+    }
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
       const size_t row = first + i * BLOCK;
       if (row >= n) continue;
-      r[i].solve();
       Pack<W, K> o;
 #pragma unroll
       for (int j = 0; j < K; ++j) {
-        const R share = r[i].share(j, g[i]);
-        if (gradValues && r[i].at[j] >= 0) gradValues[r[i].at[j]] = share;
-        o.v[j] = W(share);
+        const R d = share[i].v[j] == 0 ? R(0) : g[i] * share[i].v[j];
+        if (at[i][j] >= 0) gradValues[at[i][j]] = d;
+        o.v[j] = W(d);
       }
-      if (gradLogWeight) {
-        if constexpr (EXACT) {
-          *reinterpret_cast<Pack<W, K>*>(gradLogWeight + row * K) = o;
-        } else {
-#pragma unroll
-          for (int j = 0; j < K; ++j)
-            if (j < int(k)) gradLogWeight[row * k + j] = o.v[j];
-        }
-      }
+      if (gradLogWeight) storeSlots<W, K, EXACT>(gradLogWeight, row, k, o);
     }
   });
 }
@@ -547,33 +572,39 @@ struct LogSlots {
 };
 
 template <typename R, typename W>
-__global__ __launch_bounds__(BLOCK) void combineLogManyKernel(LogSlots<R, W> given, size_t n, R* __restrict__ out) {
+__global__ __launch_bounds__(BLOCK) void combineLogManyKernel(LogSlots<R, W> given, size_t n, R* __restrict__ out, R* __restrict__ shares) {
   forTiles((n + BLOCK - 1) / BLOCK, gridDim.x, true, [&](size_t tile) {
     const size_t row = tile * BLOCK + threadIdx.x;
     if (row >= n) return;
     LogSlots<R, W> r = given;
     r.solve(row);
     out[row] = r.peak == -INFINITY || r.peak == INFINITY ? r.peak : r.peak + (r.shift + logOf(r.total));
+    if (!shares) return;
+    for (unsigned j = 0; j < r.k; ++j) {
+      R v, lw, share = 0;
+      int32_t at;
+      if (r.read(row * r.k + j, v, lw, at) && r.peak != -INFINITY) share = expOf(lw + (v - r.peak) - r.shift) / r.total;
+      shares[row * r.k + j] = share;
+    }
   });
 }
 
 template <typename R, typename W>
-__global__ __launch_bounds__(BLOCK) void combineLogManyBackwardKernel(LogSlots<R, W> given, size_t n, const R* __restrict__ gradOut,
+__global__ __launch_bounds__(BLOCK) void combineLogManyBackwardKernel(const R* __restrict__ shares, const int32_t* __restrict__ position, size_t n,
+                                                                      unsigned k, size_t capacity, const R* __restrict__ gradOut,
                                                                       R* __restrict__ gradValues, W* __restrict__ gradLogWeight, Unused unused) {
   if (blockIdx.x >= unused.rowBlocks) return clearUnused(unused);
   forTiles((n + BLOCK - 1) / BLOCK, unused.rowBlocks, true, [&](size_t tile) {
     const size_t row = tile * BLOCK + threadIdx.x;
     if (row >= n) return;
-    LogSlots<R, W> r = given;
-    r.solve(row);
     const R g = gradOut[row];
-    for (unsigned j = 0; j < r.k; ++j) {
-      const size_t s = row * r.k + j;
-      R v, lw, share = 0;
-      int32_t at;
-      if (r.read(s, v, lw, at) && r.peak != -INFINITY) share = g * (expOf(lw + (v - r.peak) - r.shift) / r.total);
-      if (gradValues && at >= 0) gradValues[at] = share;
-      if (gradLogWeight) gradLogWeight[s] = W(share);
+    for (size_t s = row * k; s < row * k + k; ++s) {
+      const R d = shares[s] == 0 ? R(0) : g * shares[s];
+      if (gradValues) {
+        const int32_t at = position[s];
+        if (at >= 0 && size_t(at) < capacity) gradValues[at] = d;
+      }
+      if (gradLogWeight) gradLogWeight[s] = W(d);
     }
   });
 }
@@ -662,11 +693,10 @@ void checkSegments(const int32_t* starts, const int32_t* counts, unsigned expert
   if (!starts || !counts) refuse("null argument");
 }
 
-// calls fn(K, EXACT), see LogRow; K = 0 for more than eight
+// calls fn(K, EXACT), see LogRow; K = 0 for more than eight. W: the widest type that is read or written k at a time.
 template <typename W, typename Fn>
-void withLogChoices(unsigned k, const void* position, const void* weight, const void* gradWeight, Fn&& fn) {
-  const size_t piece = k * sizeof(W) < 16 ? k * sizeof(W) : 16;
-  const bool exact = (k & (k - 1)) == 0 && (address(position) | address(weight) | address(gradWeight)) % piece == 0;
+void withLogChoices(unsigned k, uintptr_t addresses, Fn&& fn) {
+  const bool exact = (k & (k - 1)) == 0 && addresses % (k * sizeof(W) < 16 ? k * sizeof(W) : 16) == 0;
   auto choose = [&](auto kb) { exact ? fn(kb, std::true_type()) : fn(kb, std::false_type()); };
   if (k == 1) return fn(std::integral_constant<int, 1>(), std::true_type());
   if (k == 2) return choose(std::integral_constant<int, 2>());
@@ -839,57 +869,59 @@ int spnc_hip_combine_backward(const void* values, int dtype, size_t capacity, si
 }
 
 int spnc_hip_combine_log(const void* values, int dtype, size_t capacity, const int32_t* position, size_t n, unsigned k, const void* log_weight,
-                         int weight_dtype, void* out, void* stream) {
+                         int weight_dtype, void* out, void* share, void* stream) {
   return guarded([&] {
     checkLogTypes(dtype, weight_dtype);
     checkSlots(n, k, capacity);
     if (n == 0) return;
     if ((capacity && !values) || !position || !log_weight || !out) refuse("null argument");
     if (capacity == 0) values = out;  // no slot is routed; there has to be a value to read and drop
+    const hipStream_t s = static_cast<hipStream_t>(stream);
     withLogTypes(dtype, weight_dtype, [&](auto r, auto w) {
       using R = decltype(r);
       using W = decltype(w);
-      withLogChoices<W>(k, position, log_weight, nullptr, [&](auto kb, auto exact) {
+      using Widest = typename std::conditional<(sizeof(R) > sizeof(W)), R, W>::type;
+      withLogChoices<Widest>(k, address(position) | address(log_weight) | address(share), [&](auto kb, auto exact) {
         constexpr int K = decltype(kb)::value;
         if constexpr (K > 0)
-          combineLogKernel<R, W, K, decltype(exact)::value><<<logGrid(n, k), BLOCK, 0, static_cast<hipStream_t>(stream)>>>(
-              static_cast<const R*>(values), capacity, position, static_cast<const W*>(log_weight), n, k, static_cast<R*>(out));
+          combineLogKernel<R, W, K, decltype(exact)::value><<<logGrid(n, k), BLOCK, 0, s>>>(
+              static_cast<const R*>(values), capacity, position, static_cast<const W*>(log_weight), n, k, static_cast<R*>(out), static_cast<R*>(share));
         else
-          combineLogManyKernel<R, W><<<logGrid(n, k), BLOCK, 0, static_cast<hipStream_t>(stream)>>>(
-              LogSlots<R, W>{static_cast<const R*>(values), capacity, position, static_cast<const W*>(log_weight), k}, n, static_cast<R*>(out));
+          combineLogManyKernel<R, W><<<logGrid(n, k), BLOCK, 0, s>>>(
+              LogSlots<R, W>{static_cast<const R*>(values), capacity, position, static_cast<const W*>(log_weight), k}, n, static_cast<R*>(out),
+              static_cast<R*>(share));
       });
     });
     launched("combine_log");
   });
 }
 
-int spnc_hip_combine_log_backward(const void* values, int dtype, size_t capacity, const int32_t* position, size_t n, unsigned k,
-                                  const void* log_weight, int weight_dtype, const void* grad_out, const int32_t* starts, const int32_t* counts,
-                                  unsigned experts, void* grad_values, void* grad_log_weight, void* stream) {
+int spnc_hip_combine_log_backward(const void* share, int dtype, size_t capacity, const int32_t* position, size_t n, unsigned k, int weight_dtype,
+                                  const void* grad_out, const int32_t* starts, const int32_t* counts, unsigned experts, void* grad_values,
+                                  void* grad_log_weight, void* stream) {
   return guarded([&] {
     checkLogTypes(dtype, weight_dtype);
     checkSlots(n, k, capacity);
     if (grad_values) checkSegments(starts, counts, experts);
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (!grad_values && !grad_log_weight) return;
-    if (n && ((capacity && !values) || !position || !log_weight || !grad_out)) refuse("null argument");
-    if (capacity == 0) values = grad_out;
-    const Unused unused =
-        unusedRows(logGrid(n, k), starts, counts, experts, capacity, elementBytes(dtype), grad_values);
+    if (n && (!share || (grad_values && !position) || !grad_out)) refuse("null argument");
+    const Unused unused = unusedRows(logGrid(n, k), starts, counts, experts, capacity, elementBytes(dtype), grad_values);
     if (unused.rowBlocks + unused.blocks == 0) return;
     withLogTypes(dtype, weight_dtype, [&](auto r, auto w) {
       using R = decltype(r);
       using W = decltype(w);
-      withLogChoices<W>(k, position, log_weight, grad_log_weight, [&](auto kb, auto exact) {
+      using Widest = typename std::conditional<(sizeof(R) > sizeof(W)), R, W>::type;
+      withLogChoices<Widest>(k, address(share) | address(grad_log_weight) | (grad_values ? address(position) : 0), [&](auto kb, auto exact) {
         constexpr int K = decltype(kb)::value;
         if constexpr (K > 0)
           combineLogBackwardKernel<R, W, K, decltype(exact)::value><<<unused.rowBlocks + unused.blocks, BLOCK, 0, s>>>(
-              static_cast<const R*>(values), capacity, position, static_cast<const W*>(log_weight), n, k, static_cast<const R*>(grad_out),
-              static_cast<R*>(grad_values), static_cast<W*>(grad_log_weight), unused);
+              static_cast<const R*>(share), position, n, k, capacity, static_cast<const R*>(grad_out), static_cast<R*>(grad_values),
+              static_cast<W*>(grad_log_weight), unused);
         else
           combineLogManyBackwardKernel<R, W><<<unused.rowBlocks + unused.blocks, BLOCK, 0, s>>>(
-              LogSlots<R, W>{static_cast<const R*>(values), capacity, position, static_cast<const W*>(log_weight), k}, n,
-              static_cast<const R*>(grad_out), static_cast<R*>(grad_values), static_cast<W*>(grad_log_weight), unused);
+              static_cast<const R*>(share), position, n, k, capacity, static_cast<const R*>(grad_out), static_cast<R*>(grad_values),
+              static_cast<W*>(grad_log_weight), unused);
       });
     });
     launched("combine_log gradient");

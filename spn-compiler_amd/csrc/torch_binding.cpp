@@ -288,32 +288,36 @@ Tensor combine(const Tensor& values, const Tensor& position, const Tensor& start
   return Combine::apply(values, weights.defined() ? std::optional<Tensor>(weights) : std::nullopt, plan);
 }
 
-Tensor combineLogForward(const Tensor& values, const Plan& plan, const Tensor& weights) {
+Tensor combineLogForward(const Tensor& values, const Plan& plan, const Tensor& weights, const Tensor& share) {
   c10::DeviceGuard guard(values.device());
   Tensor result = at::empty({plan.rows()}, values.options().requires_grad(false));
   check(spnc_hip_combine_log(data(values), elementType(values.scalar_type()), plan.capacity, ints(plan.position), plan.rows(), plan.k(), data(weights),
-                             elementType(weights.scalar_type()), out(result), streamOf(values)));
+                             elementType(weights.scalar_type()), out(result), out(share), streamOf(values)));
   return result;
 }
 
 struct CombineLog : torch::autograd::Function<CombineLog> {
   static Tensor forward(AutogradContext* ctx, const Tensor& values, const Tensor& weights, const Plan& plan) {
+    c10::DeviceGuard guard(values.device());
+    const Tensor share = at::empty(weights.sizes(), values.options().requires_grad(false));
     ctx->saved_data["capacity"] = plan.capacity;
-    ctx->save_for_backward(savedWith(plan, {values, weights}));
-    return combineLogForward(values, plan, weights);
+    ctx->saved_data["weights"] = int64_t(weights.scalar_type());
+    ctx->save_for_backward(savedWith(plan, {share}));
+    return combineLogForward(values, plan, weights, share);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Plan plan = savedPlan(ctx, saved);
-    const Tensor &values = saved[0], &weights = saved[1];
-    c10::DeviceGuard guard(values.device());
+    const Tensor& share = saved[0];
+    c10::DeviceGuard guard(share.device());
+    const auto type = at::ScalarType(ctx->saved_data["weights"].toInt());
     const Tensor grad = grads[0].contiguous();
     Tensor gradValues, gradWeights;
-    if (ctx->needs_input_grad(0)) gradValues = at::empty(values.sizes(), values.options().requires_grad(false));
-    if (ctx->needs_input_grad(1)) gradWeights = at::empty(weights.sizes(), weights.options().requires_grad(false));
-    check(spnc_hip_combine_log_backward(data(values), elementType(values.scalar_type()), plan.capacity, ints(plan.position), plan.rows(), plan.k(),
-                                        data(weights), elementType(weights.scalar_type()), data(grad), ints(plan.starts), ints(plan.counts),
-                                        plan.experts(), out(gradValues), out(gradWeights), streamOf(values)));
+    if (ctx->needs_input_grad(0)) gradValues = at::empty({plan.capacity}, share.options());
+    if (ctx->needs_input_grad(1)) gradWeights = at::empty(share.sizes(), share.options().dtype(type));
+    check(spnc_hip_combine_log_backward(data(share), elementType(share.scalar_type()), plan.capacity, ints(plan.position), plan.rows(), plan.k(),
+                                        elementType(type), data(grad), ints(plan.starts), ints(plan.counts), plan.experts(), out(gradValues),
+                                        out(gradWeights), streamOf(share)));
     return once({gradValues, gradWeights, Tensor()});
   }
 };
@@ -325,7 +329,7 @@ Tensor combineLog(const Tensor& given, const Tensor& position, const Tensor& sta
   checkWeights(logWeights, plan, true);
   onGpu({&given, &position, &starts, &counts, &logWeights});
   const Tensor values = given.contiguous(), weights = logWeights.contiguous();
-  if (!wantsGrad({&values, &weights})) return combineLogForward(values, plan, weights);
+  if (!wantsGrad({&values, &weights})) return combineLogForward(values, plan, weights, Tensor());
   return CombineLog::apply(values, weights, plan);
 }
 

@@ -108,8 +108,8 @@ def _load():
     lib.spnc_hip_dispatch.argtypes = [vp, sz, sz, sz, vp, u, sz, vp, vp, u, i, vp, vp]
     lib.spnc_hip_combine.argtypes = [vp, i, sz, sz, sz, vp, sz, u, vp, i, vp, vp]
     lib.spnc_hip_combine_backward.argtypes = [vp, i, sz, sz, sz, vp, sz, u, vp, i, vp, sz, vp, vp, u, vp, vp, vp]
-    lib.spnc_hip_combine_log.argtypes = [vp, i, sz, vp, sz, u, vp, i, vp, vp]
-    lib.spnc_hip_combine_log_backward.argtypes = [vp, i, sz, vp, sz, u, vp, i, vp, vp, vp, u, vp, vp, vp]
+    lib.spnc_hip_combine_log.argtypes = [vp, i, sz, vp, sz, u, vp, i, vp, vp, vp]
+    lib.spnc_hip_combine_log_backward.argtypes = [vp, i, sz, vp, sz, u, i, vp, vp, vp, u, vp, vp, vp]
     lib.spnc_hip_dropout.argtypes = [vp, i, sz, sz, sz, vp, sz, d, i, u64, u64, vp, vp]
     _lib = lib
     return lib

@@ -139,9 +139,10 @@ def test_c_entry_points_refuse(native):
     refused(lib.spnc_hip_combine(p, 0, 4, 4, 4, p, 2, 2, p, 1, p, None), "weights must be float32")
     refused(lib.spnc_hip_combine(ctypes.c_void_p(18), 0, 4, 4, 4, p, 2, 2, p, 0, p, None), "not aligned")
     refused(lib.spnc_hip_combine_backward(p, 0, 4, 4, 4, p, 2, 2, p, 0, p, 4, None, None, 3, p, p, None), "null argument")
-    refused(lib.spnc_hip_combine_log(p, 2, 4, p, 2, 2, p, 0, p, None), "must be float32 or float64")
-    refused(lib.spnc_hip_combine_log(p, 0, 4, p, 2, 2, None, 0, p, None), "null argument")
-    refused(lib.spnc_hip_combine_log_backward(p, 0, 4, p, 2, 2, p, 0, p, p, None, 3, p, p, None), "null argument")
+    refused(lib.spnc_hip_combine_log(p, 2, 4, p, 2, 2, p, 0, p, p, None), "must be float32 or float64")
+    refused(lib.spnc_hip_combine_log(p, 0, 4, p, 2, 2, None, 0, p, p, None), "null argument")
+    refused(lib.spnc_hip_combine_log_backward(p, 0, 4, p, 2, 2, 0, p, p, None, 3, p, p, None), "null argument")
+    refused(lib.spnc_hip_combine_log_backward(None, 0, 4, p, 2, 2, 0, p, p, p, 3, p, p, None), "null argument")
     refused(lib.spnc_hip_dropout(p, 0, 2, 4, 4, p, 4, 1.5, 0, 0, 0, None, None), "probability")
     refused(lib.spnc_hip_dropout(p, 0, 2, 4, 4, p, 4, float("nan"), 0, 0, 0, None, None), "probability")
     refused(lib.spnc_hip_dropout(p, 0, 2, 4, 3, p, 4, 0.5, 0, 0, 0, None, None), "overlap")
