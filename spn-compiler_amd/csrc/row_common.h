@@ -175,6 +175,13 @@ __device__ inline double logOf(double x) { return log(x); }
 
 [[noreturn]] inline void refuse(const std::string& what) { throw std::runtime_error(what); }
 
+// guarded() for entry points that launch: an error that someone else left behind is not this call's.
+template <typename Fn>
+int launching(Fn&& fn) {
+  (void)hipGetLastError();
+  return guarded(fn);
+}
+
 inline void launched(const char* what) {
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) refuse(std::string(what) + " launch: " + hipGetErrorString(e));

@@ -102,7 +102,7 @@ extern "C" {
 
 int spnc_hip_dropout(const void* x, int dtype, size_t n, size_t width, size_t stride, void* out, size_t out_stride, double p, int mode,
                      uint64_t seed, uint64_t offset, const uint64_t* offset_device, void* stream) {
-  return guarded([&] {
+  return launching([&] {
     elementBytes(dtype);
     if (!(p >= 0.0 && p <= 1.0)) refuse("the probability of dropping an element must be between 0 and 1");
     if (mode < SPNC_HIP_DROPOUT_ZERO || mode > SPNC_HIP_DROPOUT_MASK) refuse("unknown dropout mode " + std::to_string(mode));

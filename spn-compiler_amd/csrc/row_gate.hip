@@ -402,7 +402,7 @@ extern "C" {
 
 int spnc_hip_gate(const void* logits, int dtype, size_t n, unsigned experts, size_t stride, unsigned k, unsigned flags, int32_t* index,
                   void* weight, void* stream) {
-  return guarded([&] {
+  return launching([&] {
     checkGate(dtype, n, experts, stride, k, flags);
     if (n == 0) return;
     if (!logits || !index || !weight) refuse("null argument");
@@ -421,7 +421,7 @@ int spnc_hip_gate(const void* logits, int dtype, size_t n, unsigned experts, siz
 
 int spnc_hip_gate_backward(const void* logits, int dtype, size_t n, unsigned experts, size_t stride, unsigned k, unsigned flags,
                            const int32_t* index, const void* weight, const void* grad_weight, void* grad_logits, void* stream) {
-  return guarded([&] {
+  return launching([&] {
     checkGate(dtype, n, experts, stride, k, flags);
     if (n == 0) return;
     if ((!logits && (flags & SPNC_HIP_GATE_ALL)) || !index || !weight || !grad_weight || !grad_logits) refuse("null argument");

@@ -737,7 +737,7 @@ size_t spnc_hip_route_workspace(size_t slots, unsigned experts) {
 
 int spnc_hip_route(const int32_t* index, size_t slots, unsigned experts, unsigned align, int32_t* position, int32_t* starts, int32_t* counts,
                    void* workspace, size_t workspace_bytes, void* stream) {
-  return guarded([&] {
+  return launching([&] {
     checkExperts(experts);
     if (align == 0) refuse("align must be at least 1");
     if (slots >= (size_t(1) << 31) || slots + size_t(experts) * (align - 1) >= (size_t(1) << 31))
@@ -771,7 +771,7 @@ int spnc_hip_route(const int32_t* index, size_t slots, unsigned experts, unsigne
 
 int spnc_hip_dispatch(const void* rows, size_t n, size_t row_bytes, size_t stride_bytes, const int32_t* position, unsigned k, size_t capacity,
                       const int32_t* starts, const int32_t* counts, unsigned experts, int zero_unused, void* out, void* stream) {
-  return guarded([&] {
+  return launching([&] {
     checkSlots(n, k, capacity);
     if (row_bytes >> 31) refuse("a row must be shorter than 2 GiB");
     if (zero_unused) checkSegments(starts, counts, experts);
@@ -798,7 +798,7 @@ int spnc_hip_dispatch(const void* rows, size_t n, size_t row_bytes, size_t strid
 
 int spnc_hip_combine(const void* values, int dtype, size_t capacity, size_t width, size_t stride, const int32_t* position, size_t n, unsigned k,
                      const void* weight, int weight_dtype, void* out, void* stream) {
-  return guarded([&] {
+  return launching([&] {
     const size_t bytes = elementBytes(dtype);
     checkSlots(n, k, capacity);
     if (weight) checkWeightType(dtype, weight_dtype);
@@ -833,7 +833,7 @@ int spnc_hip_combine(const void* values, int dtype, size_t capacity, size_t widt
 int spnc_hip_combine_backward(const void* values, int dtype, size_t capacity, size_t width, size_t stride, const int32_t* position, size_t n,
                               unsigned k, const void* weight, int weight_dtype, const void* grad_out, size_t grad_stride, const int32_t* starts,
                               const int32_t* counts, unsigned experts, void* grad_values, void* grad_weight, void* stream) {
-  return guarded([&] {
+  return launching([&] {
     const size_t bytes = elementBytes(dtype);
     checkSlots(n, k, capacity);
     checkWeightType(dtype, weight_dtype);
@@ -870,7 +870,7 @@ int spnc_hip_combine_backward(const void* values, int dtype, size_t capacity, si
 
 int spnc_hip_combine_log(const void* values, int dtype, size_t capacity, const int32_t* position, size_t n, unsigned k, const void* log_weight,
                          int weight_dtype, void* out, void* share, void* stream) {
-  return guarded([&] {
+  return launching([&] {
     checkLogTypes(dtype, weight_dtype);
     checkSlots(n, k, capacity);
     if (n == 0) return;
@@ -899,7 +899,7 @@ int spnc_hip_combine_log(const void* values, int dtype, size_t capacity, const i
 int spnc_hip_combine_log_backward(const void* share, int dtype, size_t capacity, const int32_t* position, size_t n, unsigned k, int weight_dtype,
                                   const void* grad_out, const int32_t* starts, const int32_t* counts, unsigned experts, void* grad_values,
                                   void* grad_log_weight, void* stream) {
-  return guarded([&] {
+  return launching([&] {
     checkLogTypes(dtype, weight_dtype);
     checkSlots(n, k, capacity);
     if (grad_values) checkSegments(starts, counts, experts);

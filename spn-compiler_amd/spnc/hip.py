@@ -72,7 +72,8 @@ class HIPCompiler:
         return kernel
 
     def compile_mixture(self, spns, inputDataType="float64", errorModel=ErrorModel(), batchSize=64, supportMarginal=True, name="spn_hip"):
-        """Compile SPNs over the same features into the experts of a gated mixture (``spnc.mixture.Mixture``)."""
+        """Compile SPNs over the same features into the experts of a gated mixture (``spnc.mixture.Mixture``). The kernel files
+        of its ``kernels`` are the caller's, as those of ``compile_ll`` are."""
         from .mixture import Mixture
         return Mixture([self.compile_ll(spn, inputDataType, errorModel=errorModel, batchSize=batchSize, supportMarginal=supportMarginal,
                                         name=f"{name}_{i}") for i, spn in enumerate(spns)])

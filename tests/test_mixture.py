@@ -878,6 +878,19 @@ def test_captured_training_step_and_other_streams(native):
 
 
 @pytest.mark.gpu
+def test_an_error_left_behind_is_not_ours(native):
+    """Somebody's failed runtime call (a device that does not exist) leaves its code to be read by the next who asks."""
+    torch = _torch()
+    from spnc import mixture as m
+    z = torch.randn(4, 6, device="cuda")
+    want = m.gate(z, 2)
+    hip = ctypes.CDLL(os.path.join(os.path.dirname(torch.__file__), "lib", "libamdhip64.so"))      # the runtime both use
+    assert hip.hipSetDevice(ctypes.c_int(9999)) != 0 and hip.hipPeekAtLastError() != 0
+    got = m.gate(z, 2)
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.gpu
 def test_mixture_refuses_capture(native):
     torch = _torch()
     from spnc.hip import HIPCompiler
