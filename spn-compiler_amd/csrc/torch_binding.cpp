@@ -231,6 +231,7 @@ Tensor dispatch(const Tensor& rows, const Tensor& position, const Tensor& starts
            "out must be a contiguous ", rows.scalar_type(), " tensor of shape [", capacity, ", ", rows.size(1), "]");
     refuse(wantsGrad({&rows, &*result}), "dispatch with out= has no gradient; call it without");
     onGpu({&rows, &position, &starts, &counts, &*result});
+    torch::autograd::impl::bump_version(*result);  // whoever saved the buffer for a backward pass learns that it was written to
     return dispatchForward(rows, plan, *result, false);
   }
   onGpu({&rows, &position, &starts, &counts});
