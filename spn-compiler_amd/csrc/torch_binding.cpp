@@ -53,8 +53,14 @@ bool wantsGrad(std::initializer_list<const Tensor*> tensors) {
   return false;
 }
 
+// Views of a conjugate's imaginary part, which autograd hands out as gradients too, hold their numbers with the other sign. Memory that
+// holds a tensor's own numbers, a copy for such a view:
+Tensor plain(const Tensor& t) { return C10_UNLIKELY(t.is_neg()) ? t.resolve_neg() : t; }
+Tensor flat(const Tensor& t) { return plain(t).contiguous(); }
+
 // A 2-D tensor whose rows are contiguous and do not overlap; a copy where they are not.
-Tensor rowsOf(const Tensor& t) {
+Tensor rowsOf(const Tensor& given) {
+  const Tensor t = plain(given);
   const int64_t n = t.size(0), width = t.size(1);
   if ((width <= 1 || t.stride(1) == 1) && (n <= 1 || t.stride(0) >= width)) return t;
   return t.contiguous();
@@ -134,7 +140,7 @@ struct Gate : torch::autograd::Function<Gate> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &index = saved[1], &weight = saved[2];
     c10::DeviceGuard guard(index.device());
-    const Tensor logits = saved[0].defined() ? logitsOf(saved[0]) : Tensor(), grad = grads[1].contiguous();
+    const Tensor logits = saved[0].defined() ? logitsOf(saved[0]) : Tensor(), grad = flat(grads[1]);
     const int64_t flags = ctx->saved_data["flags"].toInt(), experts = ctx->saved_data["experts"].toInt();
     const auto type = at::ScalarType(ctx->saved_data["type"].toInt());
     Tensor result = at::empty({index.size(0), experts}, weight.options().dtype(type).requires_grad(false));
@@ -227,7 +233,7 @@ Tensor dispatch(const Tensor& rows, const Tensor& position, const Tensor& starts
   refuse(rows.element_size() > 8 || rows.is_complex(), "Rows of ", rows.scalar_type(), " are not supported");
   if (result) {
     refuse(result->dim() != 2 || result->size(0) != capacity || result->size(1) != rows.size(1) || result->scalar_type() != rows.scalar_type() ||
-               !result->is_contiguous(),
+               !result->is_contiguous() || result->is_neg(),
            "out must be a contiguous ", rows.scalar_type(), " tensor of shape [", capacity, ", ", rows.size(1), "]");
     refuse(wantsGrad({&rows, &*result}), "dispatch with out= has no gradient; call it without");
     onGpu({&rows, &position, &starts, &counts, &*result});
@@ -281,7 +287,7 @@ Tensor combine(const Tensor& values, const Tensor& position, const Tensor& start
   if (given) {
     checkWeights(*given, plan, values.scalar_type() == at::kDouble);
     onGpu({&values, &position, &starts, &counts, &*given});
-    weights = given->contiguous();
+    weights = flat(*given);
   } else {
     onGpu({&values, &position, &starts, &counts});
   }
@@ -312,7 +318,7 @@ struct CombineLog : torch::autograd::Function<CombineLog> {
     const Tensor& share = saved[0];
     c10::DeviceGuard guard(share.device());
     const auto type = at::ScalarType(ctx->saved_data["weights"].toInt());
-    const Tensor grad = grads[0].contiguous();
+    const Tensor grad = flat(grads[0]);
     Tensor gradValues, gradWeights;
     if (ctx->needs_input_grad(0)) gradValues = at::empty({plan.capacity}, share.options());
     if (ctx->needs_input_grad(1)) gradWeights = at::empty(share.sizes(), share.options().dtype(type));
@@ -329,7 +335,7 @@ Tensor combineLog(const Tensor& given, const Tensor& position, const Tensor& sta
   refuse(given.scalar_type() != at::kFloat && given.scalar_type() != at::kDouble, "Values must be float32 or float64, got ", given.scalar_type());
   checkWeights(logWeights, plan, true);
   onGpu({&given, &position, &starts, &counts, &logWeights});
-  const Tensor values = given.contiguous(), weights = logWeights.contiguous();
+  const Tensor values = flat(given), weights = flat(logWeights);
   if (!wantsGrad({&values, &weights})) return combineLogForward(values, plan, weights, Tensor());
   return CombineLog::apply(values, weights, plan);
 }

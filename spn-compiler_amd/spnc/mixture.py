@@ -192,6 +192,7 @@ class Mixture:
         _refuse(device.type != "cuda" or any(t.device != device for t in (plan.position, plan.starts, plan.counts)),
                 f"Rows and plan must be on one GPU, got {device} and {plan.position.device}")
         _refuse(torch.cuda.is_current_stream_capturing(), "A mixture cannot run under graph capture: the host needs the segments' sizes")
+        rows = rows.resolve_neg()
         values = torch.empty(plan.capacity, dtype=self._result, device=device)
         row_bytes, result_bytes = self.num_features * self._feature_bytes, values.element_size()
         with torch.cuda.device(device):
