@@ -223,6 +223,26 @@ inline void checkAligned(unsigned piece, const char* what) {
   if (piece == 0) refuse(std::string(what) + ": pointers are not aligned to the element type");
 }
 
+// Rows of `bytes` bytes in memory, `stride` bytes apart.
+struct Span {
+  const void* at;
+  size_t rows, bytes, stride;
+};
+
+// whether contiguous memory and rows share a byte; rows may lie around it
+inline bool overlap(const void* out, size_t outBytes, const Span& in) {
+  if (outBytes == 0 || in.rows == 0 || in.bytes == 0) return false;
+  const uintptr_t o = address(out), r = address(in.at), step = in.stride ? in.stride : 1;
+  const size_t behind = r + in.bytes > o ? 0 : (o - r - in.bytes) / step + 1;  // rows that end before it begins
+  return behind < (in.stride ? in.rows : 1) && r + behind * in.stride < o + outBytes;
+}
+
+// Kernels read through __restrict__ pointers, and while others write: no output lies in an input.
+inline void checkApart(const char* what, const void* out, size_t outBytes, std::initializer_list<Span> inputs) {
+  for (const Span& in : inputs)
+    if (overlap(out, outBytes, in)) refuse(std::string(what) + ": the output overlaps an input");
+}
+
 inline void checkExperts(unsigned experts) {
   if (experts == 0 || experts > SPNC_HIP_MAX_EXPERTS) refuse("experts must be between 1 and " + std::to_string(SPNC_HIP_MAX_EXPERTS));
 }

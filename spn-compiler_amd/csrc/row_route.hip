@@ -777,6 +777,9 @@ int spnc_hip_dispatch(const void* rows, size_t n, size_t row_bytes, size_t strid
     if (zero_unused) checkSegments(starts, counts, experts);
     if (capacity == 0 || row_bytes == 0) return;
     if (!out || (n && (!rows || !position))) refuse("null argument");
+    checkApart("dispatch", out, capacity * row_bytes, {{rows, n, row_bytes, stride_bytes}, {position, 1, n * k * sizeof(int32_t), 0},
+                                                       {starts, zero_unused ? 1u : 0u, (experts + size_t(1)) * sizeof(int32_t), 0},
+                                                       {counts, zero_unused ? 1u : 0u, experts * sizeof(int32_t), 0}});
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const unsigned piece = pieceBytes(1, {address(rows), address(out), row_bytes, stride_bytes});
     const RowShape shape = rowShape(n, row_bytes, piece, out, n < FEW_ROWS ? 8 : 6);

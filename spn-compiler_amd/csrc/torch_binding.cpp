@@ -2,6 +2,7 @@
 // outputs from PyTorch's allocator, the current stream of the tensors' device and autograd nodes; all arithmetic is behind the
 // C-ABI. In C++ because a call of a few microseconds of GPU time is otherwise dominated by the interpreter, twice so where
 // the backward pass runs on PyTorch's own thread.
+#include <ATen/MemoryOverlap.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
@@ -235,6 +236,11 @@ Tensor dispatch(const Tensor& rows, const Tensor& position, const Tensor& starts
     refuse(result->dim() != 2 || result->size(0) != capacity || result->size(1) != rows.size(1) || result->scalar_type() != rows.scalar_type() ||
                !result->is_contiguous() || result->is_neg(),
            "out must be a contiguous ", rows.scalar_type(), " tensor of shape [", capacity, ", ", rows.size(1), "]");
+    // views that this cannot tell are either told apart behind the C-ABI, which knows the rows' strides, or copied first
+    for (const Tensor* read : {&rows, &position, &starts, &counts}) {
+      const auto status = at::get_overlap_status(*result, *read);
+      refuse(status == at::MemOverlapStatus::Full || status == at::MemOverlapStatus::Partial, "out must not share memory with the rows or the plan");
+    }
     refuse(wantsGrad({&rows, &*result}), "dispatch with out= has no gradient; call it without");
     onGpu({&rows, &position, &starts, &counts, &*result});
     torch::autograd::impl::bump_version(*result);  // whoever saved the buffer for a backward pass learns that it was written to

@@ -102,8 +102,8 @@ def dispatch(rows, plan, out=None):
     """The rows in the plan's order: ``out[plan.position[i, j]] = rows[i]`` for every slot that is routed.
 
     rows : [n, width] of any type of 1, 2, 4 or 8 bytes an element; differentiable where floating point.
-    out  : [capacity, width] to write into; its rows that belong to no segment are left as they were. Without it a new
-           tensor is returned in which they are zero.
+    out  : [capacity, width] to write into, which must not share memory with rows or plan; its rows that belong to no segment are left
+           as they were. Without it a new tensor is returned in which they are zero.
     """
     return (_native or _ops()).dispatch(rows, plan.position, plan.starts, plan.counts, plan.capacity, out)
 

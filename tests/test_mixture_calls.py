@@ -1,10 +1,13 @@
 """Calls of spnc.mixture and of its C-ABI that are out of the ordinary: buffers that are used again or shared, views whose memory does not
 hold their values, kinds of derivatives that are not offered, errors of other calls."""
+import ctypes
 import os
+import random
+import subprocess
 
 import pytest
 
-from conftest import quiet
+from conftest import ROOT, quiet
 
 
 def _torch():
@@ -103,3 +106,83 @@ def test_kernels_over_negated_views(mix):
     rows = m.dispatch(x, plan)
     position = plan.position.flatten().long()
     assert torch.equal(mix.execute(torch._neg_view(-rows), plan)[position], mix.execute(rows, plan)[position])
+
+
+# ---- shared memory --------------------------------------------------------------------------------------------------
+
+def _refused(lib, rc, message):
+    text = lib.spnc_hip_last_error().decode()
+    assert rc != 0 and message in text, text
+
+
+def test_dispatch_refuses_to_write_where_it_reads(native):
+    """Through the C-ABI, with addresses that nobody reads: the calls are refused first."""
+    lib, p = native._load(), ctypes.c_void_p
+
+    def call(rows, out, n=4, row_bytes=16, stride=16, position=1 << 30, capacity=4, starts=1 << 31, counts=1 << 32, clear=0):
+        return lib.spnc_hip_dispatch(p(rows), n, row_bytes, stride, p(position), 1, capacity, p(starts), p(counts), 2, clear, p(out), None)
+
+    base = 1 << 20
+    for rows, out, more in [(base, base, {}), (base, base + 48, {}), (base + 48, base, {}), (base, base + 63, {}), (base + 16, base, dict(capacity=2)),
+                            (base, base + 63, dict(n=2, row_bytes=64, stride=256, capacity=1)),
+                            (base, base + 256 - 63, dict(n=2, row_bytes=64, stride=256, capacity=1)),
+                            (base, base + 8, dict(stride=0)),                                                      # one row for all
+                            (base, 1 << 25, dict(position=(1 << 25) + 63)), (base, 1 << 25, dict(position=(1 << 25) - 15)),
+                            (base, 1 << 25, dict(starts=1 << 25, clear=1)), (base, 1 << 25, dict(counts=(1 << 25) + 60, clear=1))]:
+        _refused(lib, call(rows, out, **more), "overlaps")
+
+
+def _overlap_program(tmp_path):
+    """The test of the entry points by itself: out, its bytes, and rows' address, number, bytes and stride a line, from standard input."""
+    src = tmp_path / "o.hip"
+    src.write_text('#include <cstdio>\n#include "row_common.h"\nstd::string& spnc_hip::lastError() { static std::string s; return s; }\n'
+                   'int main() { size_t o, l, r, n, b, s; while (scanf("%zu %zu %zu %zu %zu %zu", &o, &l, &r, &n, &b, &s) == 6)'
+                   ' putchar(spnc_hip::overlap(reinterpret_cast<void*>(o), l, {reinterpret_cast<void*>(r), n, b, s}) ? \'1\' : \'0\'); }\n')
+    exe = str(tmp_path / "o")
+    subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-std=c++17", "-Wno-unused-function", "-I", os.path.join(ROOT, "spn-compiler_amd", "csrc"), str(src), "-o", exe],
+                   check=True)
+    return exe
+
+
+def test_overlap_of_rows_and_a_buffer(tmp_path):
+    """Against sets of bytes: rows that lie around the buffer share nothing with it."""
+    rng = random.Random(3)
+    cases = [(64 + rng.randrange(60), rng.randrange(20), 64 + rng.randrange(60), rng.randrange(5), rng.randrange(9), rng.randrange(24)) for _ in range(4000)]
+    want = ""
+    for o, length, r, n, b, s in cases:
+        rows = {r + i * s + q for i in range(n) for q in range(b)}
+        want += "1" if rows & set(range(o, o + length)) else "0"
+    got = subprocess.run([_overlap_program(tmp_path)], input="\n".join(" ".join(map(str, c)) for c in cases), capture_output=True, text=True, check=True).stdout
+    assert 400 < want.count("1") < 3600 and got == want
+
+
+def test_dispatch_refuses_shared_tensors():
+    torch = _torch()
+    from spnc import mixture as m
+    plan = m.Plan(torch.zeros(4, 1, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), torch.zeros(1, dtype=torch.int32), 4)
+    x = torch.zeros(9, 4)
+    ints = torch.zeros(12, dtype=torch.int32)
+    for rows, out in [(x[:4], x[:4]), (x[:4], x[3:7]), (x[2:6], x[:4]), (x[:4].t(), x[:4]), (ints[4:8].view(4, 1), ints[5:9].view(4, 1))]:
+        with pytest.raises(RuntimeError, match="must not share memory"):
+            m.dispatch(rows, plan, out=out)
+    shared = m.Plan(ints[:4].view(4, 1), ints[4:6], ints[6:7], 4)
+    for out in (ints[3:7].view(4, 1), ints[5:9].view(4, 1), ints[6:10].view(4, 1)):
+        with pytest.raises(RuntimeError, match="must not share memory"):
+            m.dispatch(torch.zeros(4, 1, dtype=torch.int32), shared, out=out)
+    with pytest.raises(RuntimeError, match="on a GPU"):                # beside each other is fine
+        m.dispatch(x[:4], plan, out=x[5:9])
+
+
+@pytest.mark.gpu
+def test_dispatch_beside_its_rows(native):
+    """Rows that are columns of a wider buffer, and a result that lies between or behind them."""
+    torch = _torch()
+    from spnc import mixture as m
+    base = torch.randn(4, 64, device="cuda")
+    want = base[:, :4].clone()
+    assert torch.equal(m.dispatch(base[:, :4], _plan(), out=base.view(-1)[32:48].view(4, 4)), want)      # in the first row's free part
+    with pytest.raises(RuntimeError, match="overlaps an input"):
+        m.dispatch(base[:, :4], _plan(), out=base.view(-1)[52:68].view(4, 4))                            # across the second row's beginning
+    with pytest.raises(RuntimeError, match="must not share memory"):
+        m.dispatch(base[:, :64], _plan(), out=base)
+    assert torch.equal(base[:, :4], want)
