@@ -8,7 +8,8 @@
  * All pointers are device pointers unless stated otherwise; every call enqueues on `stream` (a hipStream_t, NULL for
  * the default stream) of the current device and does not wait, allocates nothing, keeps no state between calls and
  * may be captured into a graph. Functions return 0 on success and a non-zero code on failure, with the message
- * available from spnc_hip_last_error(). Results do not depend on the order in which blocks run: no atomics on results. */
+ * available from spnc_hip_last_error(). What a call writes must not overlap what it reads or writes elsewhere, except where it is
+ * said; such calls are refused. Rows of one operand may lie between those of another. Results do not depend on the order in which blocks run: no atomics on results. */
 #ifndef SPNC_HIP_ROWS_H
 #define SPNC_HIP_ROWS_H
 
@@ -54,8 +55,8 @@ SPNC_HIP_API int spnc_hip_route(const int32_t* index, size_t slots, unsigned exp
 
 /* out[position[i * k + j]] = rows[i] for all slots with 0 <= position < capacity: rows of row_bytes bytes, stride_bytes apart in `rows`,
  * contiguous in `out` [capacity]. zero_unused != 0 clears the rows of `out` that belong to no segment (starts and counts
- * as spnc_hip_route wrote them); otherwise they are left as they were and starts and counts may be NULL. `out` must not overlap
- * what is read: such calls are refused. A row is shorter than 2 GiB, here and below. */
+ * as spnc_hip_route wrote them); otherwise they are left as they were and starts and counts may be NULL. A row is shorter
+ * than 2 GiB, here and below. */
 SPNC_HIP_API int spnc_hip_dispatch(const void* rows, size_t n, size_t row_bytes, size_t stride_bytes, const int32_t* position, unsigned k,
                                    size_t capacity, const int32_t* starts, const int32_t* counts, unsigned experts, int zero_unused, void* out,
                                    void* stream);
@@ -95,7 +96,7 @@ enum {
   SPNC_HIP_DROPOUT_MASK = 2     /* 0, kept elements stay as they are: the gradient of SPNC_HIP_DROPOUT_MARGINAL */
 };
 
-/* x [n, width] -> out [n, width], rows stride and out_stride elements apart; out may be x. Element e (counted without
+/* x [n, width] -> out [n, width], rows stride and out_stride elements apart; out may be x, with the same stride. Element e (counted without
  * the strides) is dropped where word e % 4 of Philox4x32-10 with key `seed` and counter (e / 4, offset), low words first,
  * is below round(p * 2^32). The mask is a function of seed, offset and e alone: the same call on the output's gradient
  * (ZERO, or MASK after MARGINAL) is the gradient. offset_device, if not NULL, points to the offset on the device and

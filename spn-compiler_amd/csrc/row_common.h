@@ -237,10 +237,28 @@ inline bool overlap(const void* out, size_t outBytes, const Span& in) {
   return behind < (in.stride ? in.rows : 1) && r + behind * in.stride < o + outBytes;
 }
 
-// Kernels read through __restrict__ pointers, and while others write: no output lies in an input.
-inline void checkApart(const char* what, const void* out, size_t outBytes, std::initializer_list<Span> inputs) {
-  for (const Span& in : inputs)
-    if (overlap(out, outBytes, in)) refuse(std::string(what) + ": the output overlaps an input");
+// contiguous memory
+inline Span block(const void* at, size_t bytes) { return {at, at ? 1u : 0u, bytes, 0}; }
+
+// whether rows of both share a byte; they may lie between each other
+inline bool overlap(const Span& a, const Span& b) {
+  if (a.rows == 0 || b.rows == 0 || a.bytes == 0 || b.bytes == 0) return false;
+  if (a.rows == 1 || b.rows == 1) return a.rows == 1 ? overlap(a.at, a.bytes, b) : overlap(b.at, b.bytes, a);
+  if (a.stride == b.stride && a.stride >= a.bytes && a.stride >= b.bytes) {
+    const Span &low = address(a.at) <= address(b.at) ? a : b, &high = &low == &a ? b : a;
+    const uintptr_t apart = address(high.at) - address(low.at), skip = apart / a.stride, rest = apart % a.stride;
+    return (skip < low.rows && rest < low.bytes) || (skip + 1 < low.rows && a.stride - rest < high.bytes);
+  }
+  if (!overlap(a.at, (a.rows - 1) * a.stride + a.bytes, b)) return false;
+  for (size_t i = 0; i < a.rows; ++i)
+    if (overlap(static_cast<const char*>(a.at) + i * a.stride, a.bytes, b)) return true;
+  return false;
+}
+
+// Kernels read through __restrict__ pointers, and while others write: no output lies in an input or in another output.
+inline void checkApart(const char* what, const Span& out, std::initializer_list<Span> others) {
+  for (const Span& other : others)
+    if (overlap(out, other)) refuse(std::string(what) + ": an output overlaps an input or another output");
 }
 
 inline void checkExperts(unsigned experts) {

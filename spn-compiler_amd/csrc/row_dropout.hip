@@ -110,6 +110,10 @@ int spnc_hip_dropout(const void* x, int dtype, size_t n, size_t width, size_t st
     if (n == 0 || width == 0) return;
     if (!x || !out) refuse("null argument");
     if ((address(x) | address(out)) % elementBytes(dtype)) refuse("dropout: pointers are not aligned to the element type");
+    const size_t bytes = elementBytes(dtype);
+    const Span read{x, n, width * bytes, stride * bytes}, written{out, n, width * bytes, out_stride * bytes};
+    if (x != out || (n > 1 && stride != out_stride)) checkApart("dropout", written, {read});  // in place every element is read by who writes it
+    checkApart("dropout", written, {block(offset_device, sizeof(uint64_t))});
     const uint64_t threshold = uint64_t(std::llrint(p * 4294967296.0));
     const double scale = mode != SPNC_HIP_DROPOUT_ZERO ? 1.0 : threshold >> 32 ? 0.0 : 1.0 / (1.0 - p);
     const double fill = mode == SPNC_HIP_DROPOUT_MARGINAL ? NAN : 0.0;

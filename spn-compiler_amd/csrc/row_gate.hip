@@ -407,6 +407,11 @@ int spnc_hip_gate(const void* logits, int dtype, size_t n, unsigned experts, siz
     if (n == 0) return;
     if (!logits || !index || !weight) refuse("null argument");
     if (address(logits) % elementBytes(dtype)) refuse("gate: pointers are not aligned to the element type");
+    const size_t bytes = elementBytes(dtype), slots = n * k;
+    const Span read{logits, n, experts * bytes, stride * bytes}, chosen = block(index, slots * sizeof(int32_t));
+    const Span weights = block(weight, slots * (bytes < sizeof(float) ? sizeof(float) : bytes));
+    checkApart("gate", chosen, {read, weights});
+    checkApart("gate", weights, {read});
     withType(dtype, [&](auto t) {
       using T = decltype(t);
       withGateShape<T>(n, experts, k, stride, address(logits), [&](auto g, auto v, auto layout) {
@@ -426,6 +431,10 @@ int spnc_hip_gate_backward(const void* logits, int dtype, size_t n, unsigned exp
     if (n == 0) return;
     if ((!logits && (flags & SPNC_HIP_GATE_ALL)) || !index || !weight || !grad_weight || !grad_logits) refuse("null argument");
     if ((address(logits) | address(grad_logits)) % elementBytes(dtype)) refuse("gate gradient: pointers are not aligned to the element type");
+    const size_t bytes = elementBytes(dtype), slots = n * k, weightBytes = slots * (bytes < sizeof(float) ? sizeof(float) : bytes);
+    checkApart("gate gradient", block(grad_logits, n * experts * bytes),
+               {{logits, (flags & SPNC_HIP_GATE_ALL) ? n : 0, experts * bytes, stride * bytes}, block(index, slots * sizeof(int32_t)),
+                block(weight, weightBytes), block(grad_weight, weightBytes)});
     withType(dtype, [&](auto t) {
       using T = decltype(t);
       using R = wide_t<T>;

@@ -693,6 +693,9 @@ void checkSegments(const int32_t* starts, const int32_t* counts, unsigned expert
   if (!starts || !counts) refuse("null argument");
 }
 
+Span startsBlock(const int32_t* starts, unsigned experts) { return block(starts, experts ? (size_t(experts) + 1) * sizeof(int32_t) : 0); }
+Span countsBlock(const int32_t* counts, unsigned experts) { return block(counts, experts * sizeof(int32_t)); }
+
 // calls fn(K, EXACT), see LogRow; K = 0 for more than eight. W: the widest type that is read or written k at a time.
 template <typename W, typename Fn>
 void withLogChoices(unsigned k, uintptr_t addresses, Fn&& fn) {
@@ -747,6 +750,12 @@ int spnc_hip_route(const int32_t* index, size_t slots, unsigned experts, unsigne
     const size_t need = spnc_hip_route_workspace(slots, experts);
     if (address(workspace) % sizeof(uint32_t)) refuse("the workspace must be aligned to 4 bytes");
     if (workspace_bytes < need || (need && !workspace)) refuse("the workspace must hold " + std::to_string(need) + " bytes");
+    const Span placed = block(position, slots * sizeof(int32_t)), begins = startsBlock(starts, experts), sizes = countsBlock(counts, experts);
+    const Span read = block(index, slots * sizeof(int32_t)), scratch = block(workspace, need);
+    checkApart("route", placed, {read, begins, sizes, scratch});
+    checkApart("route", begins, {read, sizes, scratch});
+    checkApart("route", sizes, {read, scratch});
+    checkApart("route", scratch, {read});
     unsigned bits = 0;
     while ((1u << bits) < experts) ++bits;
     const hipStream_t s = static_cast<hipStream_t>(stream);
@@ -777,9 +786,9 @@ int spnc_hip_dispatch(const void* rows, size_t n, size_t row_bytes, size_t strid
     if (zero_unused) checkSegments(starts, counts, experts);
     if (capacity == 0 || row_bytes == 0) return;
     if (!out || (n && (!rows || !position))) refuse("null argument");
-    checkApart("dispatch", out, capacity * row_bytes, {{rows, n, row_bytes, stride_bytes}, {position, 1, n * k * sizeof(int32_t), 0},
-                                                       {starts, zero_unused ? 1u : 0u, (experts + size_t(1)) * sizeof(int32_t), 0},
-                                                       {counts, zero_unused ? 1u : 0u, experts * sizeof(int32_t), 0}});
+    if (!zero_unused) experts = 0;  // the segments are not read
+    checkApart("dispatch", block(out, capacity * row_bytes),
+               {{rows, n, row_bytes, stride_bytes}, block(position, n * k * sizeof(int32_t)), startsBlock(starts, experts), countsBlock(counts, experts)});
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const unsigned piece = pieceBytes(1, {address(rows), address(out), row_bytes, stride_bytes});
     const RowShape shape = rowShape(n, row_bytes, piece, out, n < FEW_ROWS ? 8 : 6);
@@ -808,9 +817,12 @@ int spnc_hip_combine(const void* values, int dtype, size_t capacity, size_t widt
     if (width >> 31 || width * bytes >> 31) refuse("a row must be shorter than 2 GiB");
     if (n == 0 || width == 0) return;
     if ((capacity && !values) || !position || !out) refuse("null argument");
+    const Span read{values, capacity, width * bytes, stride * bytes};
     if (capacity == 0) values = out, stride = width;  // no slot is routed; there has to be a row to read and drop
     const unsigned piece = pieceBytes(unsigned(bytes), {address(values), address(out), width * bytes, stride * bytes});
     checkAligned(piece, "combine");
+    checkApart("combine", block(out, n * width * bytes),
+               {read, block(position, n * k * sizeof(int32_t)), block(weight, weight ? n * k * elementBytes(weight_dtype) : 0)});
     const RowShape shape = rowShape(n, width * bytes, piece, nullptr, n < FEW_ROWS ? 8 : 6);
     withType(dtype, [&](auto t) {
       using T = decltype(t);
@@ -848,6 +860,13 @@ int spnc_hip_combine_backward(const void* values, int dtype, size_t capacity, si
     const unsigned piece = pieceBytes(unsigned(bytes), {address(values), address(grad_out), address(grad_values), width * bytes, stride * bytes,
                                                         grad_stride * bytes});
     checkAligned(piece, "combine gradient");
+    const size_t weightBytes = n * k * elementBytes(weight_dtype);
+    const Span toValues = block(grad_values, capacity * width * bytes), toWeight = block(grad_weight, weightBytes);
+    const Span read{values, grad_weight ? capacity : 0, width * bytes, stride * bytes}, gradient{grad_out, n, width * bytes, grad_stride * bytes};
+    const Span slots = block(position, n * k * sizeof(int32_t)), weights = block(weight, weightBytes);
+    const Span begins = startsBlock(starts, grad_values ? experts : 0), sizes = countsBlock(counts, grad_values ? experts : 0);
+    checkApart("combine gradient", toValues, {read, gradient, slots, weights, begins, sizes, toWeight});
+    checkApart("combine gradient", toWeight, {read, gradient, slots, weights, begins, sizes});
     const RowShape shape = rowShape(n, width * bytes, piece, grad_values);
     const Unused unused = unusedRows(tileGrid(shape.tiles), starts, counts, experts, capacity, width * bytes, grad_values);
     if (unused.rowBlocks + unused.blocks == 0) return;
@@ -878,6 +897,11 @@ int spnc_hip_combine_log(const void* values, int dtype, size_t capacity, const i
     checkSlots(n, k, capacity);
     if (n == 0) return;
     if ((capacity && !values) || !position || !log_weight || !out) refuse("null argument");
+    const size_t bytes = elementBytes(dtype);
+    const Span read = block(values, capacity * bytes), slots = block(position, n * k * sizeof(int32_t));
+    const Span weights = block(log_weight, n * k * elementBytes(weight_dtype)), shares = block(share, n * k * bytes);
+    checkApart("combine_log", block(out, n * bytes), {read, slots, weights, shares});
+    checkApart("combine_log", shares, {read, slots, weights});
     if (capacity == 0) values = out;  // no slot is routed; there has to be a value to read and drop
     const hipStream_t s = static_cast<hipStream_t>(stream);
     withLogTypes(dtype, weight_dtype, [&](auto r, auto w) {
@@ -909,7 +933,13 @@ int spnc_hip_combine_log_backward(const void* share, int dtype, size_t capacity,
     const hipStream_t s = static_cast<hipStream_t>(stream);
     if (!grad_values && !grad_log_weight) return;
     if (n && (!share || (grad_values && !position) || !grad_out)) refuse("null argument");
-    const Unused unused = unusedRows(logGrid(n, k), starts, counts, experts, capacity, elementBytes(dtype), grad_values);
+    const size_t bytes = elementBytes(dtype);
+    const Span toValues = block(grad_values, capacity * bytes), toWeight = block(grad_log_weight, n * k * elementBytes(weight_dtype));
+    const Span read = block(share, n * k * bytes), gradient = block(grad_out, n * bytes), slots = block(position, grad_values ? n * k * sizeof(int32_t) : 0);
+    const Span begins = startsBlock(starts, grad_values ? experts : 0), sizes = countsBlock(counts, grad_values ? experts : 0);
+    checkApart("combine_log gradient", toValues, {read, gradient, slots, begins, sizes, toWeight});
+    checkApart("combine_log gradient", toWeight, {read, gradient, slots, begins, sizes});
+    const Unused unused = unusedRows(logGrid(n, k), starts, counts, experts, capacity, bytes, grad_values);
     if (unused.rowBlocks + unused.blocks == 0) return;
     withLogTypes(dtype, weight_dtype, [&](auto r, auto w) {
       using R = decltype(r);

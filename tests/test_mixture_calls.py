@@ -156,6 +156,66 @@ def test_overlap_of_rows_and_a_buffer(tmp_path):
     assert 400 < want.count("1") < 3600 and got == want
 
 
+def test_overlap_of_rows_and_rows(tmp_path):
+    src = tmp_path / "o.hip"
+    src.write_text('#include <cstdio>\n#include "row_common.h"\nstd::string& spnc_hip::lastError() { static std::string s; return s; }\n'
+                   'int main() { size_t v[8]; while (scanf("%zu %zu %zu %zu %zu %zu %zu %zu", v, v + 1, v + 2, v + 3, v + 4, v + 5, v + 6, v + 7) == 8)'
+                   ' putchar(spnc_hip::overlap({reinterpret_cast<void*>(v[0]), v[1], v[2], v[3]}, {reinterpret_cast<void*>(v[4]), v[5], v[6], v[7]}) ? \'1\' : \'0\'); }\n')
+    exe = str(tmp_path / "o")
+    subprocess.run(["/opt/rocm/bin/hipcc", "--offload-arch=gfx950", "-std=c++17", "-Wno-unused-function", "-I", os.path.join(ROOT, "spn-compiler_amd", "csrc"), str(src), "-o", exe],
+                   check=True)
+    rng, cases, want = random.Random(4), [], ""
+    for i in range(6000):
+        a, b = [(64 + rng.randrange(70), rng.randrange(6), rng.randrange(7), rng.randrange(20)) for _ in range(2)]
+        if i % 2:
+            b = b[:3] + (a[3],)                                  # equal strides have a formula of their own
+        cases.append(a + b)
+        x, y = [{at + i * step + q for i in range(n) for q in range(width)} for at, n, width, step in (a, b)]
+        want += "1" if x & y else "0"
+    got = subprocess.run([exe], input="\n".join(" ".join(map(str, c)) for c in cases), capture_output=True, text=True, check=True).stdout
+    assert 600 < want.count("1") < 5400 and got == want
+
+
+def test_c_entry_points_refuse_to_write_where_they_read(native):
+    """Every output on top of every input and of every other output, at the first and at the last byte; addresses that nobody reads."""
+    lib = native._load()
+    n, k, experts, width, capacity = 6, 2, 4, 8, 12
+    slots = n * k
+    # name: (pointers in the order of the call: bytes and whether written), the call with their addresses
+    calls = {
+        "gate": ([(n * experts * 4, 0), (slots * 4, 1), (slots * 4, 1)], lambda z, i, w: lib.spnc_hip_gate(z, 0, n, experts, experts, k, 0, i, w, None)),
+        "gate gradient": ([(n * experts * 2, 0), (slots * 4, 0), (slots * 4, 0), (slots * 4, 0), (n * experts * 2, 1)],
+                          lambda z, i, w, g, o: lib.spnc_hip_gate_backward(z, 2, n, experts, experts, k, 1, i, w, g, o, None)),
+        "route": ([(20000 * 4, 0), (20000 * 4, 1), (20, 1), (16, 1), (lib.spnc_hip_route_workspace(20000, experts), 1)],
+                  lambda i, p, s, c, w: lib.spnc_hip_route(i, 20000, experts, 1, p, s, c, w, 1 << 20, None)),
+        "dispatch": ([(n * 32, 0), (slots * 4, 0), (20, 0), (16, 0), (capacity * 32, 1)],
+                     lambda x, p, s, c, o: lib.spnc_hip_dispatch(x, n, 32, 32, p, k, capacity, s, c, experts, 1, o, None)),
+        "combine": ([(capacity * width * 4, 0), (slots * 4, 0), (slots * 4, 0), (n * width * 4, 1)],
+                    lambda v, p, w, o: lib.spnc_hip_combine(v, 0, capacity, width, width, p, n, k, w, 0, o, None)),
+        "combine gradient": ([(capacity * width * 8, 0), (slots * 4, 0), (slots * 8, 0), (n * width * 8, 0), (20, 0), (16, 0), (capacity * width * 8, 1), (slots * 8, 1)],
+                             lambda v, p, w, g, s, c, gv, gw: lib.spnc_hip_combine_backward(v, 1, capacity, width, width, p, n, k, w, 1, g, width, s, c, experts, gv, gw, None)),
+        "combine_log": ([(capacity * 8, 0), (slots * 4, 0), (slots * 4, 0), (n * 8, 1), (slots * 8, 1)],
+                        lambda v, p, w, o, s: lib.spnc_hip_combine_log(v, 1, capacity, p, n, k, w, 0, o, s, None)),
+        "combine_log gradient": ([(slots * 4, 0), (slots * 4, 0), (n * 4, 0), (20, 0), (16, 0), (capacity * 4, 1), (slots * 8, 1)],
+                                 lambda h, p, g, s, c, gv, gw: lib.spnc_hip_combine_log_backward(h, 0, capacity, p, n, k, 1, g, s, c, experts, gv, gw, None)),
+        "dropout": ([(n * width * 4, 0), (n * width * 4, 1), (8, 0)], lambda x, o, at: lib.spnc_hip_dropout(x, 0, n, width, width, o, width, 0.5, 0, 1, 0, at, None)),
+    }
+    for name, (sizes, call) in calls.items():
+        for out, (out_bytes, written) in enumerate(sizes):
+            for other, (bytes_, _) in enumerate(sizes):
+                if not written or other == out:
+                    continue
+                for shift in (8 - out_bytes, 0, bytes_ // 8 * 8 - (8 if bytes_ % 8 == 0 else 0)):
+                    if name == "dropout" and other == 0 and shift == 0:
+                        continue                                   # in place is allowed
+                    addresses = [(1 << 20) * (i + 1) for i in range(len(sizes))]
+                    addresses[out] = addresses[other] + shift
+                    rc = call(*[ctypes.c_void_p(a) for a in addresses])
+                    _refused(lib, rc, name + ": an output overlaps")
+    p = ctypes.c_void_p
+    _refused(lib, lib.spnc_hip_dropout(p(1 << 20), 0, n, width, 16, p(1 << 20), 24, 0.5, 0, 1, 0, None, None), "overlaps")     # in place, other strides
+
+
 def test_dispatch_refuses_shared_tensors():
     torch = _torch()
     from spnc import mixture as m
@@ -186,3 +246,17 @@ def test_dispatch_beside_its_rows(native):
     with pytest.raises(RuntimeError, match="must not share memory"):
         m.dispatch(base[:, :64], _plan(), out=base)
     assert torch.equal(base[:, :4], want)
+
+
+@pytest.mark.gpu
+def test_dropout_between_its_rows_and_in_place(native):
+    """Through the C-ABI: the left half of a buffer's columns into the right half, and onto itself."""
+    torch = _torch()
+    from spnc import mixture as m
+    lib, p = native._load(), ctypes.c_void_p
+    base = torch.randn(300, 16, device="cuda")
+    want = m.dropout(base[:, :8], 0.4, 9, marginal=True).nan_to_num(7.0)
+    stream = p(torch.cuda.current_stream().cuda_stream)
+    for out in (base[:, 8:], base[:, :8]):
+        assert lib.spnc_hip_dropout(p(base.data_ptr()), 0, 300, 8, 16, p(out.data_ptr()), 16, 0.4, 1, 9, 0, None, stream) == 0
+        assert torch.equal(out.nan_to_num(7.0), want)
