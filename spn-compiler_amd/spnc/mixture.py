@@ -183,11 +183,12 @@ class Mixture:
 
     def execute(self, rows, plan):
         """Log-likelihoods [plan.capacity] of sorted rows, each segment under its kernel; rows of no segment stay undefined.
-        Waits for the plan: the host needs the segments' sizes to launch the kernels."""
+        Kernels have no gradient with respect to their features: rows that want one are refused. Waits for the plan: the host needs the segments' sizes to launch the kernels."""
         _refuse(tuple(rows.shape) != (plan.capacity, self.num_features) or not rows.is_contiguous(),
                 f"Sorted rows must be contiguous with shape {(plan.capacity, self.num_features)}, got {tuple(rows.shape)}")
         _refuse(plan.experts != len(self.kernels), f"The plan is for {plan.experts} experts, the mixture has {len(self.kernels)}")
         self._check_type(rows)
+        self._check_derivatives(rows)
         device = rows.device
         _refuse(device.type != "cuda" or any(t.device != device for t in (plan.position, plan.starts, plan.counts)),
                 f"Rows and plan must be on one GPU, got {device} and {plan.position.device}")
@@ -216,6 +217,10 @@ class Mixture:
                     lanes[0].wait_stream(lane)
         return values
 
+    @staticmethod
+    def _check_derivatives(rows):
+        _refuse(torch.is_grad_enabled() and rows.requires_grad, "Compiled kernels have no gradient with respect to their features")
+
     def _check_type(self, rows):
         kind = rows.dtype.is_floating_point
         _refuse(rows.element_size() != self._feature_bytes or kind != self._feature_is_float or rows.dtype in (torch.bool, torch.bfloat16, torch.float16)
@@ -232,7 +237,7 @@ class Mixture:
         _refuse(logits.dim() != 2 or tuple(logits.shape) != (rows.shape[0], len(self.kernels)),
                 f"Logits must have shape [{rows.shape[0]}, {len(self.kernels)}], got {tuple(logits.shape)}")
         self._check_type(rows)
-        _refuse(torch.is_grad_enabled() and rows.requires_grad, "Compiled kernels have no gradient with respect to their features")
+        self._check_derivatives(rows)
         _refuse(rows.device.type != "cuda" or logits.device != rows.device, f"Rows and logits must be on one GPU, got {rows.device} and {logits.device}")
         index, log_weights = gate(logits, k, over=over, log=True)
         plan = route(index, len(self.kernels), align=self._align)

@@ -260,3 +260,40 @@ def test_dropout_between_its_rows_and_in_place(native):
     for out in (base[:, 8:], base[:, :8]):
         assert lib.spnc_hip_dropout(p(base.data_ptr()), 0, 300, 8, 16, p(out.data_ptr()), 16, 0.4, 1, 9, 0, None, stream) == 0
         assert torch.equal(out.nan_to_num(7.0), want)
+
+
+# ---- derivatives that are not offered -------------------------------------------------------------------------------
+
+def test_kernels_refuse_rows_that_want_a_gradient(mix):
+    """In the step-by-step form too, whose rows come out of a differentiable dispatch; without a graph they are rows like others."""
+    torch = _torch()
+    from spnc import mixture as m
+    plan = m.Plan(torch.zeros(3, 1, dtype=torch.int32), torch.zeros(3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), 3)
+    x = torch.zeros(3, 6, requires_grad=True)
+    for rows in (x, x * 2.0):
+        with pytest.raises(RuntimeError, match="no gradient with respect to their features"):
+            mix.execute(rows, plan)
+        with pytest.raises(RuntimeError, match="no gradient with respect to their features"):
+            mix.log_likelihood(rows, torch.zeros(3, 2), 1)
+        with pytest.raises(RuntimeError, match="on one GPU"), torch.no_grad():
+            mix.execute(rows, plan)
+        with pytest.raises(RuntimeError, match="on one GPU"):
+            mix.execute(rows.detach(), plan)
+
+
+@pytest.mark.gpu
+def test_kernels_step_by_step(mix):
+    torch = _torch()
+    from spnc import mixture as m
+    x, z = torch.randn(50, 6, device="cuda"), torch.randn(50, 2, device="cuda", requires_grad=True)
+    index, log_weights = m.gate(z, 2, log=True)
+    plan = m.route(index, 2, align=4)
+    got = m.combine_log(mix.execute(m.dispatch(x, plan), plan), plan, log_weights)
+    want = mix.log_likelihood(x, z, 2)
+    assert torch.equal(got, want)
+    assert torch.equal(torch.autograd.grad(got.sum(), z)[0], torch.autograd.grad(want.sum(), z)[0])
+    leaf = x.clone().requires_grad_()
+    with pytest.raises(RuntimeError, match="no gradient with respect to their features"):
+        mix.execute(m.dispatch(leaf, plan), plan)
+    with torch.no_grad():
+        assert torch.equal(m.combine_log(mix.execute(m.dispatch(leaf, plan), plan), plan, log_weights), want)
