@@ -3,8 +3,11 @@
 // C-ABI. In C++ because a call of a few microseconds of GPU time is otherwise dominated by the interpreter, twice so where
 // the backward pass runs on PyTorch's own thread.
 #include <ATen/MemoryOverlap.h>
+#include <c10/core/AutogradState.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include "../../include/spnc_hip_rows.h"
@@ -52,6 +55,17 @@ bool wantsGrad(std::initializer_list<const Tensor*> tensors) {
   for (const Tensor* t : tensors)
     if (t->defined() && t->requires_grad()) return true;
   return false;
+}
+
+// The kernels are reached without PyTorch's dispatcher, so what it would do on the way is not done: a tangent would be dropped, and a trace
+// would hold the allocation of a result that nothing computes. Such calls are refused.
+void checkRecorded(std::initializer_list<const Tensor*> tensors) {
+  using c10::impl::TorchDispatchModeKey;
+  using c10::impl::TorchDispatchModeTLS;
+  refuse(torch::jit::tracer::isTracing() || (TorchDispatchModeTLS::any_modes_set() && TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY).has_value()),
+         "spnc.mixture cannot be traced");
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : tensors) refuse(t->defined() && t->_fw_grad(0).defined(), "spnc.mixture has no forward-mode derivatives");
 }
 
 // Views of a conjugate's imaginary part, which autograd hands out as gradients too, hold their numbers with the other sign. Memory that
@@ -138,6 +152,7 @@ struct Gate : torch::autograd::Function<Gate> {
     return {index, weight};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    checkRecorded({&grads[1]});
     const auto saved = ctx->get_saved_variables();
     const Tensor &index = saved[1], &weight = saved[2];
     c10::DeviceGuard guard(index.device());
@@ -157,6 +172,7 @@ std::pair<Tensor, Tensor> gate(const Tensor& logits, int64_t k, int64_t flags) {
   const int64_t experts = logits.size(1), most = std::min<int64_t>(experts, SPNC_HIP_MAX_CHOICES);
   checkExperts(experts);
   refuse(k < 1 || k > most, "k must be between 1 and ", most, ", got ", k);
+  checkRecorded({&logits});
   onGpu({&logits});
   if (!wantsGrad({&logits})) return gateForward(logits, k, flags);
   auto r = Gate::apply(logits, k, flags);
@@ -173,6 +189,7 @@ std::tuple<Tensor, Tensor, Tensor, int64_t> route(const Tensor& given, int64_t e
   const int64_t slots = given.numel();
   refuse(slots >= ROWS_LIMIT || align > ROWS_LIMIT || slots + experts * (align - 1) >= ROWS_LIMIT, slots, " slots and ", experts, " segments aligned to ",
          align, " rows exceed 2^31 rows");
+  checkRecorded({});
   onGpu({&given});
   c10::DeviceGuard guard(given.device());
   const Tensor index = given.contiguous();
@@ -222,6 +239,7 @@ struct Dispatch : torch::autograd::Function<Dispatch> {
     return dispatchForward(rows, plan, Tensor(), true);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    checkRecorded({&grads[0]});
     return once({combineForward(grads[0], savedPlan(ctx, ctx->get_saved_variables()), Tensor()), Tensor()});
   }
 };
@@ -232,7 +250,9 @@ Tensor dispatch(const Tensor& rows, const Tensor& position, const Tensor& starts
   refuse(rows.dim() != 2, "Rows must have shape [rows, width], got ", rows.sizes());
   refuse(rows.size(0) != plan.rows(), "The plan is for ", plan.rows(), " rows, got ", rows.size(0));
   refuse(rows.element_size() > 8 || rows.is_complex(), "Rows of ", rows.scalar_type(), " are not supported");
+  checkRecorded({&rows});
   if (result) {
+    checkRecorded({&*result});
     refuse(result->dim() != 2 || result->size(0) != capacity || result->size(1) != rows.size(1) || result->scalar_type() != rows.scalar_type() ||
                !result->is_contiguous() || result->is_neg(),
            "out must be a contiguous ", rows.scalar_type(), " tensor of shape [", capacity, ", ", rows.size(1), "]");
@@ -262,6 +282,7 @@ struct Combine : torch::autograd::Function<Combine> {
     return combineForward(values, plan, weights);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    checkRecorded({&grads[0]});
     const auto saved = ctx->get_saved_variables();
     const Plan plan = savedPlan(ctx, saved);
     const Tensor& weights = saved[1];
@@ -289,8 +310,10 @@ Tensor combine(const Tensor& values, const Tensor& position, const Tensor& start
   const Plan plan = planOf(position, starts, counts, capacity);
   refuse(values.dim() != 2 || values.size(0) != capacity, "Values must have shape [", capacity, ", width], got ", values.sizes());
   refuse(elementType(values.scalar_type()) < 0, "Values must be float32, float64, float16 or bfloat16, got ", values.scalar_type());
+  checkRecorded({&values});
   Tensor weights;
   if (given) {
+    checkRecorded({&*given});
     checkWeights(*given, plan, values.scalar_type() == at::kDouble);
     onGpu({&values, &position, &starts, &counts, &*given});
     weights = flat(*given);
@@ -319,6 +342,7 @@ struct CombineLog : torch::autograd::Function<CombineLog> {
     return combineLogForward(values, plan, weights, share);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    checkRecorded({&grads[0]});
     const auto saved = ctx->get_saved_variables();
     const Plan plan = savedPlan(ctx, saved);
     const Tensor& share = saved[0];
@@ -340,6 +364,7 @@ Tensor combineLog(const Tensor& given, const Tensor& position, const Tensor& sta
   refuse(given.dim() != 1 || given.size(0) != capacity, "Values must have shape [", capacity, "], got ", given.sizes());
   refuse(given.scalar_type() != at::kFloat && given.scalar_type() != at::kDouble, "Values must be float32 or float64, got ", given.scalar_type());
   checkWeights(logWeights, plan, true);
+  checkRecorded({&given, &logWeights});
   onGpu({&given, &position, &starts, &counts, &logWeights});
   const Tensor values = flat(given), weights = flat(logWeights);
   if (!wantsGrad({&values, &weights})) return combineLogForward(values, plan, weights, Tensor());
@@ -375,6 +400,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
     return dropoutForward(x, mask);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    checkRecorded({&grads[0]});
     const auto saved = ctx->get_saved_variables();
     const int64_t mode = ctx->saved_data["mode"].toInt();
     const Mask mask{ctx->saved_data["p"].toDouble(), mode == SPNC_HIP_DROPOUT_MARGINAL ? int64_t(SPNC_HIP_DROPOUT_MASK) : mode,
@@ -385,6 +411,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
 
 Tensor dropout(const Tensor& x, double p, uint64_t seed, uint64_t offset, const std::optional<Tensor>& offsetDevice, bool marginal) {
   refuse(elementType(x.scalar_type()) < 0, "x must be float32, float64, float16 or bfloat16, got ", x.scalar_type());
+  checkRecorded({&x});
   Mask mask{p, marginal ? SPNC_HIP_DROPOUT_MARGINAL : SPNC_HIP_DROPOUT_ZERO, seed, offset, Tensor()};
   if (offsetDevice) {
     refuse(offsetDevice->scalar_type() != at::kLong || offsetDevice->numel() != 1, "An offset on the device must be a one-element int64 tensor");
@@ -400,6 +427,7 @@ Tensor dropout(const Tensor& x, double p, uint64_t seed, uint64_t offset, const 
 }  // namespace
 
 PYBIND11_MODULE(_mixture_ops, m) {
+  m.def("check_recorded", [](const Tensor& t) { checkRecorded({&t}); });
   m.def("gate", &gate);
   m.def("route", &route);
   m.def("check_plan", [](const Tensor& position, const Tensor& starts, const Tensor& counts, int64_t capacity) { planOf(position, starts, counts, capacity); });

@@ -8,8 +8,9 @@ activations) bring the experts' results back in row order with the weights appli
 compiled kernels; ``HIPCompiler.compile_mixture`` builds one.
 
 All take and return torch tensors on the GPU, run on the current stream, and have gradients where their inputs are
-floating point (first order: a gradient cannot be differentiated again). Results do not change from run to run. Bad
-arguments raise ``RuntimeError``. There is no CPU path.
+floating point (first order: a gradient cannot be differentiated again; there are no forward-mode derivatives). Results do
+not change from run to run. Bad arguments raise ``RuntimeError``, and so do calls under ``torch.jit.trace`` or ``make_fx``, which
+would record nothing of them. There is no CPU path.
 """
 import math
 
@@ -184,11 +185,11 @@ class Mixture:
     def execute(self, rows, plan):
         """Log-likelihoods [plan.capacity] of sorted rows, each segment under its kernel; rows of no segment stay undefined.
         Kernels have no gradient with respect to their features: rows that want one are refused. Waits for the plan: the host needs the segments' sizes to launch the kernels."""
+        self._check_derivatives(rows)
         _refuse(tuple(rows.shape) != (plan.capacity, self.num_features) or not rows.is_contiguous(),
                 f"Sorted rows must be contiguous with shape {(plan.capacity, self.num_features)}, got {tuple(rows.shape)}")
         _refuse(plan.experts != len(self.kernels), f"The plan is for {plan.experts} experts, the mixture has {len(self.kernels)}")
         self._check_type(rows)
-        self._check_derivatives(rows)
         device = rows.device
         _refuse(device.type != "cuda" or any(t.device != device for t in (plan.position, plan.starts, plan.counts)),
                 f"Rows and plan must be on one GPU, got {device} and {plan.position.device}")
@@ -220,6 +221,7 @@ class Mixture:
     @staticmethod
     def _check_derivatives(rows):
         _refuse(torch.is_grad_enabled() and rows.requires_grad, "Compiled kernels have no gradient with respect to their features")
+        _ops().check_recorded(rows)
 
     def _check_type(self, rows):
         kind = rows.dtype.is_floating_point
@@ -233,11 +235,12 @@ class Mixture:
         rows   : [n, features] of the kernels' feature type.
         logits : [n, kernels] of the gate, see ``gate`` for ``k`` and ``over``.
         """
+        self._check_derivatives(rows)
+        _ops().check_recorded(logits)
         _refuse(rows.dim() != 2 or rows.shape[1] != self.num_features, f"Rows must have shape [rows, {self.num_features}], got {tuple(rows.shape)}")
         _refuse(logits.dim() != 2 or tuple(logits.shape) != (rows.shape[0], len(self.kernels)),
                 f"Logits must have shape [{rows.shape[0]}, {len(self.kernels)}], got {tuple(logits.shape)}")
         self._check_type(rows)
-        self._check_derivatives(rows)
         _refuse(rows.device.type != "cuda" or logits.device != rows.device, f"Rows and logits must be on one GPU, got {rows.device} and {logits.device}")
         index, log_weights = gate(logits, k, over=over, log=True)
         plan = route(index, len(self.kernels), align=self._align)

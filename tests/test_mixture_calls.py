@@ -297,3 +297,69 @@ def test_kernels_step_by_step(mix):
         mix.execute(m.dispatch(leaf, plan), plan)
     with torch.no_grad():
         assert torch.equal(m.combine_log(mix.execute(m.dispatch(leaf, plan), plan), plan, log_weights), want)
+
+
+def _calls(mix, device):
+    """(call, a floating-point tensor it takes) of everything that takes one."""
+    torch = _torch()
+    from spnc import mixture as m
+    i32 = dict(dtype=torch.int32, device=device)
+    plan = m.Plan(torch.arange(3, **i32)[:, None], torch.tensor([0, 3, 3], **i32), torch.tensor([3, 0], **i32), 3)
+    x, v, w, z = (torch.rand(shape, device=device) for shape in ((3, 6), (3,), (3, 1), (3, 2)))
+    return [(lambda t: m.gate(t, 2)[1], z), (lambda t: m.gate(t, 1, over="all", log=True)[1], z), (lambda t: m.dispatch(t, plan), x),
+            (lambda t: m.dispatch(t, plan, out=torch.empty_like(x)), x), (lambda t: m.dispatch(x, plan, out=t), x.clone()), (lambda t: m.combine(t, plan), x),
+            (lambda t: m.combine(t, plan, w), x), (lambda t: m.combine(x, plan, t), w), (lambda t: m.combine_log(t, plan, w), v), (lambda t: m.combine_log(v, plan, t), w),
+            (lambda t: m.dropout(t, 0.5, 1), x), (lambda t: m.dropout(t, 0.5, 1, marginal=True), x), (lambda t: mix.execute(t, plan), x),
+            (lambda t: mix.log_likelihood(t, z, 1), x), (lambda t: mix.log_likelihood(x, t, 1), z)]
+
+
+def test_tangents_and_traces_are_refused(mix):
+    """Before anything reaches the GPU; the same calls without a tangent or a trace get as far as the device check."""
+    torch = _torch()
+    from spnc import mixture as m
+    from torch.autograd import forward_ad
+    from torch.fx.experimental.proxy_tensor import make_fx
+    for f, t in _calls(mix, "cpu"):
+        with pytest.raises(RuntimeError, match="on (a|one) GPU"):
+            f(t)
+        with forward_ad.dual_level():
+            with pytest.raises(RuntimeError, match="on (a|one) GPU"):
+                f(t)
+            dual = forward_ad.make_dual(t, torch.ones_like(t))
+            for _ in range(2):
+                with pytest.raises(RuntimeError, match="no forward-mode derivatives"):
+                    f(dual)
+            with torch.no_grad(), pytest.raises(RuntimeError, match="no forward-mode derivatives"):       # tangents pass through this
+                f(dual)
+            with pytest.raises(RuntimeError, match="on (a|one) GPU"):
+                f(forward_ad.unpack_dual(dual).primal)
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            torch.jit.trace(f, (t,))
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            make_fx(f, tracing_mode="real")(t)
+    index = torch.zeros(3, 1, dtype=torch.int32)
+    with pytest.raises(RuntimeError, match="cannot be traced"):
+        torch.jit.trace(lambda t: m.route(t, 2).position, (index,))
+    with pytest.raises(RuntimeError, match="on a GPU"):
+        m.route(index, 2)
+
+
+@pytest.mark.gpu
+def test_tangents_of_gradients_are_refused(mix):
+    """A backward pass whose incoming gradient has a tangent; wrapped tensors (torch.func) are refused by PyTorch."""
+    torch = _torch()
+    from torch.autograd import forward_ad
+    differentiable = [c for i, c in enumerate(_calls(mix, "cuda")) if i not in (3, 4, 12, 13)]
+    for i, (f, t) in enumerate(differentiable):
+        leaf = t.clone().requires_grad_()
+        out = f(leaf)
+        want, = torch.autograd.grad(out, leaf, torch.ones_like(out), retain_graph=True)
+        with forward_ad.dual_level():
+            dual = forward_ad.make_dual(torch.ones_like(out), torch.ones_like(out))
+            with pytest.raises(RuntimeError, match="no forward-mode derivatives"):
+                torch.autograd.grad(out, leaf, dual, retain_graph=True)
+            got, = torch.autograd.grad(out, leaf, torch.ones_like(out))
+        assert torch.equal(got, want), i
+        for transform in (lambda: torch.vmap(f)(t[None]), lambda: torch.func.grad(lambda a: f(a).sum())(t), lambda: torch.func.jvp(f, (t,), (torch.ones_like(t),))):
+            with pytest.raises(RuntimeError):
+                transform()
