@@ -5,11 +5,13 @@
  * applied. Dropout marks features as missing for kernels compiled with marginalisation, or zeroes and scales activations.
  * The reference compiles one query at a time and has no counterpart of these.
  *
- * All pointers are device pointers unless stated otherwise; every call enqueues on `stream` (a hipStream_t, NULL for
- * the default stream) of the current device and does not wait, allocates nothing, keeps no state between calls and
- * may be captured into a graph. Functions return 0 on success and a non-zero code on failure, with the message
- * available from spnc_hip_last_error(). What a call writes must not overlap what it reads or writes elsewhere, except where it is
- * said; such calls are refused. Rows of one operand may lie between those of another. Results do not depend on the order in which blocks run: no atomics on results. */
+ * All pointers are device pointers unless stated otherwise, aligned to their elements; every call enqueues on `stream` (a
+ * hipStream_t, NULL for the default stream) of the current device and does not wait, allocates nothing, keeps no state
+ * between calls and may be captured into a graph. What a call writes must not overlap what it reads or writes elsewhere,
+ * except where it is said; such calls are refused. Rows of one operand may lie between those of another. Functions
+ * return 0 on success and a non-zero code on failure, with the message available from spnc_hip_last_error(); an error that
+ * another call left for hipGetLastError is neither read nor cleared. Results do not depend on the order in which blocks
+ * run: no atomics on results. */
 #ifndef SPNC_HIP_ROWS_H
 #define SPNC_HIP_ROWS_H
 

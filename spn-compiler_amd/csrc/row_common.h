@@ -8,6 +8,7 @@
 #include <initializer_list>
 #include <stdexcept>
 #include <string>
+#include <tuple>
 #include <type_traits>
 
 #include "../../include/spnc_hip_rows.h"
@@ -175,16 +176,23 @@ __device__ inline double logOf(double x) { return log(x); }
 
 [[noreturn]] inline void refuse(const std::string& what) { throw std::runtime_error(what); }
 
-// guarded() for entry points that launch: an error that someone else left behind is not this call's.
-template <typename Fn>
-int launching(Fn&& fn) {
+// Calls of the runtime return their own status, and what others left to be read by hipGetLastError is neither read nor cleared. An error
+// of one's own replaces that, so it is taken back: it is reported here.
+inline void checkCall(const char* what, hipError_t e) {
+  if (e == hipSuccess) return;
   (void)hipGetLastError();
-  return guarded(fn);
+  refuse(std::string(what) + " launch: " + hipGetErrorString(e));
 }
 
-inline void launched(const char* what) {
-  const hipError_t e = hipGetLastError();
-  if (e != hipSuccess) refuse(std::string(what) + " launch: " + hipGetErrorString(e));
+template <typename... P, typename... A>
+void launch(const char* what, void (*kernel)(P...), unsigned grid, unsigned blockSize, size_t lds, void* stream, const A&... given) {
+  std::tuple<P...> parameters(given...);
+  std::apply(
+      [&](P&... p) {
+        void* pointers[] = {const_cast<void*>(static_cast<const void*>(&p))...};
+        checkCall(what, hipLaunchKernel(reinterpret_cast<const void*>(kernel), dim3(grid), dim3(blockSize), pointers, lds, static_cast<hipStream_t>(stream)));
+      },
+      parameters);
 }
 
 inline size_t elementBytes(int dtype) {

@@ -102,7 +102,7 @@ extern "C" {
 
 int spnc_hip_dropout(const void* x, int dtype, size_t n, size_t width, size_t stride, void* out, size_t out_stride, double p, int mode,
                      uint64_t seed, uint64_t offset, const uint64_t* offset_device, void* stream) {
-  return launching([&] {
+  return guarded([&] {
     elementBytes(dtype);
     if (!(p >= 0.0 && p <= 1.0)) refuse("the probability of dropping an element must be between 0 and 1");
     if (mode < SPNC_HIP_DROPOUT_ZERO || mode > SPNC_HIP_DROPOUT_MASK) refuse("unknown dropout mode " + std::to_string(mode));
@@ -117,29 +117,26 @@ int spnc_hip_dropout(const void* x, int dtype, size_t n, size_t width, size_t st
     const uint64_t threshold = uint64_t(std::llrint(p * 4294967296.0));
     const double scale = mode != SPNC_HIP_DROPOUT_ZERO ? 1.0 : threshold >> 32 ? 0.0 : 1.0 / (1.0 - p);
     const double fill = mode == SPNC_HIP_DROPOUT_MARGINAL ? NAN : 0.0;
-    const hipStream_t s = static_cast<hipStream_t>(stream);
     withType(dtype, [&](auto t) {
       using T = decltype(t);
       using R = wide_t<T>;
       const Dropout<R> d{uint32_t(threshold - 1), threshold == 0, R(scale), R(fill), seed, offset, offset_device};
       const uintptr_t bits = address(x) | address(out);
+      const T* const from = static_cast<const T*>(x);
+      T* const to = static_cast<T*>(out);
       if (n == 1 || (stride == width && out_stride == width)) {
         constexpr int E = DROPOUT_UNIT<T>;
         const size_t elements = n * width, blocks = (elements + BLOCK * E - 1) / (BLOCK * E);
-        const unsigned grid = unsigned(blocks < MAX_GRID ? blocks : MAX_GRID);
-        if (bits % (sizeof(Pack<T, E>) < 16 ? sizeof(Pack<T, E>) : 16) == 0)
-          dropoutFlatKernel<T, true><<<grid, BLOCK, 0, s>>>(static_cast<const T*>(x), elements, static_cast<T*>(out), d);
-        else
-          dropoutFlatKernel<T, false><<<grid, BLOCK, 0, s>>>(static_cast<const T*>(x), elements, static_cast<T*>(out), d);
+        const bool vec = bits % (sizeof(Pack<T, E>) < 16 ? sizeof(Pack<T, E>) : 16) == 0;
+        launch("dropout", vec ? dropoutFlatKernel<T, true> : dropoutFlatKernel<T, false>, unsigned(blocks < MAX_GRID ? blocks : MAX_GRID), BLOCK, 0, stream, from,
+               elements, to, d);
       } else {
         const RowShape shape = rowShape(n, (width + 3) / 4, 1);
-        if (((width | stride | out_stride) % 4 | bits % (4 * sizeof(T) < 16 ? 4 * sizeof(T) : 16)) == 0)
-          dropoutRowsKernel<T, true><<<tileGrid(shape.tiles), BLOCK, 0, s>>>(static_cast<const T*>(x), n, width, stride, static_cast<T*>(out), out_stride, shape, d);
-        else
-          dropoutRowsKernel<T, false><<<tileGrid(shape.tiles), BLOCK, 0, s>>>(static_cast<const T*>(x), n, width, stride, static_cast<T*>(out), out_stride, shape, d);
+        const bool vec = ((width | stride | out_stride) % 4 | bits % (4 * sizeof(T) < 16 ? 4 * sizeof(T) : 16)) == 0;
+        launch("dropout", vec ? dropoutRowsKernel<T, true> : dropoutRowsKernel<T, false>, tileGrid(shape.tiles), BLOCK, 0, stream, from, n, width, stride, to,
+               out_stride, shape, d);
       }
     });
-    launched("dropout");
   });
 }
 

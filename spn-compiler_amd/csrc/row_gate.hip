@@ -402,7 +402,7 @@ extern "C" {
 
 int spnc_hip_gate(const void* logits, int dtype, size_t n, unsigned experts, size_t stride, unsigned k, unsigned flags, int32_t* index,
                   void* weight, void* stream) {
-  return launching([&] {
+  return guarded([&] {
     checkGate(dtype, n, experts, stride, k, flags);
     if (n == 0) return;
     if (!logits || !index || !weight) refuse("null argument");
@@ -416,17 +416,16 @@ int spnc_hip_gate(const void* logits, int dtype, size_t n, unsigned experts, siz
       using T = decltype(t);
       withGateShape<T>(n, experts, k, stride, address(logits), [&](auto g, auto v, auto layout) {
         constexpr int G = decltype(g)::value, V = decltype(v)::value;
-        gateKernel<T, G, V, decltype(layout)::value><<<tileGrid((n + BLOCK / G - 1) / (BLOCK / G)), BLOCK, 0, static_cast<hipStream_t>(stream)>>>(
-            static_cast<const T*>(logits), n, experts, stride, k, flags, index, static_cast<wide_t<T>*>(weight));
+        launch("gate", gateKernel<T, G, V, decltype(layout)::value>, tileGrid((n + BLOCK / G - 1) / (BLOCK / G)), BLOCK, 0, stream,
+               static_cast<const T*>(logits), n, experts, stride, k, flags, index, static_cast<wide_t<T>*>(weight));
       });
     });
-    launched("gate");
   });
 }
 
 int spnc_hip_gate_backward(const void* logits, int dtype, size_t n, unsigned experts, size_t stride, unsigned k, unsigned flags,
                            const int32_t* index, const void* weight, const void* grad_weight, void* grad_logits, void* stream) {
-  return launching([&] {
+  return guarded([&] {
     checkGate(dtype, n, experts, stride, k, flags);
     if (n == 0) return;
     if ((!logits && (flags & SPNC_HIP_GATE_ALL)) || !index || !weight || !grad_weight || !grad_logits) refuse("null argument");
@@ -441,12 +440,11 @@ int spnc_hip_gate_backward(const void* logits, int dtype, size_t n, unsigned exp
       withGateShape<T>(n, experts, k, (flags & SPNC_HIP_GATE_ALL) ? stride : experts,
                        address(grad_logits) | ((flags & SPNC_HIP_GATE_ALL) ? address(logits) : 0), [&](auto g, auto v, auto layout) {
         constexpr int G = decltype(g)::value, V = decltype(v)::value;
-        gateBackwardKernel<T, G, V, decltype(layout)::value><<<tileGrid((n + BLOCK / G - 1) / (BLOCK / G)), BLOCK, 0, static_cast<hipStream_t>(stream)>>>(
-            static_cast<const T*>(logits), n, experts, stride, k, flags, index, static_cast<const R*>(weight), static_cast<const R*>(grad_weight),
-            static_cast<T*>(grad_logits));
+        launch("gate gradient", gateBackwardKernel<T, G, V, decltype(layout)::value>, tileGrid((n + BLOCK / G - 1) / (BLOCK / G)), BLOCK, 0, stream,
+               static_cast<const T*>(logits), n, experts, stride, k, flags, index, static_cast<const R*>(weight), static_cast<const R*>(grad_weight),
+               static_cast<T*>(grad_logits));
       });
     });
-    launched("gate gradient");
   });
 }
 

@@ -740,7 +740,7 @@ size_t spnc_hip_route_workspace(size_t slots, unsigned experts) {
 
 int spnc_hip_route(const int32_t* index, size_t slots, unsigned experts, unsigned align, int32_t* position, int32_t* starts, int32_t* counts,
                    void* workspace, size_t workspace_bytes, void* stream) {
-  return launching([&] {
+  return guarded([&] {
     checkExperts(experts);
     if (align == 0) refuse("align must be at least 1");
     if (slots >= (size_t(1) << 31) || slots + size_t(experts) * (align - 1) >= (size_t(1) << 31))
@@ -758,29 +758,23 @@ int spnc_hip_route(const int32_t* index, size_t slots, unsigned experts, unsigne
     checkApart("route", scratch, {read});
     unsigned bits = 0;
     while ((1u << bits) < experts) ++bits;
-    const hipStream_t s = static_cast<hipStream_t>(stream);
     const size_t lds = ROUTE_WAVES * experts * sizeof(uint32_t);
     withItems(shape.items, [&](auto items) {
       constexpr int ITEMS = decltype(items)::value;
       if (lds > 48 * 1024)
-        for (const void* kernel : {reinterpret_cast<const void*>(routeCountKernel<ITEMS>), reinterpret_cast<const void*>(routeKernel<ITEMS>)}) {
-          const hipError_t e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, int(lds));
-          if (e != hipSuccess) refuse(std::string("route: ") + hipGetErrorString(e));
-        }
-      if (shape.blocks > 1) {
-        routeCountKernel<ITEMS><<<shape.blocks, ROUTE_BLOCK, lds, s>>>(index, slots, experts, shape.chunk, static_cast<uint32_t*>(workspace));
-        launched("route");
-      }
-      routeKernel<ITEMS><<<shape.blocks, ROUTE_BLOCK, lds, s>>>(index, slots, experts, bits, align, shape.chunk, static_cast<const uint32_t*>(workspace),
-                                                              position, starts, counts);
+        for (const void* kernel : {reinterpret_cast<const void*>(routeCountKernel<ITEMS>), reinterpret_cast<const void*>(routeKernel<ITEMS>)})
+          checkCall("route", hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, int(lds)));
+      if (shape.blocks > 1)
+        launch("route", routeCountKernel<ITEMS>, shape.blocks, ROUTE_BLOCK, lds, stream, index, slots, experts, shape.chunk, static_cast<uint32_t*>(workspace));
+      launch("route", routeKernel<ITEMS>, shape.blocks, ROUTE_BLOCK, lds, stream, index, slots, experts, bits, align, shape.chunk,
+             static_cast<const uint32_t*>(workspace), position, starts, counts);
     });
-    launched("route");
   });
 }
 
 int spnc_hip_dispatch(const void* rows, size_t n, size_t row_bytes, size_t stride_bytes, const int32_t* position, unsigned k, size_t capacity,
                       const int32_t* starts, const int32_t* counts, unsigned experts, int zero_unused, void* out, void* stream) {
-  return launching([&] {
+  return guarded([&] {
     checkSlots(n, k, capacity);
     if (row_bytes >> 31) refuse("a row must be shorter than 2 GiB");
     if (zero_unused) checkSegments(starts, counts, experts);
@@ -789,7 +783,6 @@ int spnc_hip_dispatch(const void* rows, size_t n, size_t row_bytes, size_t strid
     if (!zero_unused) experts = 0;  // the segments are not read
     checkApart("dispatch", block(out, capacity * row_bytes),
                {{rows, n, row_bytes, stride_bytes}, block(position, n * k * sizeof(int32_t)), startsBlock(starts, experts), countsBlock(counts, experts)});
-    const hipStream_t s = static_cast<hipStream_t>(stream);
     const unsigned piece = pieceBytes(1, {address(rows), address(out), row_bytes, stride_bytes});
     const RowShape shape = rowShape(n, row_bytes, piece, out, n < FEW_ROWS ? 8 : 6);
     const Unused unused = unusedRows(tileGrid(shape.tiles), starts, counts, experts, capacity, row_bytes, zero_unused ? out : nullptr);
@@ -798,19 +791,18 @@ int spnc_hip_dispatch(const void* rows, size_t n, size_t row_bytes, size_t strid
       using P = decltype(p);
       withChoices(k, [&](auto kb, auto) {
         constexpr int KB = decltype(kb)::value;
-        withStream<sizeof(P)>(shape, [&](auto stream) {
-          dispatchKernel<P, KB, decltype(stream)::value><<<unused.rowBlocks + unused.blocks, BLOCK, 0, s>>>(
-              static_cast<const unsigned char*>(rows), n, stride_bytes, shape, position, k, capacity, static_cast<P*>(out), unused);
+        withStream<sizeof(P)>(shape, [&](auto past) {
+          launch("dispatch", dispatchKernel<P, KB, decltype(past)::value>, unused.rowBlocks + unused.blocks, BLOCK, 0, stream,
+                 static_cast<const unsigned char*>(rows), n, stride_bytes, shape, position, k, capacity, static_cast<P*>(out), unused);
         });
       });
     });
-    launched("dispatch");
   });
 }
 
 int spnc_hip_combine(const void* values, int dtype, size_t capacity, size_t width, size_t stride, const int32_t* position, size_t n, unsigned k,
                      const void* weight, int weight_dtype, void* out, void* stream) {
-  return launching([&] {
+  return guarded([&] {
     const size_t bytes = elementBytes(dtype);
     checkSlots(n, k, capacity);
     if (weight) checkWeightType(dtype, weight_dtype);
@@ -831,30 +823,27 @@ int spnc_hip_combine(const void* values, int dtype, size_t capacity, size_t widt
         withWeight<T>(weight_dtype, [&](auto w) {
           using W = decltype(w);
           withChoices(k, [&](auto kb, auto one) {
-            auto launch = [&](auto weighted) {
-              combineKernel<T, N, W, decltype(kb)::value, decltype(one)::value, decltype(weighted)::value>
-                  <<<tileGrid(shape.tiles), BLOCK, 0, static_cast<hipStream_t>(stream)>>>(
-                      static_cast<const T*>(values), capacity, stride, shape, position, n, k, static_cast<const W*>(weight), static_cast<Pack<T, N>*>(out));
-            };
-            weight ? launch(std::true_type()) : launch(std::false_type());
+            launch("combine",
+                   weight ? combineKernel<T, N, W, decltype(kb)::value, decltype(one)::value, true>
+                          : combineKernel<T, N, W, decltype(kb)::value, decltype(one)::value, false>,
+                   tileGrid(shape.tiles), BLOCK, 0, stream, static_cast<const T*>(values), capacity, stride, shape, position, n, k,
+                   static_cast<const W*>(weight), static_cast<Pack<T, N>*>(out));
           });
         });
       });
     });
-    launched("combine");
   });
 }
 
 int spnc_hip_combine_backward(const void* values, int dtype, size_t capacity, size_t width, size_t stride, const int32_t* position, size_t n,
                               unsigned k, const void* weight, int weight_dtype, const void* grad_out, size_t grad_stride, const int32_t* starts,
                               const int32_t* counts, unsigned experts, void* grad_values, void* grad_weight, void* stream) {
-  return launching([&] {
+  return guarded([&] {
     const size_t bytes = elementBytes(dtype);
     checkSlots(n, k, capacity);
     checkWeightType(dtype, weight_dtype);
     if (width >> 31 || width * bytes >> 31) refuse("a row must be shorter than 2 GiB");
     if (grad_values) checkSegments(starts, counts, experts);
-    const hipStream_t s = static_cast<hipStream_t>(stream);
     if (!grad_values && !grad_weight) return;
     if (n && ((capacity && width && !values) || !position || !weight || (width && !grad_out))) refuse("null argument");
     const unsigned piece = pieceBytes(unsigned(bytes), {address(values), address(grad_out), address(grad_values), width * bytes, stride * bytes,
@@ -878,21 +867,20 @@ int spnc_hip_combine_backward(const void* values, int dtype, size_t capacity, si
           using W = decltype(w);
           withChoices(k, [&](auto kb, auto) {
             withStream<sizeof(T) * N>(shape, [&](auto past) {
-              combineBackwardKernel<T, N, W, decltype(kb)::value, decltype(past)::value><<<unused.rowBlocks + unused.blocks, BLOCK, 0, s>>>(
-                  static_cast<const T*>(values), capacity, stride, shape, position, n, k, static_cast<const W*>(weight),
-                  static_cast<const T*>(grad_out), grad_stride, static_cast<Pack<T, N>*>(grad_values), static_cast<W*>(grad_weight), unused);
+              launch("combine gradient", combineBackwardKernel<T, N, W, decltype(kb)::value, decltype(past)::value>, unused.rowBlocks + unused.blocks,
+                     BLOCK, 0, stream, static_cast<const T*>(values), capacity, stride, shape, position, n, k, static_cast<const W*>(weight),
+                     static_cast<const T*>(grad_out), grad_stride, static_cast<Pack<T, N>*>(grad_values), static_cast<W*>(grad_weight), unused);
             });
           });
         });
       });
     });
-    launched("combine gradient");
   });
 }
 
 int spnc_hip_combine_log(const void* values, int dtype, size_t capacity, const int32_t* position, size_t n, unsigned k, const void* log_weight,
                          int weight_dtype, void* out, void* share, void* stream) {
-  return launching([&] {
+  return guarded([&] {
     checkLogTypes(dtype, weight_dtype);
     checkSlots(n, k, capacity);
     if (n == 0) return;
@@ -903,7 +891,6 @@ int spnc_hip_combine_log(const void* values, int dtype, size_t capacity, const i
     checkApart("combine_log", block(out, n * bytes), {read, slots, weights, shares});
     checkApart("combine_log", shares, {read, slots, weights});
     if (capacity == 0) values = out;  // no slot is routed; there has to be a value to read and drop
-    const hipStream_t s = static_cast<hipStream_t>(stream);
     withLogTypes(dtype, weight_dtype, [&](auto r, auto w) {
       using R = decltype(r);
       using W = decltype(w);
@@ -911,26 +898,24 @@ int spnc_hip_combine_log(const void* values, int dtype, size_t capacity, const i
       withLogChoices<Widest>(k, address(position) | address(log_weight) | address(share), [&](auto kb, auto exact) {
         constexpr int K = decltype(kb)::value;
         if constexpr (K > 0)
-          combineLogKernel<R, W, K, decltype(exact)::value><<<logGrid(n, k), BLOCK, 0, s>>>(
-              static_cast<const R*>(values), capacity, position, static_cast<const W*>(log_weight), n, k, static_cast<R*>(out), static_cast<R*>(share));
+          launch("combine_log", combineLogKernel<R, W, K, decltype(exact)::value>, logGrid(n, k), BLOCK, 0, stream, static_cast<const R*>(values), capacity,
+                 position, static_cast<const W*>(log_weight), n, k, static_cast<R*>(out), static_cast<R*>(share));
         else
-          combineLogManyKernel<R, W><<<logGrid(n, k), BLOCK, 0, s>>>(
-              LogSlots<R, W>{static_cast<const R*>(values), capacity, position, static_cast<const W*>(log_weight), k}, n, static_cast<R*>(out),
-              static_cast<R*>(share));
+          launch("combine_log", combineLogManyKernel<R, W>, logGrid(n, k), BLOCK, 0, stream,
+                 LogSlots<R, W>{static_cast<const R*>(values), capacity, position, static_cast<const W*>(log_weight), k}, n, static_cast<R*>(out),
+                 static_cast<R*>(share));
       });
     });
-    launched("combine_log");
   });
 }
 
 int spnc_hip_combine_log_backward(const void* share, int dtype, size_t capacity, const int32_t* position, size_t n, unsigned k, int weight_dtype,
                                   const void* grad_out, const int32_t* starts, const int32_t* counts, unsigned experts, void* grad_values,
                                   void* grad_log_weight, void* stream) {
-  return launching([&] {
+  return guarded([&] {
     checkLogTypes(dtype, weight_dtype);
     checkSlots(n, k, capacity);
     if (grad_values) checkSegments(starts, counts, experts);
-    const hipStream_t s = static_cast<hipStream_t>(stream);
     if (!grad_values && !grad_log_weight) return;
     if (n && (!share || (grad_values && !position) || !grad_out)) refuse("null argument");
     const size_t bytes = elementBytes(dtype);
@@ -948,16 +933,14 @@ int spnc_hip_combine_log_backward(const void* share, int dtype, size_t capacity,
       withLogChoices<Widest>(k, address(share) | address(grad_log_weight) | (grad_values ? address(position) : 0), [&](auto kb, auto exact) {
         constexpr int K = decltype(kb)::value;
         if constexpr (K > 0)
-          combineLogBackwardKernel<R, W, K, decltype(exact)::value><<<unused.rowBlocks + unused.blocks, BLOCK, 0, s>>>(
-              static_cast<const R*>(share), position, n, k, capacity, static_cast<const R*>(grad_out), static_cast<R*>(grad_values),
-              static_cast<W*>(grad_log_weight), unused);
+          launch("combine_log gradient", combineLogBackwardKernel<R, W, K, decltype(exact)::value>, unused.rowBlocks + unused.blocks, BLOCK, 0, stream,
+                 static_cast<const R*>(share), position, n, k, capacity, static_cast<const R*>(grad_out), static_cast<R*>(grad_values),
+                 static_cast<W*>(grad_log_weight), unused);
         else
-          combineLogManyBackwardKernel<R, W><<<unused.rowBlocks + unused.blocks, BLOCK, 0, s>>>(
-              static_cast<const R*>(share), position, n, k, capacity, static_cast<const R*>(grad_out), static_cast<R*>(grad_values),
-              static_cast<W*>(grad_log_weight), unused);
+          launch("combine_log gradient", combineLogManyBackwardKernel<R, W>, unused.rowBlocks + unused.blocks, BLOCK, 0, stream, static_cast<const R*>(share),
+                 position, n, k, capacity, static_cast<const R*>(grad_out), static_cast<R*>(grad_values), static_cast<W*>(grad_log_weight), unused);
       });
     });
-    launched("combine_log gradient");
   });
 }
 

@@ -26,7 +26,13 @@ void refuse(bool condition, const Args&... args) {
   if (C10_UNLIKELY(condition)) throw std::runtime_error(c10::str(args...));
 }
 
-void check(int rc) { refuse(rc != 0, spnc_hip_last_error()); }
+// Behind the C-ABI an error that an earlier, foreign call left behind is not touched. PyTorch would raise it from whichever operation comes
+// next; here, where the call it belongs to can still be guessed, it is told as a warning.
+void check(int rc) {
+  refuse(rc != 0, spnc_hip_last_error());
+  if (C10_LIKELY(hipPeekAtLastError() == hipSuccess)) return;
+  TORCH_WARN("a HIP call before this one of spnc.mixture left an error behind: ", hipGetErrorString(hipGetLastError()));
+}
 
 int elementType(at::ScalarType t) {
   switch (t) {

@@ -363,3 +363,64 @@ def test_tangents_of_gradients_are_refused(mix):
         for transform in (lambda: torch.vmap(f)(t[None]), lambda: torch.func.grad(lambda a: f(a).sum())(t), lambda: torch.func.jvp(f, (t,), (torch.ones_like(t),))):
             with pytest.raises(RuntimeError):
                 transform()
+
+
+# ---- errors of other calls ------------------------------------------------------------------------------------------
+
+def _runtime():
+    torch = _torch()
+    return ctypes.CDLL(os.path.join(os.path.dirname(torch.__file__), "lib", "libamdhip64.so"))        # the runtime both use
+
+
+@pytest.mark.gpu
+def test_c_entry_points_leave_a_foreign_error_to_its_reader(native):
+    """A failed call (a device that does not exist) before each entry point: they succeed, and its code can still be read afterwards."""
+    torch = _torch()
+    from spnc import mixture as m
+    lib, p, hip = native._load(), ctypes.c_void_p, _runtime()
+    z, x = torch.randn(5, 7, device="cuda"), torch.randn(5, 4, device="cuda")
+    index, weight = m.gate(z, 2)
+    plan = m.route(index, 7)
+    rows, logs, lls = m.dispatch(x, plan), weight.log(), torch.randn(10, device="cuda")
+    joined, mixed = m.combine(rows, plan, weight), m.combine_log(lls, plan, logs)
+    dropped = m.dropout(x, 0.5, 3)
+    outs = [torch.empty_like(t) for t in (index, weight, z, plan.position, plan.starts, plan.counts, rows, joined, rows, weight, mixed, weight, lls, logs, dropped)]
+    gi, gw, gz, rp, rs, rc, dr, cj, cv, cw, lm, ls, lv, lw, do = outs
+    at = lambda t: p(t.data_ptr())
+    stream = p(torch.cuda.current_stream().cuda_stream)
+    calls = [lambda: lib.spnc_hip_gate(at(z), 0, 5, 7, 7, 2, 0, at(gi), at(gw), stream),
+             lambda: lib.spnc_hip_gate_backward(at(z), 0, 5, 7, 7, 2, 0, at(index), at(weight), at(weight), at(gz), stream),
+             lambda: lib.spnc_hip_route(at(index), 10, 7, 1, at(rp), at(rs), at(rc), None, 0, stream),
+             lambda: lib.spnc_hip_dispatch(at(x), 5, 16, 16, at(plan.position), 2, 10, at(plan.starts), at(plan.counts), 7, 1, at(dr), stream),
+             lambda: lib.spnc_hip_combine(at(rows), 0, 10, 4, 4, at(plan.position), 5, 2, at(weight), 0, at(cj), stream),
+             lambda: lib.spnc_hip_combine_backward(at(rows), 0, 10, 4, 4, at(plan.position), 5, 2, at(weight), 0, at(joined), 4, at(plan.starts), at(plan.counts), 7,
+                                                   at(cv), at(cw), stream),
+             lambda: lib.spnc_hip_combine_log(at(lls), 0, 10, at(plan.position), 5, 2, at(logs), 0, at(lm), at(ls), stream),
+             lambda: lib.spnc_hip_combine_log_backward(at(ls), 0, 10, at(plan.position), 5, 2, 0, at(mixed), at(plan.starts), at(plan.counts), 7, at(lv), at(lw), stream),
+             lambda: lib.spnc_hip_dropout(at(x), 0, 5, 4, 4, at(do), 4, 0.5, 0, 3, 0, None, stream)]
+    torch.cuda.synchronize()
+    for call in calls:
+        assert hip.hipSetDevice(ctypes.c_int(9999)) != 0
+        left = hip.hipPeekAtLastError()
+        assert left != 0 and call() == 0
+        assert hip.hipGetLastError() == left and hip.hipPeekAtLastError() == 0
+    for got, want in ((gi, index), (gw, weight), (rp, plan.position), (rs, plan.starts), (rc, plan.counts), (dr, rows), (cj, joined), (lm, mixed), (do, dropped)):
+        assert torch.equal(got, want)
+
+
+@pytest.mark.gpu
+def test_python_calls_tell_of_a_foreign_error(native, capfd):
+    """PyTorch raises whatever error it finds at its next launch; the call says where it was found and goes on."""
+    torch = _torch()
+    from spnc import mixture as m
+    z, hip = torch.randn(4, 6, device="cuda"), _runtime()
+    want = m.gate(z, 2)
+    torch.cuda.synchronize()
+    capfd.readouterr()
+    assert hip.hipSetDevice(ctypes.c_int(9999)) != 0
+    got = m.gate(z, 2)
+    assert hip.hipPeekAtLastError() == 0
+    assert "left an error behind: invalid device ordinal" in capfd.readouterr().err
+    m.gate(z, 2)
+    assert "left an error" not in capfd.readouterr().err
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
