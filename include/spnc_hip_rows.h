@@ -58,7 +58,7 @@ SPNC_HIP_API int spnc_hip_route(const int32_t* index, size_t slots, unsigned exp
 /* out[position[i * k + j]] = rows[i] for all slots with 0 <= position < capacity: rows of row_bytes bytes, stride_bytes apart in `rows`,
  * contiguous in `out` [capacity]. zero_unused != 0 clears the rows of `out` that belong to no segment (starts and counts
  * as spnc_hip_route wrote them); otherwise they are left as they were and starts and counts may be NULL. A row is shorter
- * than 2 GiB, here and below. */
+ * than 2 GiB, n * k and the capacity are below 2^31, here and below. */
 SPNC_HIP_API int spnc_hip_dispatch(const void* rows, size_t n, size_t row_bytes, size_t stride_bytes, const int32_t* position, unsigned k,
                                    size_t capacity, const int32_t* starts, const int32_t* counts, unsigned experts, int zero_unused, void* out,
                                    void* stream);

@@ -620,7 +620,7 @@ void withItems(unsigned items, Fn&& fn) {
 
 void checkSlots(size_t n, unsigned k, size_t capacity) {
   if (k == 0) refuse("k must be at least 1");
-  if (n > (size_t(1) << 31) / k) refuse("too many slots: n * k must be below 2^31");
+  if (n > ((size_t(1) << 31) - 1) / k) refuse("too many slots: n * k must be below 2^31");
   if (capacity >= (size_t(1) << 31)) refuse("too many rows: the capacity must be below 2^31");
 }
 

@@ -424,3 +424,19 @@ def test_python_calls_tell_of_a_foreign_error(native, capfd):
     m.gate(z, 2)
     assert "left an error" not in capfd.readouterr().err
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+# ---- limits ---------------------------------------------------------------------------------------------------------
+
+def test_slots_must_be_below_two_to_the_31(native):
+    """n * k of exactly 2^31 is refused by everything that takes slots, as the message says; before anything reaches the GPU."""
+    lib, p = native._load(), [ctypes.c_void_p(i << 40) for i in range(1, 9)]
+    for n, k in ((1 << 31, 1), (1 << 30, 2), (1 << 28, 8), (715827883, 3)):
+        _refused(lib, lib.spnc_hip_dispatch(p[0], n, 4, 4, p[1], k, 4, None, None, 0, 0, p[2], None), "n * k must be below 2^31")
+        _refused(lib, lib.spnc_hip_combine(p[0], 0, 4, 4, 4, p[1], n, k, p[2], 0, p[3], None), "n * k must be below 2^31")
+        _refused(lib, lib.spnc_hip_combine_backward(p[0], 0, 4, 4, 4, p[1], n, k, p[2], 0, p[3], 4, None, None, 0, None, p[4], None), "n * k must be below 2^31")
+        _refused(lib, lib.spnc_hip_combine_log(p[0], 0, 4, p[1], n, k, p[2], 0, p[3], None, None), "n * k must be below 2^31")
+        _refused(lib, lib.spnc_hip_combine_log_backward(p[0], 0, 4, p[1], n, k, 0, p[2], None, None, 0, None, p[3], None), "n * k must be below 2^31")
+    # one fewer is no such error: the capacity is the next check
+    for n, k in (((1 << 31) - 1, 1), ((1 << 30) - 1, 2), (715827882, 3)):
+        _refused(lib, lib.spnc_hip_dispatch(p[0], n, 4, 4, p[1], k, 1 << 31, None, None, 0, 0, p[2], None), "the capacity must be below 2^31")
