@@ -64,9 +64,9 @@ inline unsigned tileGrid(size_t tiles) {
 // A group of 2^shift lanes, a wave or with few rows up to a block, handles a row, a piece of up to 16 bytes a lane at a time.
 //
 // Rows that are written to scattered places bypass the caches where they consist of whole 64-byte halves of cache lines: 1 M rows
-// of 64 bytes to two places each take 36 us instead of 50, of 2 KB to four places 52 instead of 67 (a consumer that reads
-// them next loses up to half of that where they would have fit the last-level cache). Rows that share their halves must not: 48
-// bytes take 87 us instead of 61, since each piece goes to memory by itself.
+// of 64 bytes to two places each take 36 us instead of 53, 32769 of 2 KB to four places 53 instead of 65 (a consumer that reads
+// them next loses up to half of that where they would have fit the last-level cache). Rows that share their halves must not: 1 M of 48
+// bytes to two places take 70 us instead of 53, since each piece goes to memory by itself.
 struct RowShape {
   unsigned pieces;  // of a row
   unsigned shift;
@@ -82,8 +82,8 @@ inline RowShape rowShape(size_t n, size_t rowBytes, unsigned pieceBytes, const v
   while (s.shift < most && (1u << s.shift) < s.pieces) ++s.shift;
   const size_t rows = BLOCK >> s.shift;
   s.tiles = (n + rows - 1) / rows;
-  // In the order of the blocks from 1 KB on: 4 x 32769 rows of 2 KB are combined in 59 us instead of 61. Of 8 bytes, 4 x 2 M rows take 32
-  // instead of 26 that way, of 24 bytes 78 instead of 67.
+  // In the order of the blocks from 1 KB on: 4 x 32769 rows of 2 KB are combined in 60 us instead of 63. 4 x 2 M rows of 8 bytes take 38
+  // instead of 37 that way, of 24 bytes 93 instead of 82, and to be dispatched 114 instead of 102.
   s.byDie = rowBytes < 1024;
   s.stream = pieceBytes == 16 && rowBytes % 64 == 0 && reinterpret_cast<uintptr_t>(scattered) % 64 == 0;
   return s;

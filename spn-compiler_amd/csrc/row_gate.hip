@@ -139,8 +139,9 @@ __device__ inline void gateInsert(uint32_t (&list)[4], uint32_t key) {
 
 // G lanes hold a row, V logits each, so the logits are read once. k rounds: the largest key of the group, the lowest expert that has it, and
 // out it goes; lane j keeps the choice of round j, and the softmax is computed by the lanes that have one. Bound by instructions: 262144
-// rows of 64 float32, four choices, take 18 us (76 MB, 4.3 TB/s), 65537 of 509 bfloat16, eight choices over all, 26 us (71 MB; 800
-// vector instructions a wave of four rows are 21 us of issue).
+// rows of 64 float32, four choices, take 17 us (76 MB, 4.4 TB/s), 65537 of 509 bfloat16, eight choices over all, 26 us (71 MB; 800
+// vector instructions a wave of four rows are 21 us of issue). Every round of float32 and float64 looks at all logits again, so the time grows with
+// experts times choices: 262144 rows of 128 float32, eight choices, take 47 us, of 256 93, twice what their bytes take.
 template <typename T, int G, int V, int LAYOUT>
 __global__ __launch_bounds__(BLOCK) void gateKernel(const T* __restrict__ logits, size_t n, unsigned experts, size_t stride, unsigned k,
                                                     unsigned flags, int32_t* __restrict__ index, wide_t<T>* __restrict__ weight) {
@@ -233,7 +234,7 @@ __global__ __launch_bounds__(BLOCK) void gateKernel(const T* __restrict__ logits
 
 // dz_e of the experts that were not chosen is 0, or -p_e times the sum over the slots under "all"; the k chosen ones get their
 // slot's term on top. A block's rows are one stretch of the output. It is put together in LDS, the chosen entries over the others,
-// and goes out 16 bytes a lane whatever the width of a row: 65537 rows of 509 bfloat16 take 30 us, 40 if every group
+// and goes out 16 bytes a lane whatever the width of a row: 65537 rows of 509 bfloat16 take 29 us, 40 if every group
 // writes its own row.
 template <typename T, int G, int V, int LAYOUT>
 __global__ __launch_bounds__(BLOCK) void gateBackwardKernel(const T* __restrict__ logits, size_t n, unsigned experts, size_t stride, unsigned k,

@@ -176,8 +176,8 @@ class Mixture:
 
     def _lanes(self, device):
         """The current stream and three others, made once a device. Segments are short and their kernels long chains that leave most of
-        the chip free: ten 16-feature kernels over 4096 rows take 141 us this way and 198 one after the other, over 1 M rows 291 and 347,
-        the wait for the segments' sizes included."""
+        the chip free: a call of ten 16-feature kernels over 4096 rows takes 211 us this way and 223 one after the other, over 1 M rows
+        384 and 428, the wait for the segments' sizes included; over 30 rows 220 and 191, since there the host's launches are all of it."""
         if device not in self._side:
             self._side[device] = [torch.cuda.Stream(device) for _ in range(3)]
         return [torch.cuda.current_stream(device)] + self._side[device]
