@@ -4,6 +4,7 @@
 // the backward pass runs on PyTorch's own thread.
 #include <ATen/MemoryOverlap.h>
 #include <c10/core/AutogradState.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -68,7 +69,8 @@ bool wantsGrad(std::initializer_list<const Tensor*> tensors) {
 void checkRecorded(std::initializer_list<const Tensor*> tensors) {
   using c10::impl::TorchDispatchModeKey;
   using c10::impl::TorchDispatchModeTLS;
-  refuse(torch::jit::tracer::isTracing() || (TorchDispatchModeTLS::any_modes_set() && TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY).has_value()),
+  refuse(torch::jit::tracer::isTracing() || c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch) ||
+             (TorchDispatchModeTLS::any_modes_set() && TorchDispatchModeTLS::get_mode(TorchDispatchModeKey::PROXY).has_value()),
          "spnc.mixture cannot be traced");
   if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
   for (const Tensor* t : tensors) refuse(t->defined() && t->_fw_grad(0).defined(), "spnc.mixture has no forward-mode derivatives");

@@ -9,8 +9,9 @@ compiled kernels; ``HIPCompiler.compile_mixture`` builds one.
 
 All take and return torch tensors on the GPU, run on the current stream, and have gradients where their inputs are
 floating point (first order: a gradient cannot be differentiated again; there are no forward-mode derivatives). Results do
-not change from run to run. Bad arguments raise ``RuntimeError``, and so do calls under ``torch.jit.trace`` or ``make_fx``, which
-would record nothing of them. An error that an earlier HIP call of the thread left unread is told as a warning. There is no CPU path.
+not change from run to run. Bad arguments raise ``RuntimeError``, and so do calls under ``torch.jit.trace``, ``make_fx`` or
+``torch.export``, which would record nothing of them. An error that an earlier HIP call of the thread left unread is told as a
+warning. There is no CPU path.
 """
 import math
 

@@ -337,6 +337,8 @@ def test_tangents_and_traces_are_refused(mix):
             torch.jit.trace(f, (t,))
         with pytest.raises(RuntimeError, match="cannot be traced"):
             make_fx(f, tracing_mode="real")(t)
+        with pytest.raises(RuntimeError, match="cannot be traced"):
+            make_fx(f, tracing_mode="real", pre_dispatch=True)(t)              # as torch.export records
     index = torch.zeros(3, 1, dtype=torch.int32)
     with pytest.raises(RuntimeError, match="cannot be traced"):
         torch.jit.trace(lambda t: m.route(t, 2).position, (index,))
